@@ -218,6 +218,100 @@ int momoe_bias_update(float* biases_N, const int64_t* sizes_N, int32_t N, int32_
                       momoe_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------------------
+ * Operators around the expert layer (no counterpart in the reference).
+ *
+ * Types: 0 bf16, 1 fp16, 2 fp32.  Strides count elements and are multiples of 8; rows start on 16-byte boundaries and
+ * their columns are contiguous.
+ *
+ * 8-bit rows: e4m3 values q[r, c] and one e8m0 byte for each 128 columns of a row; the value is q * 2^(byte - 127), with
+ * the smallest power of two for which max|x| <= 448 * 2^e (byte 127 for a block of zeros, byte 255, NaN, for a block
+ * that holds an infinity or a NaN).  Token-major: bytes [rows, ceil(cols / 128)].  Expert-major: 512 bytes for each
+ * (128-row tile, 512 columns), [tile, ceil(cols / 512)], where row r, block b have byte
+ * (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/* r = round(x + residual), y = r / sqrt(mean(r^2) + eps) * weight, row by row of [M, D].
+ *   residual and r: both NULL (then r is x) or both non-NULL; r [M, D] contiguous, rounded to `type`
+ *   y [M, D] contiguous in `type`, or NULL;  q [M, D], scale [M, ceil(D / 128)]: y before its rounding as 8-bit rows, or
+ *   both NULL (one of y and q is needed);  rstd fp32 [M] or NULL: 1 / sqrt(mean(r^2) + eps)
+ *   weight [D] in `type` or fp32 (weight_type).  D a multiple of 8, at most 16384.  M = 0 does nothing. */
+int momoe_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                   int32_t type, int32_t weight_type, int32_t M, int32_t D, float eps, void* r, void* y, float* rstd,
+                   uint8_t* q, uint8_t* scale, momoe_stream_t stream);
+
+/* Backward of momoe_rms_norm.  gy [M, D]: gradient of y; gr [M, D] or NULL: gradient of r from elsewhere; r: what the
+ * forward pass wrote (x without a residual).  gx [M, D] = gradient of x and of the residual alike; gw [D] in
+ * weight_type, or NULL.  The workspace (16-byte aligned) is needed for gw only.  Sums run in a fixed order. */
+size_t momoe_rms_norm_backward_workspace_bytes(int32_t M, int32_t D);
+int momoe_rms_norm_backward(const void* gy, const void* gr, const void* r, int64_t r_stride, const void* weight,
+                            const float* rstd, int32_t type, int32_t weight_type, int32_t M, int32_t D, void* gx,
+                            void* gw, void* workspace, size_t workspace_bytes, momoe_stream_t stream);
+
+/* x [M, D] -> token-major 8-bit rows. */
+int momoe_quantize_rows(const void* x, int64_t x_stride, int32_t type, int32_t M, int32_t D, uint8_t* q, uint8_t* scale,
+                        momoe_stream_t stream);
+
+/* Balance loss and z-loss of a router, with per-expert counts.  logits [M, N] contiguous in bf16 or fp32; topk_idx_MK
+ * int32 [M, K], ids outside [0, N) are not counted.  The M rows are B sequences: sequence b is rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 (int32 [B + 1], ascending; rows outside are neither read nor counted), or, with cu_seqlens
+ * NULL, consecutive sequences of seq_len rows (the last may be shorter; B = ceil(M / seq_len)).  With p the softmax over
+ * the Ng = N - Ks gating logits, T_b a sequence's tokens, T all tokens and B' the sequences that are not empty:
+ *   loss = balance_coef / B' * sum_b sum_e [Ng / ((K - Ks) T_b) count[b, e]] [mean over b of p[., e]]
+ *        + z_coef / T * sum_t (log sum_e exp logit[t, e])^2
+ * loss fp32 [1]; counts_BN int64 [B, N]; grad_BN fp32 [B, N]: for the backward pass.  N <= 1024, B <= 65535.
+ * Deterministic.  Replaces nothing: the reference balances by bias only (momoe/sample_moe.py:64-66). */
+size_t momoe_balance_loss_workspace_bytes(int32_t M, int32_t N, int32_t B);
+int momoe_balance_loss(const void* logits_MN, int32_t type, const int32_t* topk_idx_MK, const int32_t* cu_seqlens,
+                       int32_t seq_len, int32_t M, int32_t N, int32_t K, int32_t Ks, int32_t B, float balance_coef,
+                       float z_coef, float* loss, int64_t* counts_BN, float* grad_BN, void* workspace,
+                       size_t workspace_bytes, momoe_stream_t stream);
+
+/* Gradient of the logits: G_logits = grad_loss[0] * dloss/dlogits (+ add_MN, if it is not NULL; it may be G_logits_MN
+ * itself), in the type of the logits; zero for shared experts and for rows outside every sequence. */
+int momoe_balance_loss_backward(const void* logits_MN, int32_t type, const int32_t* cu_seqlens, int32_t seq_len,
+                                const float* grad_BN, int32_t M, int32_t N, int32_t Ks, int32_t B, float z_coef,
+                                const float* grad_loss, const void* add_MN, void* G_logits_MN, momoe_stream_t stream);
+
+/* Weights W [N, Kd, groups * C] (bf16 or fp32) -> q e4m3 [N, groups * C, Kd] and one e8m0 byte for each 128 x 128 block,
+ * S [N, groups, ceil(C / 128), ceil(Kd / 128)].  Up/gate weights: Kd = D, groups = 2, C = H; down weights: Kd = H,
+ * groups = 1, C = D.  Kd a multiple of 16. */
+int momoe_fp8_quantize_weights(const void* W, int32_t type, int32_t N, int32_t Kd, int32_t groups, int32_t C, uint8_t* q,
+                               uint8_t* S, momoe_stream_t stream);
+
+/* Token-major rows -> expert-major 8-bit rows: x is bf16 [M, D] (x_scale NULL) or e4m3 [M, D] with scales
+ * [M, ceil(D / 128)].  Padding rows keep whatever the buffers held: no later kernel's real rows depend on them.  A token
+ * that names an expert twice sets *status to 203.  D and H multiples of 16. */
+int momoe_fp8_gather_rows(const momoe_plan_t* plan, const void* x, const uint8_t* x_scale, uint8_t* dst_sorted,
+                          uint8_t* dst_scale, momoe_stream_t stream);
+
+/* Up/gate GEMM + SwiGLU on 8-bit operands: a, b = x W1[e]^T (fp32), h = b sigmoid(b) a as 8-bit rows (rounded once, from
+ * fp32).  W1 [N, 2H, D], S1 [N, 2, ceil(H / 128), ceil(D / 128)].  The second form is for a few rows an expert. */
+int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const uint8_t* x_sorted, const uint8_t* x_scale,
+                        const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
+                        momoe_stream_t stream);
+int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const uint8_t* x_sorted, const uint8_t* x_scale,
+                               const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
+                               momoe_stream_t stream);
+
+/* Down GEMM on 8-bit operands: y_sorted[r, :] = bf16(w[r] * (h[r, :] W2[e]^T)).  W2 [N, D, H],
+ * S2 [N, ceil(D / 128), ceil(H / 128)]; y_sorted 32-byte aligned. */
+int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
+                         const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, momoe_stream_t stream);
+int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
+                                const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, momoe_stream_t stream);
+
+/* The whole forward pass of 8-bit experts from a compact routing: permutation, gather, up, down, combine, out of one
+ * workspace (256-byte aligned).  x as for momoe_fp8_gather_rows; y_MD bf16 [M, D]; sizes_N int64 [N].  Calls with at
+ * most decode_max_avg_rows * N (token, expert) pairs use the decode forms. */
+size_t momoe_fp8_experts_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t D, int32_t H);
+int momoe_fp8_experts_launches(int32_t M, int32_t N, int32_t K);
+int momoe_fp8_experts_forward(const void* x_MD, const uint8_t* x_scale, const int32_t* topk_idx_MK,
+                              const float* topk_w_MK, int32_t M, int32_t N, int32_t K, int32_t D, int32_t H,
+                              const uint8_t* W1_N2HD, const uint8_t* S1, const uint8_t* W2_NDH, const uint8_t* S2,
+                              int32_t decode_max_avg_rows, void* y_MD, int64_t* sizes_N, void* workspace,
+                              size_t workspace_bytes, int32_t* status, momoe_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------------------
  * Expert parallelism over peer memory (no counterpart in the reference, whose README lists expert parallelism as
  * unsupported).  R <= 8 ranks of one NVLink node, one process per GPU; rank r owns experts [r*N/R, (r+1)*N/R).
  * `peer_*` arguments are HOST arrays of R device pointers: entry p is rank p's buffer, mapped into this process

@@ -1,0 +1,109 @@
+// 8-bit rows: e4m3 values with one power of two (e8m0 byte, 2^(byte - 127)) for each block of 128.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+namespace momoe {
+
+constexpr int FP8_BLOCK = 128;          // values that share a scale
+constexpr int FP8_GROUP = 4;            // blocks whose scale bytes share a 32-bit word
+constexpr int FP8_ATOM = 512;           // bytes of the scales of 128 rows x 4 blocks
+
+// Scales of expert-major rows lie as the tensor core reads them: 512 bytes for each (128-row tile, 4 blocks of 128
+// columns), byte (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4.
+__host__ __device__ __forceinline__ size_t fp8_atom_offset(size_t row, int group, int n_groups) {
+    return ((row >> 7) * static_cast<size_t>(n_groups) + group) * FP8_ATOM + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+}
+
+// The byte of the smallest 2^e with amax <= 448 * 2^e, from the bit pattern of amax >= 0.  448 = 1.75 * 2^8, so this is
+// integer arithmetic and exact.  127 (a scale of 1) for a block of zeros; 255 (NaN) where the block holds an infinity or
+// a NaN, so that the block's products are NaN as they would be in 32 bits.  A power of two makes the division below
+// exact: the one rounding is the conversion to e4m3.
+__device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax_bits) {
+    if (amax_bits >= 0x7F800000u) return 255u;
+    if (amax_bits == 0u) return 127u;
+    const int b = static_cast<int>(amax_bits >> 23) - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return static_cast<uint32_t>(b < 0 ? 0 : b);
+}
+// 1 / scale (NaN for byte 255); byte is at most 247 otherwise.
+__device__ __forceinline__ float fp8_inv_scale(uint32_t byte) {
+    return byte == 255u ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float((254u - byte) << 23);
+}
+// Larger magnitude of two as bit patterns: orders infinities and NaN above every finite value.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
+__device__ __forceinline__ uint8_t fp8_one(float a) { return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3); }
+
+// Eight consecutive values of a row in 32 bits.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+template <>
+__device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+// Rounds the eight values to T, stores them and leaves the rounded values in v.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, float (&v)[8]);
+template <>
+__device__ __forceinline__ void store8<float>(float* p, float (&v)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <>
+__device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <>
+__device__ __forceinline__ void store8<__half>(__half* p, float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        const float2 f = __half22float2(h);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+}  // namespace momoe

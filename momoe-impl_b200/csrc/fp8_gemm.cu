@@ -1,0 +1,546 @@
+// The experts' two forward GEMMs on 8-bit rows and weights (e4m3, a power of two for each block of 128), sm_100a.
+//
+//   up    a = x W1[e][:H]^T, b = x W1[e][H:]^T, h = b sigmoid(b) a in 32 bits, h -> 8-bit rows (128 columns a scale)
+//   down  y[r, :] = bf16(row_weight[r] * (h W2[e]^T))
+//
+// Weights are K-major ([N, 2H, D] and [N, D, H]) with one scale for each 128 x 128 block.  All scales are powers of two,
+// so the tensor core applies them (kind::mxf8f6f4, block-scaled): accumulation is fp32 over the whole k axis and there is
+// no per-block pass over the accumulators, which fp32 scales would need.
+//
+// Tensor-bound at large row counts.  The structure is that of the 16-bit grouped GEMM: a CTA pair computes 256 x 256, each
+// CTA loads its 128 rows of A and half of B, ring of 3 stages of two 128-byte k slices (a slice is 128 values here), warp
+// 0 loads, warp 1 of the leader issues the MMAs, warps 2..9 are the epilogue.  What differs:
+//
+// Scales.  Warp 10 of each CTA fills a ring of four 1.5 KiB slots, each with the scales of four slices (512 k): one
+// 512-byte block for the CTA's 128 rows, copied as it lies in memory, and two for the 256 weight columns, one word each
+// repeated 128 times.  tcgen05.cp moves a slot to TMEM in front of the four slices' MMAs, which pick their byte of each
+// word through the scale ids of the instruction descriptor.  Two TMEM copies alternate; a copy is overwritten only after
+// the commit behind the MMAs that read it has arrived.
+//
+// TMEM.  Two accumulators of 256 columns and 24 columns of scales do not fit 512 columns, so the accumulators overlap: the
+// first takes columns 0..255, the second 224..479, the scales 480..503.  The epilogue reads the 32 shared columns of a
+// tile first and hands them back at once (`bar_ovl`), so the next tile's MMAs wait for an eighth of the read-out, not all.
+//
+// Padding rows hold anything: no row of a forward pass depends on another, and no consumer reads their results.
+#include <cstring>
+
+#include "fp8.cuh"
+#include "internal.h"
+#include "ptx.cuh"
+#include "../../include/momoe_b200.h"
+
+namespace momoe {
+
+constexpr int F8_EPI_WARPS = 8;
+constexpr int F8_THREADS = 32 * (3 + F8_EPI_WARPS);
+constexpr int F8_PAIR_N = 256;
+constexpr int F8_K = 128;                                 // values of a k slice (128 bytes)
+constexpr int F8_A_BYTES = TILE_M * F8_K;                 // 16 KiB
+constexpr int F8_B_BYTES = F8_PAIR_N / 2 * F8_K;          // 16 KiB
+constexpr int F8_SLICE_BYTES = F8_A_BYTES + F8_B_BYTES;
+constexpr int F8_STAGE_BYTES = 2 * F8_SLICE_BYTES;
+constexpr int F8_STAGES = 3;
+constexpr int F8_SF_SLOTS = 4;
+constexpr int F8_SF_BYTES = 3 * FP8_ATOM;
+constexpr int F8_EPI_BYTES = 2048;                        // staging of one epilogue warp: 32 rows x 64 bytes
+constexpr int F8_SMEM_BYTES =
+    F8_STAGES * F8_STAGE_BYTES + F8_SF_SLOTS * F8_SF_BYTES + F8_EPI_WARPS * F8_EPI_BYTES + 1024;
+constexpr int F8_ACC1 = 224;                              // first column of the second accumulator
+constexpr int F8_SF_COL = 480;
+constexpr int F8_SF_COLS = 12;                            // 4 for A, 8 for B
+
+struct Fp8Args {
+    const int* sched;
+    const int* tile_expert;
+    const int* pair_info;
+    int* status;
+    int n_nblk;                 // column blocks of 128 (up, both halves) or 256 (down)
+    int nkb;                    // k slices
+    int out_cols;               // H (up) or D (down)
+    const uint8_t* a_scale;     // blocks of 512 bytes, [tile, ceil(nkb / 4)]
+    const uint8_t* b_scale;     // up: [N, 2, n_nblk, nkb]; down: [N, ceil(D / 128), nkb]
+    int b_blocks;               // down: ceil(D / 128)
+    uint8_t* h_scale;           // up: scales of h, blocks of 512 bytes
+    const float* row_weight;    // down
+    __nv_bfloat16* y;           // down
+};
+
+__device__ __forceinline__ uint32_t f8_pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ float f8_swiglu(float a, float b) { return b * __fdividef(1.0f, 1.0f + __expf(-b)) * a; }
+
+struct Fp8Work {
+    int tile, nb, e;
+    bool valid;
+};
+__device__ __forceinline__ Fp8Work f8_work(const Fp8Args& g, int item, uint32_t cta_rank) {
+    Fp8Work w;
+    w.nb = item % g.n_nblk;
+    const int info = __ldg(g.pair_info + item / g.n_nblk);
+    w.tile = (info >> 1) + static_cast<int>(cta_rank);
+    w.valid = cta_rank == 0 || (info & 1) != 0;
+    w.e = __ldg(g.tile_expert + (info >> 1));
+    return w;
+}
+
+template <bool UP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8_THREADS, 1)
+fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                        const __grid_constant__ CUtensorMap tmO, const Fp8Args g) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bar_full[F8_STAGES];
+    __shared__ uint64_t bar_empty[F8_STAGES];
+    __shared__ uint64_t bar_sf_full[F8_SF_SLOTS];    // leader: both CTAs' scale warps have filled the slot
+    __shared__ uint64_t bar_sf_empty[F8_SF_SLOTS];   // both: the MMAs that use the slot's scales have completed
+    __shared__ uint64_t bar_acc_full[2];
+    __shared__ uint64_t bar_acc_empty[2];            // leader
+    __shared__ uint64_t bar_ovl;                     // leader: the shared columns of the latest tile have been read
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    __shared__ uint32_t s_top[UP ? 2 : 1][UP ? 2 : 1][UP ? TILE_M : 1];   // up: [accumulator][column half][row]
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t cta_rank = cluster_ctarank();
+    const bool leader = cta_rank == 0;
+    const int cluster_id = blockIdx.x >> 1;
+    const int n_clusters = gridDim.x >> 1;
+    const uint32_t stage_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sf_base = stage_base + F8_STAGES * F8_STAGE_BYTES;
+    const uint32_t epi_base = sf_base + F8_SF_SLOTS * F8_SF_BYTES;
+
+    const int total_items = __ldg(g.sched + SCHED_N_PAIRS) * g.n_nblk;
+    if (total_items <= 0 || cluster_id >= total_items) return;   // both CTAs of the cluster leave together
+    const int n_groups = (g.nkb + FP8_GROUP - 1) / FP8_GROUP;
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < F8_STAGES; ++s) {
+            mbar_init(smem_u32(&bar_full[s]), 1);
+            mbar_init(smem_u32(&bar_empty[s]), 1);
+        }
+        for (int s = 0; s < F8_SF_SLOTS; ++s) {
+            mbar_init(smem_u32(&bar_sf_full[s]), 2);
+            mbar_init(smem_u32(&bar_sf_empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&bar_acc_full[b]), 1);
+            mbar_init(smem_u32(&bar_acc_empty[b]), 2 * F8_EPI_WARPS);
+        }
+        mbar_init(smem_u32(&bar_ovl), F8_EPI_WARPS);   // four warps of each CTA read the shared columns
+        fence_mbar_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+        tma_prefetch_desc(&tmO);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(&tmem_slot), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
+    volatile int* abortp = &abort_flag;
+
+    if (warp == 0) {
+        // ================================================================ loads
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            const int r = static_cast<int>(cta_rank);
+            for (int item = cluster_id; ok && item < total_items; item += n_clusters) {
+                const Fp8Work w = f8_work(g, item, cta_rank);
+                for (int kb = 0; kb < g.nkb; kb += 2) {
+                    ok = mbar_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, abortp, g.status, DEV_TIMEOUT_PRODUCER);
+                    if (!ok) break;
+                    if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[stage]), 2 * F8_STAGE_BYTES);
+                    const uint32_t full = mapa_shared(smem_u32(&bar_full[stage]), 0);
+                    // tensor maps count in 16-bit units; a slice past the end of the k axis is zero-filled
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t sa = stage_base + stage * F8_STAGE_BYTES + h * F8_SLICE_BYTES;
+                        const int k0 = (kb + h) * (F8_K / 2);
+                        tma_load_2d_pair(sa, &tmA, full, k0, w.tile * TILE_M);
+                        // up: the leader loads 128 rows of the linear half of W1[e], its peer the matching gate rows
+                        if constexpr (UP) tma_load_3d_pair(sa + F8_A_BYTES, &tmB, full, k0, w.nb * 128, w.e * 2 + r);
+                        else tma_load_3d_pair(sa + F8_A_BYTES, &tmB, full, k0, w.nb * F8_PAIR_N + r * 128, w.e);
+                    }
+                    if (++stage == F8_STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ================================================================ MMAs (leader CTA only)
+        if (lane == 0 && leader) {
+            constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);   // SBO 1024, version 1, 128-byte swizzle
+            const uint32_t a_lo0 = ((stage_base >> 4) & 0x3FFFu) | (1u << 16);
+            constexpr uint32_t b_off = F8_A_BYTES >> 4;
+            int stage = 0;
+            uint32_t phase = 0;
+            uint32_t a_lo = a_lo0;
+            int it = 0, gi = 0;        // tiles and scale groups so far
+            bool ok = true;
+            for (int item = cluster_id; ok && item < total_items; item += n_clusters, ++it) {
+                const int ab = it & 1;
+                ok = mbar_wait(smem_u32(&bar_acc_empty[ab]), ((it >> 1) & 1u) ^ 1u, abortp, g.status, DEV_TIMEOUT_MMA);
+                if (ok && it > 0) ok = mbar_wait(smem_u32(&bar_ovl), (it - 1) & 1u, abortp, g.status, DEV_TIMEOUT_MMA);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t tmem_d = tmem_base + ab * F8_ACC1;
+                for (int grp = 0; ok && grp < n_groups; ++grp, ++gi) {
+                    const int slot = gi % F8_SF_SLOTS;
+                    const uint32_t sf = tmem_base + F8_SF_COL + (gi & 1) * F8_SF_COLS;
+                    ok = mbar_wait_cluster(smem_u32(&bar_sf_full[slot]), (gi / F8_SF_SLOTS) & 1u, abortp, g.status,
+                                           DEV_TIMEOUT_MMA);
+                    // the TMEM copy was last read by the MMAs of the group before the previous one
+                    if (ok && gi >= 2)
+                        ok = mbar_wait(smem_u32(&bar_sf_empty[(gi - 2) % F8_SF_SLOTS]), ((gi - 2) / F8_SF_SLOTS) & 1u,
+                                       abortp, g.status, DEV_TIMEOUT_MMA);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t sf_smem = sf_base + slot * F8_SF_BYTES;
+                    tmem_cp_scales_pair(sf, scales_smem_desc(sf_smem));
+                    tmem_cp_scales_pair(sf + 4, scales_smem_desc(sf_smem + FP8_ATOM));
+                    tmem_cp_scales_pair(sf + 8, scales_smem_desc(sf_smem + 2 * FP8_ATOM));
+                    const int kb0 = grp * FP8_GROUP;
+#pragma unroll
+                    for (int j = 0; j < FP8_GROUP; ++j) {
+                        if (kb0 + j < g.nkb) {
+                            if ((j & 1) == 0) {
+                                ok = ok && mbar_wait(smem_u32(&bar_full[stage]), phase, abortp, g.status, DEV_TIMEOUT_MMA);
+                                tc_fence_after();
+                            }
+                            if (ok) {
+                                const uint32_t idesc = umma_idesc_fp8(2 * TILE_M, F8_PAIR_N, j);
+                                const uint32_t lo = a_lo + (j & 1) * (F8_SLICE_BYTES >> 4);
+#pragma unroll
+                                for (uint32_t k = 0; k < 4; ++k)
+                                    umma_fp8_pair_lohi(tmem_d, lo + k * 2u, desc_hi, lo + b_off + k * 2u, desc_hi, idesc,
+                                                       sf, sf + 4, (kb0 + j + static_cast<int>(k)) != 0 ? 1u : 0u);
+                                if ((j & 1) == 1 || kb0 + j + 1 == g.nkb) {
+                                    umma_commit_pair(smem_u32(&bar_empty[stage]), 3);
+                                    a_lo += F8_STAGE_BYTES >> 4;
+                                    if (++stage == F8_STAGES) { stage = 0; phase ^= 1u; a_lo = a_lo0; }
+                                }
+                            }
+                        }
+                    }
+                    if (ok) umma_commit_pair(smem_u32(&bar_sf_empty[slot]), 3);
+                }
+                if (ok) umma_commit_pair(smem_u32(&bar_acc_full[ab]), 3);
+            }
+        }
+    } else if (warp == 2 + F8_EPI_WARPS) {
+        // ================================================================ scales (both CTAs, whole warp)
+        int slot = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const uint32_t full0 = mapa_shared(smem_u32(&bar_sf_full[0]), 0);
+        for (int item = cluster_id; ok && item < total_items; item += n_clusters) {
+            const Fp8Work w = f8_work(g, item, cta_rank);
+            const int tile = w.valid ? w.tile : w.tile - 1;     // a missing half reads its partner's scales
+            const uint4* src = reinterpret_cast<const uint4*>(g.a_scale + static_cast<size_t>(tile) * n_groups * FP8_ATOM);
+            // the two blocks of 128 weight columns of this item
+            const int i = (lane >> 2) & 1;
+            const uint8_t* bs;
+            bool have;
+            if constexpr (UP) {
+                bs = g.b_scale + ((static_cast<size_t>(w.e) * 2 + i) * g.n_nblk + w.nb) * g.nkb;
+                have = true;
+            } else {
+                bs = g.b_scale + (static_cast<size_t>(w.e) * g.b_blocks + w.nb * 2 + i) * g.nkb;
+                have = w.nb * 2 + i < g.b_blocks;
+            }
+            for (int grp = 0; grp < n_groups; ++grp) {
+                const uint4 a = __ldg(src + grp * 32 + lane);
+                const int kb = grp * FP8_GROUP + (lane & 3);
+                uint32_t word = have && kb < g.nkb ? __ldg(bs + kb) : 127u;
+                word <<= 8 * (lane & 3);
+                word |= __shfl_xor_sync(0xffffffffu, word, 1);
+                word |= __shfl_xor_sync(0xffffffffu, word, 2);
+                const uint32_t b0 = __shfl_sync(0xffffffffu, word, 0), b1 = __shfl_sync(0xffffffffu, word, 4);
+                int okw = 1;
+                if (lane == 0)
+                    okw = mbar_wait(smem_u32(&bar_sf_empty[slot]), phase ^ 1u, abortp, g.status, DEV_TIMEOUT_PRODUCER)
+                              ? 1 : 0;
+                okw = __shfl_sync(0xffffffffu, okw, 0);
+                if (okw == 0) { ok = false; break; }
+                const uint32_t dst = sf_base + slot * F8_SF_BYTES + lane * 16;
+                st_shared_v4(dst, a.x, a.y, a.z, a.w);
+                st_shared_v4(dst + FP8_ATOM, b0, b0, b0, b0);
+                st_shared_v4(dst + 2 * FP8_ATOM, b1, b1, b1, b1);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(full0 + static_cast<uint32_t>(slot * sizeof(uint64_t)));
+                if (++slot == F8_SF_SLOTS) { slot = 0; phase ^= 1u; }
+            }
+        }
+    } else {
+        // ================================================================ epilogue (warps 2..9, both CTAs)
+        const int q = warp & 3;
+        const int row = q * 32 + lane;
+        const int half = (warp - 2) >> 2;
+        const uint32_t acc_empty_leader = mapa_shared(smem_u32(&bar_acc_empty[0]), 0);
+        const uint32_t ovl_leader = mapa_shared(smem_u32(&bar_ovl), 0);
+        const uint32_t stage_area = epi_base + (warp - 2) * F8_EPI_BYTES;
+        int it = 0;
+        bool ok = true;
+        bool stored = false;
+        for (int item = cluster_id; ok && item < total_items; item += n_clusters, ++it) {
+            const Fp8Work w = f8_work(g, item, cta_rank);
+            const int ab = it & 1;
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + ab * F8_ACC1;
+            // the accumulator whose neighbour follows above shares its last 32 columns, the other one its first
+            const bool shares = ab == 0 ? half == 1 : half == 0;
+            auto hand_back_shared = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(ovl_leader);
+            };
+            auto hand_back_all = [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(acc_empty_leader + ab * static_cast<uint32_t>(sizeof(uint64_t)));
+            };
+            float wgt = 0.0f;
+            const size_t grow = static_cast<size_t>(w.tile) * TILE_M + row;
+            if constexpr (!UP) wgt = w.valid ? __ldg(g.row_weight + grow) : 0.0f;
+            ok = mbar_wait(smem_u32(&bar_acc_full[ab]), (it >> 1) & 1u, abortp, g.status, DEV_TIMEOUT_EPILOGUE) &&
+                 *abortp == 0;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
+                // the partner warp may be on its way into the meeting below: it must not wait for this one
+                if constexpr (UP) asm volatile("bar.arrive %0, 64;" ::"r"(1 + q) : "memory");
+                break;
+            }
+            tc_fence_after();
+            if constexpr (UP) {
+                // columns 32c .. 32c + 31 of the block, first the chunk that touches the shared columns
+                const int s0 = half;                     // position of the first chunk inside this warp's 64 columns
+                float h0[32], h1[32];
+                {
+                    uint32_t ra[32], rb[32];
+                    const int c = half * 2 + s0;
+                    tmem_ld32(taddr + c * 32, ra);
+                    tmem_ld32(taddr + 128 + c * 32, rb);
+                    tmem_ld_wait();
+                    if (shares) hand_back_shared();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) h0[i] = f8_swiglu(__uint_as_float(ra[i]), __uint_as_float(rb[i]));
+                    const int c1 = half * 2 + (s0 ^ 1);
+                    tmem_ld32(taddr + c1 * 32, ra);
+                    tmem_ld32(taddr + 128 + c1 * 32, rb);
+                    tmem_ld_wait();
+                    hand_back_all();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) h1[i] = f8_swiglu(__uint_as_float(ra[i]), __uint_as_float(rb[i]));
+                }
+                // columns past H have zero weights, so h is zero there and leaves the maximum alone
+                uint32_t top = 0u;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) top = max(top, max(abs_bits(h0[i]), abs_bits(h1[i])));
+                s_top[ab][half][row] = top;
+                // two warps share a row's 128 columns; s_top[ab] is written again two tiles later, after the partner has
+                // passed the next meeting, i.e. after it has read this one
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+                top = max(top, s_top[ab][half ^ 1][row]);
+                const uint32_t byte = fp8_scale_byte(top);
+                const float inv = fp8_inv_scale(byte);
+                const int col0 = w.nb * 128 + half * 64;
+                if (w.valid) {
+                    if (half == 0)
+                        g.h_scale[fp8_atom_offset(grow, w.nb >> 2, (g.n_nblk + 3) >> 2) + (w.nb & 3)] =
+                            static_cast<uint8_t>(byte);
+                    if (col0 < g.out_cols) {
+                        if (stored && lane == 0) bulk_wait_read<0>();
+                        __syncwarp();
+                        // [32 rows x 64 bytes], 64-byte swizzle: 16-byte chunk j of row r at chunk j ^ ((r >> 1) & 3)
+                        const uint32_t base = stage_area + lane * 64;
+                        const uint32_t x = (lane >> 1) & 3;
+                        uint32_t p[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            p[i] = fp8_pack4(h0[4 * i] * inv, h0[4 * i + 1] * inv, h0[4 * i + 2] * inv, h0[4 * i + 3] * inv);
+                        const uint32_t j0 = 2 * s0, j1 = 2 * (s0 ^ 1);
+                        st_shared_v4(base + ((j0 ^ x) << 4), p[0], p[1], p[2], p[3]);
+                        st_shared_v4(base + (((j0 + 1) ^ x) << 4), p[4], p[5], p[6], p[7]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            p[i] = fp8_pack4(h1[4 * i] * inv, h1[4 * i + 1] * inv, h1[4 * i + 2] * inv, h1[4 * i + 3] * inv);
+                        st_shared_v4(base + ((j1 ^ x) << 4), p[0], p[1], p[2], p[3]);
+                        st_shared_v4(base + (((j1 + 1) ^ x) << 4), p[4], p[5], p[6], p[7]);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&tmO, stage_area, col0 / 2, w.tile * TILE_M + q * 32);
+                            bulk_commit();
+                        }
+                        stored = true;
+                    }
+                }
+            } else {
+                uint32_t r[32];
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) {
+                    // half 1 starts with the last chunk, which may be the shared one
+                    const int c = half == 0 ? i : 4 + ((i + 3) & 3);
+                    tmem_ld32(taddr + c * 32, r);
+                    tmem_ld_wait();
+                    if (i == 0 && shares) hand_back_shared();
+                    if (i == 3) hand_back_all();
+                    const int col0 = w.nb * F8_PAIR_N + c * 32;
+                    if (w.valid && col0 < g.out_cols) {
+                        __nv_bfloat16* dst = g.y + grow * g.out_cols + col0;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            if (col0 + j * 16 < g.out_cols) {     // D is a multiple of 16: 32-byte pieces are whole
+                                uint32_t v[8];
+#pragma unroll
+                                for (int u = 0; u < 8; ++u)
+                                    v[u] = f8_pack_bf16(__uint_as_float(r[j * 16 + 2 * u]) * wgt,
+                                                        __uint_as_float(r[j * 16 + 2 * u + 1]) * wgt);
+                                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + j * 16),
+                                             "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                                             "r"(v[6]), "r"(v[7])
+                                             : "memory");
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_all<0>();   // the staging area must outlive every store issued from it
+        __syncwarp();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (*abortp) {
+        // a wait was abandoned: give loads still in flight time to land before shared memory is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+    }
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+template <bool UP>
+static int f8_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmO, const Fp8Args& g,
+                     cudaStream_t stream) {
+    static bool attr_set[64] = {false};
+    static int pairs[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MOMOE_ERR_CUDA;
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(fp8_grouped_gemm_kernel<UP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 F8_SMEM_BYTES) != cudaSuccess)
+            return MOMOE_ERR_CUDA;
+        attr_set[dev] = true;
+    }
+    if (pairs[dev] == 0) {
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
+        cfg.blockDim = dim3(F8_THREADS);
+        cfg.dynamicSmemBytes = F8_SMEM_BYTES;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2;
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, fp8_grouped_gemm_kernel<UP>, &cfg) != cudaSuccess || n <= 0) {
+            (void)cudaGetLastError();
+            n = sm_count() / 2;
+        }
+        pairs[dev] = n < sm_count() / 2 ? n : sm_count() / 2;
+    }
+    fp8_grouped_gemm_kernel<UP><<<2 * pairs[dev], F8_THREADS, F8_SMEM_BYTES, stream>>>(tmA, tmB, tmO, g);
+    return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
+}
+
+int fp8_check_plan(const momoe_plan_t* p) {
+    if (p == nullptr || p->sched == nullptr || p->tile_expert == nullptr || p->pair_info == nullptr ||
+        p->row_weight == nullptr || p->row_token == nullptr || p->pos_MK == nullptr || p->status == nullptr)
+        return MOMOE_ERR_ARG;
+    if (p->M <= 0 || p->N <= 0 || p->K <= 0 || p->D <= 0 || p->H <= 0 || p->rows_capacity <= 0) return MOMOE_ERR_ARG;
+    if (p->D % 16 != 0 || p->H % 16 != 0) return MOMOE_ERR_UNSUPPORTED;   // TMA row pitch of 8-bit rows: 16 bytes
+    if (p->rows_capacity % TILE_M != 0) return MOMOE_ERR_ARG;
+    return MOMOE_OK;
+}
+
+static inline int f8_cdiv(int a, int b) { return (a + b - 1) / b; }
+static inline bool f8_aligned(const void* p, uintptr_t n) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace momoe
+
+using namespace momoe;
+
+#define MOMOE_API extern "C" __attribute__((visibility("default")))
+
+MOMOE_API int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const uint8_t* x_sorted, const uint8_t* x_scale,
+                                  const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
+                                  momoe_stream_t stream) {
+    int rc = fp8_check_plan(plan);
+    if (rc != MOMOE_OK) return rc;
+    if (!f8_aligned(x_sorted, 16) || !f8_aligned(x_scale, 16) || !f8_aligned(W1_N2HD, 16) || S1 == nullptr ||
+        !f8_aligned(h_sorted, 16) || !f8_aligned(h_scale, 16))
+        return MOMOE_ERR_ARG;
+    const int D = plan->D, H = plan->H;
+    CUtensorMap tmA, tmB, tmO;
+    if ((rc = encode_tmap_2d(&tmA, x_sorted, plan->rows_capacity, D / 2, TILE_M, F8_K / 2)) != MOMOE_OK) return rc;
+    if ((rc = encode_tmap_3d(&tmB, W1_N2HD, static_cast<uint64_t>(plan->N) * 2, H, D / 2, 128, F8_K / 2)) != MOMOE_OK)
+        return rc;
+    if ((rc = encode_tmap_2d(&tmO, h_sorted, plan->rows_capacity, H / 2, 32, 32, TMAP_SWIZZLE_64B)) != MOMOE_OK) return rc;
+    Fp8Args g;
+    memset(&g, 0, sizeof(g));
+    g.sched = plan->sched;
+    g.tile_expert = plan->tile_expert;
+    g.pair_info = plan->pair_info;
+    g.status = plan->status;
+    g.n_nblk = f8_cdiv(H, 128);
+    g.nkb = f8_cdiv(D, F8_K);
+    g.out_cols = H;
+    g.a_scale = x_scale;
+    g.b_scale = S1;
+    g.h_scale = h_scale;
+    return f8_launch<true>(tmA, tmB, tmO, g, static_cast<cudaStream_t>(stream));
+}
+
+MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
+                                   const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, momoe_stream_t stream) {
+    int rc = fp8_check_plan(plan);
+    if (rc != MOMOE_OK) return rc;
+    if (!f8_aligned(h_sorted, 16) || !f8_aligned(h_scale, 16) || !f8_aligned(W2_NDH, 16) || S2 == nullptr ||
+        !f8_aligned(y_sorted, 32))
+        return MOMOE_ERR_ARG;
+    const int D = plan->D, H = plan->H;
+    CUtensorMap tmA, tmB;
+    if ((rc = encode_tmap_2d(&tmA, h_sorted, plan->rows_capacity, H / 2, TILE_M, F8_K / 2)) != MOMOE_OK) return rc;
+    if ((rc = encode_tmap_3d(&tmB, W2_NDH, plan->N, D, H / 2, 128, F8_K / 2)) != MOMOE_OK) return rc;
+    Fp8Args g;
+    memset(&g, 0, sizeof(g));
+    g.sched = plan->sched;
+    g.tile_expert = plan->tile_expert;
+    g.pair_info = plan->pair_info;
+    g.status = plan->status;
+    g.n_nblk = f8_cdiv(D, F8_PAIR_N);
+    g.nkb = f8_cdiv(H, F8_K);
+    g.out_cols = D;
+    g.a_scale = h_scale;
+    g.b_scale = S2;
+    g.b_blocks = f8_cdiv(D, 128);
+    g.row_weight = plan->row_weight;
+    g.y = static_cast<__nv_bfloat16*>(y_sorted);
+    return f8_launch<false>(tmA, tmB, tmA, g, static_cast<cudaStream_t>(stream));
+}

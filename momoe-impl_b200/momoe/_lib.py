@@ -60,6 +60,27 @@ _PROTOS = {
                                         c_vp]),
     "momoe_router_backward_compact": (C.c_int, [c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp]),
     "momoe_bias_update": (C.c_int, [c_vp, c_vp, c_i32, c_i32, C.c_float, C.c_float, c_vp]),
+    "momoe_rms_norm": (C.c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i32, c_i32, c_i32, c_i32, C.c_float, c_vp, c_vp, c_vp,
+                                 c_vp, c_vp, c_vp]),
+    "momoe_rms_norm_backward_workspace_bytes": (c_sz, [c_i32, c_i32]),
+    "momoe_rms_norm_backward": (C.c_int, [c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp,
+                                          c_vp, c_sz, c_vp]),
+    "momoe_quantize_rows": (C.c_int, [c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp]),
+    "momoe_balance_loss_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
+    "momoe_balance_loss": (C.c_int, [c_vp, c_i32, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, C.c_float,
+                                     C.c_float, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "momoe_balance_loss_backward": (C.c_int, [c_vp, c_i32, c_vp, c_i32, c_vp, c_i32, c_i32, c_i32, c_i32, C.c_float,
+                                              c_vp, c_vp, c_vp, c_vp]),
+    "momoe_fp8_quantize_weights": (C.c_int, [c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp]),
+    "momoe_fp8_gather_rows": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "momoe_fp8_up_swiglu": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "momoe_fp8_up_swiglu_decode": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "momoe_fp8_down_scale": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "momoe_fp8_down_scale_decode": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "momoe_fp8_experts_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "momoe_fp8_experts_launches": (C.c_int, [c_i32, c_i32, c_i32]),
+    "momoe_fp8_experts_forward": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp,
+                                            c_vp, c_i32, c_vp, c_vp, c_vp, c_sz, c_vp, c_vp]),
     "momoe_ep_set_wait_limit": (c_i64, [c_i64]),
     "momoe_ep_publish_counts": (C.c_int, [c_vp, c_i32, c_vp, c_vp, c_i32, c_i32, c_u32, c_vp, c_vp]),
     "momoe_ep_barrier": (C.c_int, [c_vp, c_i32, c_i32, c_u32, c_vp, c_vp]),
@@ -105,7 +126,35 @@ def stream_ptr():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}     # type codes of the C ABI
+
+
 def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("momoe (B200 build) runs on CUDA tensors only; there is no CPU path")
+
+
+def require_one_device(*tensors):
+    """The CUDA device that all given tensors (None is skipped) are on."""
+    require_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise RuntimeError("all tensors must be on the same device, but got: %s" % sorted(map(str, devices)))
+    return devices.pop()
+
+
+def as_rows(t):
+    """t [..., D] as a [M, D] tensor whose rows the kernels can read: contiguous columns, a row pitch of a multiple of 8
+    elements, a 16-byte aligned start.  A view where the layout allows it, a copy otherwise."""
+    r = t.reshape(-1, t.shape[-1])
+    if r.shape[0] <= 1 and r.stride(1) == 1 and r.data_ptr() % 16 == 0:
+        return r
+    if r.stride(1) != 1 or r.stride(0) % 8 != 0 or r.stride(0) < 0 or r.data_ptr() % 16 != 0:
+        r = r.clone(memory_format=torch.contiguous_format)
+    return r
+
+
+def pitch(r):
+    """Row pitch in elements of a tensor from as_rows."""
+    return r.stride(0) if r.shape[0] > 1 else r.shape[1]

@@ -1,0 +1,160 @@
+"""The experts' forward pass in 8-bit floating point: e4m3 rows and weights with a power of two (e8m0) for each block of
+128, multiplied on the tensor cores with 32-bit accumulation.  Forward only; weights take half the memory of bfloat16.
+
+    experts = quantize_experts(moe.momoe.Wl1_ND2H, moe.momoe.Wl2_NHD)       # once, when the weights are final
+    y_MD, tokens_per_expert_N = experts_forward(x_MD, topk_idx_MK, topk_w_MK, experts)
+
+`MoE.quantize_experts()` does the first and makes the module use the second."""
+from typing import NamedTuple
+
+import torch
+
+from . import _lib, ops
+from ._lib import as_rows, lib, pitch, ptr, stream_ptr
+
+BLOCK = 128                      # values that share a scale
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+class Fp8Rows(NamedTuple):
+    """Rows in 8 bits: the value of column c is q[m, c] * scale[m, c // 128]."""
+    q: torch.Tensor              # float8_e4m3fn [M, D]
+    scale: torch.Tensor          # float8_e8m0fnu [M, ceil(D / 128)]
+
+
+class Fp8Experts(NamedTuple):
+    """Expert weights in 8 bits, the contraction axis last, one scale for each 128 x 128 block."""
+    W1_N2HD: torch.Tensor        # float8_e4m3fn [N, 2H, D]: rows [:H] linear half, [H:] gate half
+    S1: torch.Tensor             # float8_e8m0fnu [N, 2, ceil(H / 128), ceil(D / 128)]
+    W2_NDH: torch.Tensor         # float8_e4m3fn [N, D, H]
+    S2: torch.Tensor             # float8_e8m0fnu [N, ceil(D / 128), ceil(H / 128)]
+
+    @property
+    def sizes(self):
+        """(N, D, H)."""
+        return self.W2_NDH.shape
+
+
+def _blocks(n):
+    return -(-n // BLOCK)
+
+
+def quantize_rows(x):
+    """x [..., D] (bfloat16, float16 or float32; D a multiple of 8) -> Fp8Rows of the [M, D] view.  The scale of a block
+    is the smallest power of two that brings its largest magnitude to 448 at most (1 for a block of zeros, NaN for a block
+    that holds an infinity or a NaN), so only the conversion to e4m3 rounds."""
+    _lib.require_cuda(x)
+    if x.dtype not in _lib.TYPES:
+        raise RuntimeError("quantize_rows works on bfloat16, float16 or float32, but got: %s" % x.dtype)
+    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % 8 != 0:
+        raise RuntimeError("the width of 8-bit rows must be a multiple of 8, but got: %s" % list(x.shape))
+    with torch.cuda.device(x.device):
+        r = as_rows(x.detach())
+        M, D = r.shape
+        rows = Fp8Rows(torch.empty((M, D), dtype=E4M3, device=x.device),
+                       torch.empty((M, _blocks(D)), dtype=E8M0, device=x.device))
+        if M > 0:
+            ops._call("momoe_quantize_rows", 1, lib.momoe_quantize_rows, ptr(r), pitch(r), _lib.TYPES[r.dtype], M, D,
+                      ptr(rows.q), ptr(rows.scale), stream_ptr())
+    return rows
+
+
+def _quantize_weights(W, groups):
+    N, Kd, C = W.shape
+    W = W.detach().contiguous()
+    if W.dtype not in (torch.bfloat16, torch.float32):
+        W = W.to(torch.float32)
+    q = torch.empty((N, C, Kd), dtype=E4M3, device=W.device)
+    S = torch.empty((N, groups, _blocks(C // groups), _blocks(Kd)), dtype=E8M0, device=W.device)
+    ops._call("momoe_fp8_quantize_weights", 1, lib.momoe_fp8_quantize_weights, ptr(W), _lib.TYPES[W.dtype], N, Kd, groups,
+              C // groups, ptr(q), ptr(S), stream_ptr())
+    return q, S
+
+
+def quantize_experts(Wl1_ND2H, Wl2_NHD):
+    """Up/gate weights [N, D, 2H] and down weights [N, H, D], as `MoMoE` holds them -> Fp8Experts."""
+    dev = _lib.require_one_device(Wl1_ND2H, Wl2_NHD)
+    if Wl1_ND2H.dim() != 3 or Wl2_NHD.dim() != 3:
+        raise RuntimeError("expert weights must be [N, D, 2H] and [N, H, D], but got: %s and %s"
+                           % (list(Wl1_ND2H.shape), list(Wl2_NHD.shape)))
+    N, H, D = Wl2_NHD.shape
+    if tuple(Wl1_ND2H.shape) != (N, D, 2 * H):
+        raise RuntimeError("expert weights must be [N, D, 2H] and [N, H, D], but got: %s and %s"
+                           % (list(Wl1_ND2H.shape), list(Wl2_NHD.shape)))
+    if N == 0 or D == 0 or H == 0 or D % 16 != 0 or H % 16 != 0:
+        raise RuntimeError("8-bit experts need D and H in multiples of 16, but got: D = %d, H = %d" % (D, H))
+    with torch.cuda.device(dev):
+        W1, S1 = _quantize_weights(Wl1_ND2H, 2)
+        W2, S2 = _quantize_weights(Wl2_NHD, 1)
+    return Fp8Experts(W1, S1, W2, S2.view(N, _blocks(D), _blocks(H)))
+
+
+def _check_tensor(t, name, shape, dtype):
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
+        raise RuntimeError("%s must be a contiguous %s of shape %s, but got: %s of shape %s, strides %s"
+                           % (name, dtype, list(shape), t.dtype, list(t.shape), list(t.stride())))
+    if t.data_ptr() % 16 != 0:
+        raise RuntimeError("%s must start on a 16-byte boundary" % name)
+
+
+def experts_forward(x, topk_idx_MK, topk_w_MK, experts):
+    """Weighted sum of the K chosen experts' outputs for each token, in 8 bits.
+
+    x: bfloat16 [M, D] (converted on the way; other float types are cast to bfloat16 first), or Fp8Rows;
+    topk_idx_MK int32 [M, K]: distinct expert ids; topk_w_MK float32 [M, K]; experts: Fp8Experts.  D, H multiples of 16,
+    N <= 1024, K <= 32.  Returns (y bfloat16 [M, D], tokens_per_expert_N int64 [N]).  The hidden values are converted to
+    8-bit rows once, from 32 bits.  No host synchronisation: an expert id out of range (202) or a token that names an
+    expert twice (203) is reported through the device's status word like the other problems only the device can see."""
+    rows8 = isinstance(x, Fp8Rows)
+    data = x.q if rows8 else x
+    dev = _lib.require_one_device(data, x.scale if rows8 else None, topk_idx_MK, topk_w_MK, *experts)
+    if torch.is_grad_enabled() and (data.requires_grad or topk_w_MK.requires_grad):
+        raise RuntimeError("8-bit experts have no backward pass: call them under torch.no_grad()")
+    if experts.W2_NDH.dim() != 3 or data.dim() != 2 or topk_idx_MK.dim() != 2 or topk_idx_MK.shape[0] != data.shape[0]:
+        raise RuntimeError("x must be [M, D], topk_idx_MK [M, K] and the weights [N, 2H, D] and [N, D, H], but got: %s, %s, "
+                           "%s and %s" % (list(data.shape), list(topk_idx_MK.shape), list(experts.W1_N2HD.shape),
+                                          list(experts.W2_NDH.shape)))
+    N, D, H = experts.sizes
+    M, K = topk_idx_MK.shape
+    if D % 16 != 0 or H % 16 != 0 or D == 0 or H == 0:
+        raise RuntimeError("8-bit experts need D and H in multiples of 16, but got: D = %d, H = %d" % (D, H))
+    _check_tensor(experts.W1_N2HD, "W1_N2HD", (N, 2 * H, D), E4M3)
+    _check_tensor(experts.W2_NDH, "W2_NDH", (N, D, H), E4M3)
+    _check_tensor(experts.S1, "S1", (N, 2, _blocks(H), _blocks(D)), E8M0)
+    _check_tensor(experts.S2, "S2", (N, _blocks(D), _blocks(H)), E8M0)
+    if K == 0 or K > N:
+        raise RuntimeError("each token needs 1 to N = %d experts, but got K = %d" % (N, K))
+    if topk_idx_MK.dtype != torch.int32:
+        topk_idx_MK = topk_idx_MK.to(torch.int32)
+    with torch.cuda.device(dev):
+        if rows8:
+            if data.shape[1] != D:
+                raise RuntimeError("x must be [M, %d], but got: %s" % (D, list(data.shape)))
+            data, scale = data.contiguous(), x.scale.contiguous()
+            data = data if data.data_ptr() % 16 == 0 else data.clone()
+            _check_tensor(data, "x.q", (M, D), E4M3)
+            if scale.shape != (M, _blocks(D)) or scale.dtype != E8M0:
+                raise RuntimeError("x.scale must be %s of shape %s, but got: %s of shape %s"
+                                   % (E8M0, [M, _blocks(D)], scale.dtype, list(scale.shape)))
+        else:
+            scale = None
+            if data.shape[1] != D or not data.is_floating_point():
+                raise RuntimeError("x must be floating-point [M, %d], but got: %s %s" % (D, data.dtype, list(data.shape)))
+            data = data.detach().to(torch.bfloat16).contiguous()
+            data = data if data.data_ptr() % 16 == 0 else data.clone()
+        if topk_w_MK.shape != topk_idx_MK.shape:
+            raise RuntimeError("topk_w_MK must be like topk_idx_MK, %s, but got: %s"
+                               % (list(topk_idx_MK.shape), list(topk_w_MK.shape)))
+        idx = topk_idx_MK.contiguous()
+        w = topk_w_MK.detach().to(torch.float32).contiguous()
+        y = torch.empty((M, D), dtype=torch.bfloat16, device=dev)
+        if M == 0:
+            return y, torch.zeros(N, dtype=torch.int64, device=dev)
+        sizes = torch.empty(N, dtype=torch.int64, device=dev)
+        nbytes = int(lib.momoe_fp8_experts_workspace_bytes(M, N, K, D, H))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ops._call("momoe_fp8_experts_forward", int(lib.momoe_fp8_experts_launches(M, N, K)),
+                  lib.momoe_fp8_experts_forward, ptr(data), ptr(scale), ptr(idx), ptr(w), M, N, K, D, H,
+                  ptr(experts.W1_N2HD), ptr(experts.S1), ptr(experts.W2_NDH), ptr(experts.S2), ops.DECODE_MAX_AVG_ROWS,
+                  ptr(y), ptr(sizes), ptr(ws), nbytes, ptr(ops.status_word(dev)), stream_ptr())
+    return y, sizes

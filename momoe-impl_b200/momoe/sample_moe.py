@@ -4,22 +4,27 @@
 By default the wrapper runs router and experts as one autograd node that keeps the routing in its compact form
 (top-k ids, weights, permutation): the dense `mask_NM` / `s_NM` of the two-module composition, the dense `G_s_NM` and
 the dense router backward are never materialised.  `MoE.fused = False` restores the literal composition
-`TopKRouter -> MoMoE`; both give the same output bit for bit."""
+`TopKRouter -> MoMoE`; both give the same output bit for bit.
+
+Two things the reference does not have are switched on by attributes: `balance_coef` / `z_coef` add the router's balance
+loss and z-loss (`momoe.balance`; the value is `MoE.aux_loss`, to be added to the training loss), and `quantize_experts()`
+makes forward-only calls run the experts in 8 bits (`momoe.fp8`)."""
 import torch
 import torch.nn as nn
 
-from . import ops
+from . import balance, fp8, ops
 from ._lib import require_cuda
-from .momoe import MoMoE, _CHECK
+from .momoe import MoMoE, _CHECK, compact_routing_of
 from .topk_router import TopKRouter
 
 
 class FusedMoEFunction(torch.autograd.Function):
     """Gate GEMM -> router kernel -> permutation -> experts, and the matching backward, on compact routing data.
-    Stands in for momoe/topk_router.py:85-145 plus momoe/momoe.py:847-903 of the reference."""
+    Stands in for momoe/topk_router.py:85-145 plus momoe/momoe.py:847-903 of the reference.  With a balance or z
+    coefficient there is a third output, the router's auxiliary loss, each of the B sequences balanced on its own."""
 
     @staticmethod
-    def forward(ctx, x_BSD, Wg_DN, Wl1_ND2H, Wl2_NHD, biases_N, K, Ks, save_percent):
+    def forward(ctx, x_BSD, Wg_DN, Wl1_ND2H, Wl2_NHD, biases_N, K, Ks, save_percent, balance_coef, z_coef):
         B, S, D = x_BSD.shape
         assert Wg_DN.dtype == torch.bfloat16, "Wg_DN must be of type torch.bfloat16"
         assert Wl1_ND2H.device == Wl2_NHD.device, \
@@ -38,11 +43,17 @@ class FusedMoEFunction(torch.autograd.Function):
             plan = ops.RoutingPlan.from_topk(topk_idx, topk_w, N, D, H, save_percent)
             y_MD, a_save, b_save = ops.experts_forward(plan, x_MD, W1, W2,
                                                           inference=not any(ctx.needs_input_grad))
+            ctx.aux = balance_coef != 0 or z_coef != 0
+            if ctx.aux:
+                aux_loss, _, g_BN = balance._loss(logits_MN, topk_idx, Ks, balance_coef, z_coef, None, S, B)
         ctx.plan = plan
         ctx.shape = (B, S, D)
         ctx.Ks = Ks
+        ctx.z_coef = z_coef
         ctx.x_device = x_BSD.device
         saved = [x_MD, Wg, W1, W2, d["Ng_M"], d["Ks_M"]]
+        if ctx.aux:
+            saved += [logits_MN, g_BN]
         ctx.has_ab = a_save is not None
         if ctx.has_ab:
             saved += [a_save, b_save]
@@ -51,13 +62,14 @@ class FusedMoEFunction(torch.autograd.Function):
         ops.status_post(dev)
         if _CHECK:
             ops.check_status(dev)
-        return y_MD.reshape(B, S, D).to(device=x_BSD.device), plan.sizes
+        y_BSD = y_MD.reshape(B, S, D).to(device=x_BSD.device)
+        return (y_BSD, plan.sizes, aux_loss) if ctx.aux else (y_BSD, plan.sizes)
 
     @staticmethod
-    def backward(ctx, G_y_BSD, _):
+    def backward(ctx, G_y_BSD, _, G_aux=None):
         saved = ctx.saved_tensors
         x_MD, Wg, W1, W2, Ng_M, Ks_M = saved[:6]
-        a_save, b_save = (saved[6], saved[7]) if ctx.has_ab else (None, None)
+        a_save, b_save = (saved[-2], saved[-1]) if ctx.has_ab else (None, None)
         B, S, D = ctx.shape
         plan = ctx.plan
         dev = W1.device
@@ -66,12 +78,16 @@ class FusedMoEFunction(torch.autograd.Function):
             G_x, G_W1, G_W2, gs_part = ops.experts_backward(plan, g_MD, x_MD, W1, W2, a_save, b_save,
                                                             need_gs_dense=False)
             G_L = ops.router_backward_compact(plan, gs_part, Ng_M, Ks_M, ctx.Ks)
+            if ctx.aux:
+                # the experts' share of the logits' gradient is in 16 bits already; the sum is formed in 32 and rounded
+                # once more, like every gradient that reaches the two gate GEMMs
+                G_L = balance._loss_backward(saved[6], saved[7], ctx.Ks, ctx.z_coef, None, S, B, G_aux, add=G_L)
             G_x = torch.addmm(G_x, G_L, Wg.T)
             G_Wg = x_MD.T @ G_L
         ops.status_post(dev)
         if _CHECK:
             ops.check_status(dev)
-        return G_x.reshape(B, S, D).to(ctx.x_device), G_Wg, G_W1, G_W2, None, None, None, None
+        return G_x.reshape(B, S, D).to(ctx.x_device), G_Wg, G_W1, G_W2, None, None, None, None, None, None
 
 
 class MoE(nn.Module):
@@ -97,16 +113,68 @@ class MoE(nn.Module):
                        torch.full((self.Ks,), float("-inf"), device=dev, dtype=torch.float32)], dim=-1),
             requires_grad=False)
         self.fused = True
+        self.balance_coef = 0.0     # weight of the balance loss (each of a batch's sequences on its own)
+        self.z_coef = 0.0           # weight of the z-loss
+        self.aux_loss = None        # their sum of the latest forward pass, float32 [], differentiable; None if both are 0
+        self.experts_fp8 = None     # 8-bit weights of forward-only calls, from quantize_experts()
+        self._fp8_versions = None
 
-    def forward(self, x_BSD):
-        if self.fused:
+    def quantize_experts(self):
+        """From now on forward passes use an 8-bit copy of the expert weights as they are now.  Such passes have no
+        backward: they run under torch.no_grad() (or with nothing that requires a gradient).  When the weights have
+        changed since, forward raises; call this again, or set `experts_fp8 = None` to go back to 16 bits."""
+        self.experts_fp8 = fp8.quantize_experts(self.momoe.Wl1_ND2H, self.momoe.Wl2_NHD)
+        self._fp8_versions = (self.momoe.Wl1_ND2H._version, self.momoe.Wl2_NHD._version)
+
+    def _forward_fp8(self, x_BSD, rows):
+        if torch.is_grad_enabled() and (x_BSD.requires_grad or any(p.requires_grad for p in self.parameters())):
+            raise RuntimeError("8-bit experts have no backward pass: call the layer under torch.no_grad()")
+        if self._fp8_versions != (self.momoe.Wl1_ND2H._version, self.momoe.Wl2_NHD._version):
+            raise RuntimeError("the expert weights have changed since quantize_experts(): call it again")
+        Wg = self.router.Wg_DN
+        assert Wg.dtype == torch.bfloat16, "Wg_DN must be of type torch.bfloat16"
+        dev = Wg.device
+        require_cuda(Wg)
+        ops.status_poll(dev)
+        B, S, D = x_BSD.shape
+        with torch.cuda.device(dev):
+            x_MD = x_BSD.detach().reshape(B * S, D).to(device=dev, dtype=torch.bfloat16)
+            topk_idx, topk_w, _ = ops.route_topk(x_MD @ Wg.detach(), self.biases_N.detach(), self.K, self.Ks, dense=False)
+            y_MD, sizes_N = fp8.experts_forward(x_MD if rows is None else rows, topk_idx, topk_w, self.experts_fp8)
+        ops.status_post(dev)
+        if _CHECK:
+            ops.check_status(dev)
+        return y_MD.reshape(B, S, D).to(device=x_BSD.device), sizes_N
+
+    def forward(self, x_BSD, rows_fp8=None):
+        """x_BSD [B, S, D] -> y_BSD.  rows_fp8: the same rows in 8 bits (momoe.fp8.Fp8Rows), if the caller has them, for
+        a layer with 8-bit experts; the router always reads x_BSD."""
+        self.aux_loss = None        # before the new graph is built: an old one must not keep its gradient nodes alive
+        aux = self.balance_coef != 0 or self.z_coef != 0
+        if self.experts_fp8 is not None:
+            if aux:
+                raise RuntimeError("balance_coef and z_coef are for training: 8-bit experts have no backward pass")
+            y_BSD, sizes_N = self._forward_fp8(x_BSD, rows_fp8)
+        elif rows_fp8 is not None:
+            raise RuntimeError("8-bit rows need 8-bit experts: call quantize_experts() first")
+        elif self.fused:
             ops.status_poll(self.momoe.Wl1_ND2H.device)  # raises if an earlier pass left a device-side error code
-            y_BSD, sizes_N = FusedMoEFunction.apply(x_BSD, self.router.Wg_DN, self.momoe.Wl1_ND2H,
-                                                    self.momoe.Wl2_NHD, self.biases_N, self.K, self.Ks,
-                                                    self.save_percent)
+            out = FusedMoEFunction.apply(x_BSD, self.router.Wg_DN, self.momoe.Wl1_ND2H, self.momoe.Wl2_NHD,
+                                         self.biases_N, self.K, self.Ks, self.save_percent, float(self.balance_coef),
+                                         float(self.z_coef))
+            y_BSD, sizes_N = out[:2]
+            if aux:
+                self.aux_loss = out[2]
         else:
+            x_in = x_BSD
             x_BSD, mask_NM, s_NM = self.router(x_BSD, self.biases_N)
             y_BSD, sizes_N = self.momoe(x_BSD, mask_NM, s_NM)
+            if aux:
+                topk_idx, _ = compact_routing_of(mask_NM, s_NM)
+                Wg = self.router.Wg_DN
+                logits_MN = x_in.reshape(-1, self.D).to(device=Wg.device, dtype=torch.bfloat16) @ Wg
+                self.aux_loss, _ = balance.balance_loss(logits_MN, topk_idx, self.Ks, self.balance_coef, self.z_coef,
+                                                        seq_len=x_in.shape[1])
         # DeepSeek-style auxiliary-loss-free balancing: push the bias of under-loaded experts up
         B, S, _ = x_BSD.shape
         c_avg = B * S * (self.K - self.Ks) / (self.N - self.Ks)

@@ -1,0 +1,399 @@
+"""8-bit rows, 8-bit weights and the experts' forward pass on them, stage by stage against 64 bits.
+
+Each stage is fed what the previous kernel wrote, so that a value next to a border of e4m3 cannot blur the next stage.
+Tolerances: a product of two e4m3 values and powers of two is exact in 32 bits; the tensor core adds 32 of them and the
+accumulator at a time, at most 2^-21 of the sum of magnitudes an addition, over at most 4096 / 32 additions: 2^-14.
+exp and the division of the activation: 2^-20 relative.  e4m3 is off by half a step (2^-4 relative, 2^-10 of the scale
+below 2^-6 of it), bfloat16 by 2^-8 relative."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+ACC = 2.0 ** -14
+# M, N, K, D, H, skew
+SHAPES = [
+    (1, 8, 2, 64, 32, 0.0),
+    (1, 128, 8, 2048, 768, 0.0),
+    (5, 4, 4, 16, 16, 0.0),           # smaller than one block in every axis; every expert sees every token
+    (37, 6, 3, 144, 272, 0.0),        # ragged in both widths
+    (70, 2, 1, 512, 640, 0.0),        # more than one 32-row block
+    (300, 4, 2, 528, 400, 1.0),
+    (1000, 16, 4, 640, 1152, 2.0),    # skewed: empty experts, experts of many tiles
+    (257, 3, 1, 2176, 128, 0.0),
+    (129, 1, 1, 128, 4096, 0.0),
+    (640, 5, 3, 4096, 48, 0.0),
+]
+
+
+@pytest.fixture(scope="module")
+def fp8():
+    import __graft_entry__
+    __graft_entry__.build()
+    from momoe import fp8
+    return fp8
+
+
+def rows_of(v):
+    """Values in 64 bits -> codes and scales by the definition."""
+    C = v.shape[-1]
+    top = torch.nn.functional.pad(v.abs(), (0, -C % 128)).unflatten(-1, (-1, 128)).amax(-1)
+    m, x = torch.frexp(top / 448)
+    e = torch.where(m > 0.5, x, x - 1)
+    scale = torch.where(top > 0, torch.ldexp(torch.ones_like(top), e), 1.0)
+    scale = torch.where(torch.isfinite(top), scale, float("nan"))
+    return (v / wide(scale, C)).float().to(torch.float8_e4m3fn), scale
+
+
+def wide(scale, C):
+    return scale.repeat_interleave(128, -1)[..., :C]
+
+
+def value(q, scale):
+    return q.double() * wide(scale.double(), q.shape[-1])
+
+
+def weights(fp8, N, D, H, seed):
+    g = torch.Generator().manual_seed(seed)
+    W1 = (torch.randn(N, D, 2 * H, generator=g) * torch.exp(torch.randn(N, D, 1, generator=g)) / D ** 0.5).bfloat16().cuda()
+    W2 = (torch.randn(N, H, D, generator=g) / H ** 0.5).bfloat16().cuda()
+    return W1, W2
+
+
+def block_values(q, S):
+    """Dequantised [.., C, Kd] of codes [.., C, Kd] and block scales."""
+    C, Kd = q.shape[-2:]
+    return q.double() * S.double().repeat_interleave(128, -2)[..., :C, :].repeat_interleave(128, -1)[..., :Kd]
+
+
+def routing(M, N, K, seed, skew):
+    from helpers import make_routing
+    return make_routing(M, N, K, seed, skew)
+
+
+def unpack_scales(buf, rows, blocks):
+    """Expert-major scale bytes as the GEMMs read them -> scales [rows, blocks]."""
+    g = -(-blocks // 4)
+    r, b = torch.arange(rows, device=buf.device)[:, None], torch.arange(blocks, device=buf.device)[None]
+    at = (r // 128 * g + b // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + b % 4
+    return torch.exp2(buf[at].double() - 127)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantize_rows(fp8, dtype):
+    for M, D in ((1, 8), (3, 128), (130, 136), (7, 2048), (1001, 264)):
+        g = torch.Generator().manual_seed(M)
+        x = (torch.randn(M, D, generator=g) * torch.exp(3 * torch.randn(M, 1, generator=g))).to(dtype).cuda()
+        x[0, :min(D, 128)] = 0
+        got = fp8.quantize_rows(x)
+        q, scale = rows_of(x.double())
+        # the largest rows overflow float16: an infinity makes its block's scale NaN (by the definition), no other
+        fine = torch.isfinite(scale)
+        assert torch.isnan(got.scale.double()[~fine]).all() and torch.equal(got.scale.double()[fine], scale[fine])
+        at = wide(fine, D)
+        assert torch.equal(got.q.float()[at], q.float()[at])
+        view = fp8.quantize_rows(torch.cat([x, x], 1)[:, :D] if D % 8 == 0 else x)
+        assert torch.equal(view.q.view(torch.uint8), got.q.view(torch.uint8))
+    assert fp8.quantize_rows(x[:0]).scale.shape == (0, 3)
+
+
+def test_scale_borders_and_bad_values(fp8):
+    """448 * 2^e keeps its power, the next larger value takes the next one; tiny, huge and bad values."""
+    x = torch.zeros(8, 128, device="cuda")
+    x[0, 3] = 448.0
+    x[1, 3] = torch.nextafter(torch.tensor(448.0), torch.tensor(1e9))
+    x[2, 3] = -1.75 * 2.0 ** -20
+    x[3, 3] = 2.0 ** -149                    # smallest subnormal: the scale stops at 2^-127
+    x[4, 3] = torch.finfo(torch.float32).max
+    x[5, 3], x[5, 4] = float("inf"), 1.0
+    x[6, 3] = float("nan")
+    r = fp8.quantize_rows(x)
+    s = r.scale.view(torch.uint8).flatten().tolist()
+    assert s == [127, 128, 127 - 28, 0, 127 + 120, 255, 255, 127]
+    v = value(r.q, r.scale)
+    assert float(v[0, 3]) == 448 and float(v[1, 3]) == 448 and float(v[2, 3]) == -1.75 * 2.0 ** -20
+    assert torch.isnan(v[5]).all() and torch.isnan(v[6]).all() and not v[7].any() and torch.isfinite(v[:5]).all()
+
+
+@pytest.mark.parametrize("N,D,H", [(1, 16, 16), (3, 144, 272), (2, 512, 128), (4, 2176, 48)])
+def test_quantize_experts(fp8, N, D, H):
+    W1, W2 = weights(fp8, N, D, H, 3)
+    W2[0, :, :min(D, 128)] = 0
+    for cast in (torch.bfloat16, torch.float32):
+        e = fp8.quantize_experts(W1.to(cast), W2.to(cast))
+        assert e.sizes == (N, D, H)
+        for q, S, w in ((e.W1_N2HD.view(N, 2, H, D), e.S1, W1.double().transpose(1, 2).reshape(N, 2, H, D)),
+                        (e.W2_NDH, e.S2, W2.double().transpose(1, 2))):
+            C, Kd = w.shape[-2:]
+            top = torch.nn.functional.pad(w.abs(), (0, -Kd % 128, 0, -C % 128)).unflatten(-1, (-1, 128)).unflatten(-3, (-1, 128)).amax((-3, -1))
+            assert S.shape == top.shape
+            s = S.double()
+            assert (s[top == 0] == 1).all()
+            assert (top <= 448 * s).all() and (top > 224 * s)[top > 0].all()
+            step = s.repeat_interleave(128, -2)[..., :C, :].repeat_interleave(128, -1)[..., :Kd]
+            assert torch.equal(q.float(), (w / step).float().to(torch.float8_e4m3fn).float())
+
+
+@pytest.mark.parametrize("decode", [False, True])
+@pytest.mark.parametrize("M,N,K,D,H,skew", SHAPES)
+def test_stages_against_64_bits(fp8, M, N, K, D, H, skew, decode):
+    from momoe import _lib, ops
+    lib, ptr, st = _lib.lib, _lib.ptr, _lib.stream_ptr()
+    idx, w = routing(M, N, K, M + D, skew)
+    W1, W2 = weights(fp8, N, D, H, D + H)
+    e = fp8.quantize_experts(W1, W2)
+    plan = ops.RoutingPlan.from_topk(idx, w, N, D, H)
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(M, D, generator=g).bfloat16().cuda()
+    rows, tiles = plan.rows_capacity, plan.tile_capacity
+    u8 = lambda n: torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")
+    xs, xsc, hs, hsc = u8(rows * D), u8(tiles * -(-D // 512) * 512), u8(rows * H), u8(tiles * -(-H // 512) * 512)
+    ys = torch.full((rows, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+    _lib.check(lib.momoe_fp8_gather_rows(plan.ref, ptr(x), None, ptr(xs), ptr(xsc), st), "gather")
+    up, down = ((lib.momoe_fp8_up_swiglu_decode, lib.momoe_fp8_down_scale_decode) if decode
+                else (lib.momoe_fp8_up_swiglu, lib.momoe_fp8_down_scale))
+    _lib.check(up(plan.ref, ptr(xs), ptr(xsc), ptr(e.W1_N2HD), ptr(e.S1), ptr(hs), ptr(hsc), st), "up")
+    _lib.check(down(plan.ref, ptr(hs), ptr(hsc), ptr(e.W2_NDH), ptr(e.S2), ptr(ys), st), "down")
+    torch.cuda.synchronize()
+    ops.check_status()
+    real = (plan.row_token >= 0).nonzero().flatten()
+    token = plan.row_token[real].long()
+    expert = plan.tile_expert[real // 128].long()
+    # gather: the converted row of each token, bit for bit
+    q, scale = rows_of(x.double())
+    xq = xs.view(torch.float8_e4m3fn).view(rows, D)[real]
+    assert torch.equal(xq.float(), q[token].float())
+    assert torch.equal(unpack_scales(xsc, rows, -(-D // 128))[real], scale[token])
+    xv = value(xq, scale[token])
+    hq = hs.view(torch.float8_e4m3fn).view(rows, H)[real]
+    hscale = unpack_scales(hsc, rows, -(-H // 128))[real]
+    hv = value(hq, hscale)
+    W1v = block_values(e.W1_N2HD.view(N, 2, H, D), e.S1)
+    W2v = block_values(e.W2_NDH, e.S2)
+    for n in range(N):
+        at = (expert == n).nonzero().flatten()
+        if len(at) == 0:
+            continue
+        a, b = xv[at] @ W1v[n, 0].T, xv[at] @ W1v[n, 1].T
+        da, db = ACC * (xv[at].abs() @ W1v[n, 0].abs().T), ACC * (xv[at].abs() @ W1v[n, 1].abs().T)
+        s = torch.sigmoid(b)
+        h = a * b * s
+        # |d(b sigmoid(b))/db| <= 1.1
+        dh = da * (b * s).abs() + 1.1 * db * a.abs() + 1.1 * da * db + 2.0 ** -20 * h.abs()
+        top = torch.nn.functional.pad(h.abs(), (0, -H % 128)).unflatten(-1, (-1, 128)).amax(-1)
+        dtop = torch.nn.functional.pad(dh, (0, -H % 128)).unflatten(-1, (-1, 128)).amax(-1)
+        sc = hscale[at]
+        assert (top - dtop <= 448 * sc).all() and (top + dtop >= 224 * sc).all()
+        tol = torch.maximum((h.abs() + dh) * 2.0 ** -4, wide(sc, H) * 2.0 ** -10) + dh
+        assert ((hv[at] - h).abs() <= tol).all(), "h of expert %d: %g" % (n, float(((hv[at] - h).abs() / tol).max()))
+        y = hv[at] @ W2v[n].T * plan.row_weight[real[at], None].double()
+        dy = ACC * (hv[at].abs() @ W2v[n].abs().T) * plan.row_weight[real[at], None].double()
+        off = (ys[real[at]].double() - y).abs()
+        assert (off <= 2.0 ** -8 * (y.abs() + dy) + dy).all(), "y of expert %d" % n
+    # the whole call is these stages and the combine, bit for bit, from 16-bit and from 8-bit rows
+    want = ops.combine_rows(plan, ys, D)
+    saved = ops.DECODE_MAX_AVG_ROWS
+    try:
+        ops.DECODE_MAX_AVG_ROWS = 2 ** 20 if decode else 0
+        for rows_in in (x, fp8.Fp8Rows(q, scale.to(torch.float8_e8m0fnu)), fp8.quantize_rows(x)):
+            y, sizes = fp8.experts_forward(rows_in, idx, w, e)
+            assert torch.equal(y, want) and torch.equal(sizes, plan.sizes)
+    finally:
+        ops.DECODE_MAX_AVG_ROWS = saved
+    ops.check_status()
+
+
+def test_bad_rows_stay_alone_and_strides(fp8):
+    M, N, K, D, H = 200, 8, 2, 256, 192
+    idx, w = routing(M, N, K, 0, 0.0)
+    e = fp8.quantize_experts(*weights(fp8, N, D, H, 0))
+    x = torch.randn(M, D, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+    want, sizes = fp8.experts_forward(x, idx, w, e)
+    bad = x.clone()
+    bad[3, 7], bad[9, 200] = float("nan"), float("inf")
+    y, _ = fp8.experts_forward(bad, idx, w, e)
+    good = [i for i in range(M) if i not in (3, 9)]
+    assert torch.equal(y[good], want[good]) and torch.isnan(y[3]).all() and torch.isnan(y[9]).all()
+    y, _ = fp8.experts_forward(torch.cat([x, x], 1)[:, D:], idx.long(), w.t().contiguous().t(), e)
+    assert torch.equal(y, want)
+    odd = torch.empty(M * D + 1, dtype=torch.bfloat16, device="cuda")[1:].view(M, D).copy_(x)
+    assert torch.equal(fp8.experts_forward(odd, idx, w, e)[0], want)
+    assert torch.equal(fp8.experts_forward(x.float(), idx, w, e)[0], want)
+    zero, none = fp8.experts_forward(x[:0], idx[:0], w[:0], e)
+    assert zero.shape == (0, D) and none.tolist() == [0] * N
+
+
+def test_capture_other_stream_and_two_graphs(fp8):
+    from momoe import ops
+    N, K, D, H = 16, 4, 384, 256
+    e = fp8.quantize_experts(*weights(fp8, N, D, H, 1))
+    cases = []
+    for M in (3, 700):
+        idx, w = routing(M, N, K, M, 0.5)
+        x = torch.randn(M, D, generator=torch.Generator().manual_seed(M)).bfloat16().cuda()
+        cases.append((x, idx, w, fp8.experts_forward(x, idx, w, e)))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = [fp8.experts_forward(x, idx, w, e) for x, idx, w, _ in cases]
+    s.synchronize()
+    for (y, n), (_, _, _, (want, sizes)) in zip(got, cases):
+        assert torch.equal(y, want) and torch.equal(n, sizes)
+    graphs = []
+    for x, idx, w, want in cases:
+        buf, ibuf = torch.zeros_like(x), idx.flip(0).contiguous()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = fp8.experts_forward(buf, ibuf, w, e)
+        graphs.append((graph, buf, ibuf, out))
+    for _ in range(2):
+        for (graph, buf, ibuf, out), (x, idx, w, want) in zip(graphs, cases):
+            buf.copy_(x)
+            ibuf.copy_(idx)
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, _, out), (_, _, _, want) in zip(graphs, cases):
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    ops.check_status()
+
+
+def test_device_side_reports(fp8):
+    from momoe import ops
+    e = fp8.quantize_experts(*weights(fp8, 8, 64, 32, 1))
+    x = torch.randn(4, 64, device="cuda").bfloat16()
+    w = torch.full((4, 2), 0.5, device="cuda")
+    ops.check_status()
+    for ids, code in (([[0, 1], [2, 3], [4, 4], [5, 6]], "203"), ([[0, 1], [2, 8], [4, 5], [5, 6]], "202")):
+        fp8.experts_forward(x, torch.tensor(ids, dtype=torch.int32, device="cuda"), w, e)
+        with pytest.raises(RuntimeError, match=code):
+            ops.check_status()
+    ops.check_status()
+
+
+def test_refusals(fp8):
+    N, K, D, H = 4, 2, 64, 32
+    W1, W2 = weights(fp8, N, D, H, 2)
+    e = fp8.quantize_experts(W1, W2)
+    idx, w = routing(6, N, K, 0, 0.0)
+    x = torch.zeros(6, D, dtype=torch.bfloat16, device="cuda")
+    r = fp8.quantize_rows(x)
+    for bad in (lambda: fp8.experts_forward(x[:, :48], idx, w, e), lambda: fp8.experts_forward(x[:5], idx, w, e),
+                lambda: fp8.experts_forward(x, idx, w[:, :1], e), lambda: fp8.experts_forward(x.cpu(), idx, w, e),
+                lambda: fp8.experts_forward(x.clone().requires_grad_(True), idx, w, e),
+                lambda: fp8.experts_forward(x, idx, w.clone().requires_grad_(True), e),
+                lambda: fp8.experts_forward(x.int(), idx, w, e),
+                lambda: fp8.experts_forward(fp8.Fp8Rows(r.q, r.scale[:5]), idx, w, e),
+                lambda: fp8.experts_forward(fp8.Fp8Rows(r.q.view(torch.uint8), r.scale), idx, w, e),
+                lambda: fp8.experts_forward(x, idx, w, e._replace(S1=e.S1[:, :1])),
+                lambda: fp8.experts_forward(x, idx, w, e._replace(W2_NDH=e.W2_NDH.transpose(1, 2))),
+                lambda: fp8.experts_forward(x, torch.zeros(6, 5, dtype=torch.int32, device="cuda"), torch.zeros(6, 5, device="cuda"), e),
+                lambda: fp8.quantize_experts(W1, W2[:, :24]), lambda: fp8.quantize_experts(W1[:, :40, :], W2[:, :, :40]),
+                lambda: fp8.quantize_rows(x[:, :4]), lambda: fp8.quantize_rows(x.int()), lambda: fp8.quantize_rows(x.cpu())):
+        with pytest.raises(RuntimeError):
+            bad()
+
+
+# ------------------------------------------------------------------------------------------------- the layer
+def layer(D, H, N, K, Ks, seed, **kw):
+    import momoe
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)
+    return momoe.MoE(D, H, N, K, Ks, Wg_DN=(r(D, N) / D ** 0.5).bfloat16().cuda(),
+                     Wl1_ND2H=(r(N, D, 2 * H) / D ** 0.5).bfloat16().cuda(),
+                     Wl2_NHD=(r(N, H, D) / H ** 0.5).bfloat16().cuda(), **kw)
+
+
+def test_prenorm_layer_in_eight_bits_is_its_operators_in_a_row(fp8):
+    from momoe import norm, ops
+    B, S, D, H, N, K, Ks = 3, 41, 256, 128, 12, 4, 1
+    moe = layer(D, H, N, K, Ks, 0)
+    block = norm.PreNormMoE(norm.RMSNorm(D, weight=1 + 0.1 * torch.randn(D, device="cuda").bfloat16()), moe)
+    x, res = torch.randn(2, B, S, D, device="cuda").bfloat16()
+    bias = moe.biases_N.detach().clone()
+    with torch.no_grad():
+        y16, r16 = block(x, res)
+        moe.biases_N.copy_(bias)
+        moe.quantize_experts()
+        y, r = block(x, res)
+        assert torch.equal(r, r16) and y.shape == (B, S, D) and y.dtype == torch.bfloat16
+        n = norm.rms_norm_fp8(x, block.norm.weight, res)
+        logits = n.y.view(-1, D) @ moe.router.Wg_DN
+        idx, w, _ = ops.route_topk(logits, bias, K, Ks, dense=False)
+        want, sizes = fp8.experts_forward(n.rows, idx, w, moe.experts_fp8)
+        assert torch.equal(y.view(-1, D), want)
+        # the bias moved as it does in 16 bits
+        c_avg = B * S * (K - Ks) / (N - Ks)
+        step = moe.bias_update_rate * torch.sign(c_avg - sizes[:N - Ks].float())
+        assert torch.allclose(moe.biases_N[:N - Ks], bias[:N - Ks] + step, rtol=0, atol=1e-9)
+        # e4m3 in x, W and h, each off by up to 2^-4 and on average about 2^-5.3 of its value: y follows to some 8 %
+        assert float((y.float() - y16.float()).norm() / y16.float().norm()) < 0.12
+        alone = block(x)
+        assert torch.equal(alone[1], x)
+    # refusals: gradients, stale weights, rows without 8-bit experts, training coefficients
+    with pytest.raises(RuntimeError, match="no backward"):
+        moe(x)
+    with torch.no_grad():
+        moe.balance_coef = 0.1
+        with pytest.raises(RuntimeError, match="training"):
+            moe(x)
+        moe.balance_coef = 0.0
+        moe.momoe.Wl2_NHD.mul_(0.5)
+        with pytest.raises(RuntimeError, match="changed"):
+            moe(x)
+        moe.quantize_experts()
+        moe(x)
+        moe.experts_fp8 = None
+        with pytest.raises(RuntimeError, match="8-bit experts"):
+            moe(x, n.rows)
+        moe(x)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_layer_with_balance_loss_trains_on_the_sum_of_both(fp8, fused):
+    """The auxiliary loss and its share of the gradients are those of the operator on the layer's own logits."""
+    from momoe import balance, norm, ops
+    B, S, D, H, N, K, Ks = 4, 33, 192, 64, 10, 4, 1
+    def run(coefs, use_y=True):
+        moe = layer(D, H, N, K, Ks, 5)
+        moe.fused = fused
+        moe.balance_coef, moe.z_coef = coefs
+        block = norm.PreNormMoE(norm.RMSNorm(D), moe)
+        g = torch.Generator().manual_seed(3)
+        x = torch.randn(B, S, D, generator=g).bfloat16().cuda().requires_grad_(True)
+        y, r = block(x, torch.ones_like(x))
+        loss = (y.float() * torch.randn(B, S, D, generator=g).cuda()).sum() * (1.0 if use_y else 0.0)
+        if moe.aux_loss is not None:
+            loss = loss + 100 * moe.aux_loss
+        loss.backward()
+        return moe, block, x, y
+    plain, pblock, px, py = run((0.0, 0.0))
+    assert plain.aux_loss is None
+    moe, block, x, y = run((0.2, 0.05))
+    assert torch.equal(y, py)
+    # the operator on the same logits
+    with torch.no_grad():
+        n, _ = norm.rms_norm(x, block.norm.weight, torch.ones_like(x))
+        logits = n.view(-1, D) @ moe.router.Wg_DN
+        idx, _, _ = ops.route_topk(logits, layer(D, H, N, K, Ks, 5).biases_N, K, Ks, dense=False)
+    leaf = logits.detach().requires_grad_(True)
+    aux, counts = balance.balance_loss(leaf, idx, Ks, 0.2, 0.05, seq_len=S)
+    assert counts.shape == (B, N) and int(counts.sum()) == B * S * K
+    assert float(aux.detach()) == float(moe.aux_loss.detach())
+    (100 * aux).backward()
+    # gate weights: the two shares add up; each term is rounded to 16 bits on its way (2^-8 of the larger one, twice, and
+    # the products are rounded once more)
+    share = n.view(-1, D).double().T @ leaf.grad.double()
+    got = moe.router.Wg_DN.grad.double() - plain.router.Wg_DN.grad.double()
+    mags = n.view(-1, D).double().abs().T @ (leaf.grad.double().abs() * 2.0 ** -7)
+    both = moe.router.Wg_DN.grad.double().abs() + plain.router.Wg_DN.grad.double().abs()
+    # the logits' gradient of the experts is not at hand: bound it through the gate gradient's own size per column
+    lim = mags + 2.0 ** -7 * both + 2.0 ** -7 * both.amax(0, keepdim=True)
+    assert ((got - share).abs() <= lim).all(), float(((got - share).abs() / lim).max())
+    assert torch.equal(moe.momoe.Wl1_ND2H.grad, plain.momoe.Wl1_ND2H.grad)
+    # alone: the upstream gradient of y is zero, so only the operator's share remains
+    only, oblock, ox, _ = run((0.2, 0.05), use_y=False)
+    got = only.router.Wg_DN.grad.double()
+    assert ((got - share).abs() <= 2.0 ** -8 * share.abs() + mags).all()
+    assert not only.momoe.Wl2_NHD.grad.any() and ox.grad.any()
+    ops.check_status()
