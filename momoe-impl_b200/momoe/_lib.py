@@ -2,7 +2,9 @@
 
 There is no fallback: if the library is missing, importing this module raises with the build command.
 """
+import contextlib
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -137,24 +139,56 @@ def require_cuda(*tensors):
 
 def require_one_device(*tensors):
     """The CUDA device that all given tensors (None is skipped) are on."""
-    require_cuda(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise RuntimeError("all tensors must be on the same device, but got: %s" % sorted(map(str, devices)))
-    return devices.pop()
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        d = t.device
+        if dev is None:
+            dev = d
+        if d.type != "cuda":
+            require_cuda(t)
+        if d != dev:
+            raise RuntimeError("all tensors must be on the same device, but got: %s and %s" % (dev, d))
+    return dev
+
+
+_STAY = contextlib.nullcontext()
+
+
+def on_device(dev):
+    """Context in which `dev` is the current device; costs nothing where it already is."""
+    return _STAY if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+
+
+def raw_stream(dev):
+    """The current stream of a device as an integer (what a c_void_p argument takes)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def aligned(t, n=16):
+    """t itself where it starts on an n-byte boundary, a copy otherwise."""
+    return t if t.data_ptr() % n == 0 else t.clone()
 
 
 def as_rows(t):
     """t [..., D] as a [M, D] tensor whose rows the kernels can read: contiguous columns, a row pitch of a multiple of 8
     elements, a 16-byte aligned start.  A view where the layout allows it, a copy otherwise."""
-    r = t.reshape(-1, t.shape[-1])
-    if r.shape[0] <= 1 and r.stride(1) == 1 and r.data_ptr() % 16 == 0:
-        return r
+    r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if r.is_contiguous():
+        return aligned(r)
     if r.stride(1) != 1 or r.stride(0) % 8 != 0 or r.stride(0) < 0 or r.data_ptr() % 16 != 0:
-        r = r.clone(memory_format=torch.contiguous_format)
+        return r.contiguous()
     return r
 
 
 def pitch(r):
     """Row pitch in elements of a tensor from as_rows."""
     return r.stride(0) if r.shape[0] > 1 else r.shape[1]
+
+
+# Sizes that a shape asks for, remembered: a call into the library costs more than the look-up.
+rms_norm_backward_workspace_bytes = functools.lru_cache(4096)(lib.momoe_rms_norm_backward_workspace_bytes)
+balance_loss_workspace_bytes = functools.lru_cache(4096)(lib.momoe_balance_loss_workspace_bytes)
+fp8_experts_workspace_bytes = functools.lru_cache(4096)(lib.momoe_fp8_experts_workspace_bytes)
+fp8_experts_launches = functools.lru_cache(4096)(lib.momoe_fp8_experts_launches)

@@ -11,7 +11,7 @@ of `MoE`, which balances over the whole batch; `MoE.balance_coef` / `MoE.z_coef`
 import torch
 
 from . import _lib, ops
-from ._lib import lib, ptr, stream_ptr
+from ._lib import aligned, lib, on_device, raw_stream
 
 MAX_EXPERTS, MAX_SEQUENCES = 1024, 65535
 
@@ -25,11 +25,11 @@ def _loss(logits, idx, Ks, balance_coef, z_coef, cu, seq_len, B):
     g = torch.empty((B, N), dtype=torch.float32, device=dev)
     if M == 0:
         return loss.zero_(), counts.zero_(), g.zero_()
-    nbytes = int(lib.momoe_balance_loss_workspace_bytes(M, N, B))
+    nbytes = _lib.balance_loss_workspace_bytes(M, N, B)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    ops._call("momoe_balance_loss", 2, lib.momoe_balance_loss, ptr(logits), _lib.TYPES[logits.dtype], ptr(idx), ptr(cu),
-              seq_len, M, N, idx.shape[1], Ks, B, balance_coef, z_coef, ptr(loss), ptr(counts), ptr(g), ptr(ws), nbytes,
-              stream_ptr())
+    ops._call("momoe_balance_loss", 2, lib.momoe_balance_loss, logits.data_ptr(), _lib.TYPES[logits.dtype],
+              idx.data_ptr(), cu.data_ptr() if cu is not None else None, seq_len, M, N, idx.shape[1], Ks, B, balance_coef,
+              z_coef, loss.data_ptr(), counts.data_ptr(), g.data_ptr(), ws.data_ptr(), nbytes, raw_stream(dev))
     return loss, counts, g
 
 
@@ -38,19 +38,18 @@ def _loss_backward(logits, g, Ks, z_coef, cu, seq_len, B, G_loss, add=None):
     M, N = logits.shape
     out = add if add is not None else torch.empty_like(logits)
     if M > 0:
-        G_loss = G_loss.to(device=logits.device, dtype=torch.float32).contiguous()
-        ops._call("momoe_balance_loss_backward", 1, lib.momoe_balance_loss_backward, ptr(logits),
-                  _lib.TYPES[logits.dtype], ptr(cu), seq_len, ptr(g), M, N, Ks, B, z_coef, ptr(G_loss), ptr(add), ptr(out),
-                  stream_ptr())
+        ops._call("momoe_balance_loss_backward", 1, lib.momoe_balance_loss_backward, logits.data_ptr(),
+                  _lib.TYPES[logits.dtype], cu.data_ptr() if cu is not None else None, seq_len, g.data_ptr(), M, N, Ks, B,
+                  z_coef, G_loss.data_ptr(), add.data_ptr() if add is not None else None, out.data_ptr(),
+                  raw_stream(logits.device))
     return out
 
 
 class BalanceLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, idx, Ks, balance_coef, z_coef, cu, seq_len, B):
-        with torch.cuda.device(logits.device):
-            x = logits.detach().contiguous()
-            x = x if x.data_ptr() % 16 == 0 else x.clone()
+        with on_device(logits.device):
+            x = aligned(logits.contiguous())
             loss, counts, g = _loss(x, idx, Ks, balance_coef, z_coef, cu, seq_len, B)
         ctx.save_for_backward(x, g, cu)
         ctx.args = (Ks, z_coef, seq_len, B)
@@ -62,7 +61,7 @@ class BalanceLossFunction(torch.autograd.Function):
     def backward(ctx, G_loss, _):
         x, g, cu = ctx.saved_tensors
         Ks, z_coef, seq_len, B = ctx.args
-        with torch.cuda.device(x.device):
+        with on_device(x.device):
             out = _loss_backward(x, g, Ks, z_coef, cu, seq_len, B, G_loss)
         return out, None, None, None, None, None, None, None
 
@@ -89,7 +88,7 @@ def balance_loss(logits_MN, topk_idx_MK, num_shared_experts=0, balance_coef=1.0,
                            % (MAX_EXPERTS, Ks, K, N))
     if cu_seqlens is not None and seq_len is not None:
         raise RuntimeError("give cu_seqlens or seq_len, not both")
-    with torch.cuda.device(dev):
+    with on_device(dev):
         if topk_idx_MK.dtype != torch.int32:
             topk_idx_MK = topk_idx_MK.to(torch.int32)
         idx = topk_idx_MK.contiguous()

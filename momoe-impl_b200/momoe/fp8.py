@@ -10,7 +10,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, ops
-from ._lib import as_rows, lib, pitch, ptr, stream_ptr
+from ._lib import aligned, as_rows, lib, on_device, pitch, ptr, raw_stream
 
 BLOCK = 128                      # values that share a scale
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -48,14 +48,14 @@ def quantize_rows(x):
         raise RuntimeError("quantize_rows works on bfloat16, float16 or float32, but got: %s" % x.dtype)
     if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % 8 != 0:
         raise RuntimeError("the width of 8-bit rows must be a multiple of 8, but got: %s" % list(x.shape))
-    with torch.cuda.device(x.device):
+    with on_device(x.device):
         r = as_rows(x.detach())
         M, D = r.shape
         rows = Fp8Rows(torch.empty((M, D), dtype=E4M3, device=x.device),
                        torch.empty((M, _blocks(D)), dtype=E8M0, device=x.device))
         if M > 0:
             ops._call("momoe_quantize_rows", 1, lib.momoe_quantize_rows, ptr(r), pitch(r), _lib.TYPES[r.dtype], M, D,
-                      ptr(rows.q), ptr(rows.scale), stream_ptr())
+                      ptr(rows.q), ptr(rows.scale), raw_stream(x.device))
     return rows
 
 
@@ -67,7 +67,7 @@ def _quantize_weights(W, groups):
     q = torch.empty((N, C, Kd), dtype=E4M3, device=W.device)
     S = torch.empty((N, groups, _blocks(C // groups), _blocks(Kd)), dtype=E8M0, device=W.device)
     ops._call("momoe_fp8_quantize_weights", 1, lib.momoe_fp8_quantize_weights, ptr(W), _lib.TYPES[W.dtype], N, Kd, groups,
-              C // groups, ptr(q), ptr(S), stream_ptr())
+              C // groups, ptr(q), ptr(S), raw_stream(W.device))
     return q, S
 
 
@@ -83,7 +83,7 @@ def quantize_experts(Wl1_ND2H, Wl2_NHD):
                            % (list(Wl1_ND2H.shape), list(Wl2_NHD.shape)))
     if N == 0 or D == 0 or H == 0 or D % 16 != 0 or H % 16 != 0:
         raise RuntimeError("8-bit experts need D and H in multiples of 16, but got: D = %d, H = %d" % (D, H))
-    with torch.cuda.device(dev):
+    with on_device(dev):
         W1, S1 = _quantize_weights(Wl1_ND2H, 2)
         W2, S2 = _quantize_weights(Wl2_NHD, 1)
     return Fp8Experts(W1, S1, W2, S2.view(N, _blocks(D), _blocks(H)))
@@ -124,37 +124,35 @@ def experts_forward(x, topk_idx_MK, topk_w_MK, experts):
     _check_tensor(experts.S2, "S2", (N, _blocks(D), _blocks(H)), E8M0)
     if K == 0 or K > N:
         raise RuntimeError("each token needs 1 to N = %d experts, but got K = %d" % (N, K))
-    if topk_idx_MK.dtype != torch.int32:
-        topk_idx_MK = topk_idx_MK.to(torch.int32)
-    with torch.cuda.device(dev):
+    if topk_w_MK.shape != topk_idx_MK.shape:
+        raise RuntimeError("topk_w_MK must be like topk_idx_MK, %s, but got: %s"
+                           % (list(topk_idx_MK.shape), list(topk_w_MK.shape)))
+    if data.shape[1] != D or not data.is_floating_point():
+        raise RuntimeError("x must be floating-point [M, %d], but got: %s %s" % (D, data.dtype, list(data.shape)))
+    with on_device(dev):
+        scale_ptr = None
         if rows8:
-            if data.shape[1] != D:
-                raise RuntimeError("x must be [M, %d], but got: %s" % (D, list(data.shape)))
-            data, scale = data.contiguous(), x.scale.contiguous()
-            data = data if data.data_ptr() % 16 == 0 else data.clone()
+            data, scale = aligned(data.contiguous()), x.scale.contiguous()
             _check_tensor(data, "x.q", (M, D), E4M3)
             if scale.shape != (M, _blocks(D)) or scale.dtype != E8M0:
                 raise RuntimeError("x.scale must be %s of shape %s, but got: %s of shape %s"
                                    % (E8M0, [M, _blocks(D)], scale.dtype, list(scale.shape)))
+            scale_ptr = scale.data_ptr()
         else:
-            scale = None
-            if data.shape[1] != D or not data.is_floating_point():
-                raise RuntimeError("x must be floating-point [M, %d], but got: %s %s" % (D, data.dtype, list(data.shape)))
-            data = data.detach().to(torch.bfloat16).contiguous()
-            data = data if data.data_ptr() % 16 == 0 else data.clone()
-        if topk_w_MK.shape != topk_idx_MK.shape:
-            raise RuntimeError("topk_w_MK must be like topk_idx_MK, %s, but got: %s"
-                               % (list(topk_idx_MK.shape), list(topk_w_MK.shape)))
-        idx = topk_idx_MK.contiguous()
-        w = topk_w_MK.detach().to(torch.float32).contiguous()
+            if data.dtype != torch.bfloat16:
+                data = data.detach().to(torch.bfloat16)
+            data = aligned(data.contiguous())
+        idx = (topk_idx_MK if topk_idx_MK.dtype == torch.int32 else topk_idx_MK.to(torch.int32)).contiguous()
+        w = (topk_w_MK if topk_w_MK.dtype == torch.float32 else topk_w_MK.detach().to(torch.float32)).contiguous()
         y = torch.empty((M, D), dtype=torch.bfloat16, device=dev)
         if M == 0:
             return y, torch.zeros(N, dtype=torch.int64, device=dev)
         sizes = torch.empty(N, dtype=torch.int64, device=dev)
-        nbytes = int(lib.momoe_fp8_experts_workspace_bytes(M, N, K, D, H))
+        nbytes = _lib.fp8_experts_workspace_bytes(M, N, K, D, H)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        ops._call("momoe_fp8_experts_forward", int(lib.momoe_fp8_experts_launches(M, N, K)),
-                  lib.momoe_fp8_experts_forward, ptr(data), ptr(scale), ptr(idx), ptr(w), M, N, K, D, H,
-                  ptr(experts.W1_N2HD), ptr(experts.S1), ptr(experts.W2_NDH), ptr(experts.S2), ops.DECODE_MAX_AVG_ROWS,
-                  ptr(y), ptr(sizes), ptr(ws), nbytes, ptr(ops.status_word(dev)), stream_ptr())
+        ops._call("momoe_fp8_experts_forward", _lib.fp8_experts_launches(M, N, K), lib.momoe_fp8_experts_forward,
+                  data.data_ptr(), scale_ptr, idx.data_ptr(), w.data_ptr(), M, N, K, D, H, experts.W1_N2HD.data_ptr(),
+                  experts.S1.data_ptr(), experts.W2_NDH.data_ptr(), experts.S2.data_ptr(), ops.DECODE_MAX_AVG_ROWS,
+                  y.data_ptr(), sizes.data_ptr(), ws.data_ptr(), nbytes, ops.status_word(dev).data_ptr(),
+                  raw_stream(dev))
     return y, sizes

@@ -10,8 +10,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib, ops
-from ._lib import as_rows, lib, pitch, ptr, stream_ptr
-from .fp8 import BLOCK, Fp8Rows
+from ._lib import aligned, as_rows, lib, on_device, pitch, raw_stream
+from .fp8 import BLOCK, E4M3, E8M0, Fp8Rows
 
 MAX_D = 16384
 
@@ -29,82 +29,98 @@ def _check(x, weight, residual):
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise RuntimeError("the residual must be like x, %s in %s, but got: %s in %s"
                            % (list(x.shape), x.dtype, list(residual.shape), residual.dtype))
-    return dev, D
+    return dev
 
 
-def _weight(w):
-    w = w.detach().contiguous()
-    return w if w.data_ptr() % 16 == 0 else w.clone()
+def _learns(x, weight, residual):
+    return torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                        (residual is not None and residual.requires_grad))
 
 
-def _forward(x, w, residual, eps, want_y, want_rows, want_rstd):
-    """x, residual: rows [M, D].  Returns r (None without a residual), y, rstd, q, scale (None where not wanted)."""
+def _forward(x, weight, residual, eps, want_rows, want_rstd):
+    """Runs the kernel on checked tensors.  Returns the input rows [M, D] (the sum r where there is a residual), the weight
+    as the kernel read it, y, rstd and the 8-bit rows (None where not wanted)."""
+    dev, dtype = x.device, x.dtype
+    x = as_rows(x)
+    w = aligned(weight if weight.is_contiguous() else weight.contiguous())
     M, D = x.shape
-    dev = x.device
-    r = torch.empty((M, D), dtype=x.dtype, device=dev) if residual is not None else None
-    y = torch.empty((M, D), dtype=x.dtype, device=dev) if want_y else None
-    rstd = torch.empty(M, dtype=torch.float32, device=dev) if want_rstd else None
-    q = scale = None
+    y = torch.empty((M, D), dtype=dtype, device=dev)
+    r = rstd = rows = res_ptr = r_ptr = None
+    res_pitch = 0
+    if residual is not None:
+        residual = as_rows(residual)
+        r = torch.empty((M, D), dtype=dtype, device=dev)
+        res_ptr, r_ptr, res_pitch = residual.data_ptr(), r.data_ptr(), pitch(residual)
+    if want_rstd:
+        rstd = torch.empty(M, dtype=torch.float32, device=dev)
     if want_rows:
-        q = torch.empty((M, D), dtype=torch.float8_e4m3fn, device=dev)
-        scale = torch.empty((M, -(-D // BLOCK)), dtype=torch.float8_e8m0fnu, device=dev)
+        rows = Fp8Rows(torch.empty((M, D), dtype=E4M3, device=dev), torch.empty((M, -(-D // BLOCK)), dtype=E8M0, device=dev))
     if M > 0:
-        ops._call("momoe_rms_norm", 1, lib.momoe_rms_norm, ptr(x), pitch(x), ptr(residual),
-                  pitch(residual) if residual is not None else 0, ptr(w), _lib.TYPES[x.dtype], _lib.TYPES[w.dtype], M, D,
-                  eps, ptr(r), ptr(y), ptr(rstd), ptr(q), ptr(scale), stream_ptr())
-    return r, y, rstd, q, scale
+        ops._call("momoe_rms_norm", 1, lib.momoe_rms_norm, x.data_ptr(), pitch(x), res_ptr, res_pitch, w.data_ptr(),
+                  _lib.TYPES[dtype], _lib.TYPES[w.dtype], M, D, eps, r_ptr, y.data_ptr(),
+                  rstd.data_ptr() if want_rstd else None, rows.q.data_ptr() if want_rows else None,
+                  rows.scale.data_ptr() if want_rows else None, raw_stream(dev))
+    return (x if r is None else r), w, y, rstd, rows
 
 
 class RMSNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        dev, D = _check(x, weight, residual)
         ctx.set_materialize_grads(False)
-        w = _weight(weight)
-        with torch.cuda.device(dev):
-            rows = as_rows(x.detach())
-            res = as_rows(residual.detach()) if residual is not None else None
-            r, y, rstd, _, _ = _forward(rows, w, res, eps, True, False, any(ctx.needs_input_grad))
-        ctx.save_for_backward(r if r is not None else rows, w, rstd)
-        y = y.view(x.shape)
-        return (y, r.view(x.shape)) if r is not None else y
+        shape = x.shape
+        with on_device(x.device):
+            r, w, y, rstd, _ = _forward(x, weight, residual, eps, False, True)
+        ctx.save_for_backward(r, w, rstd)
+        ctx.shape = shape
+        if len(shape) != 2:
+            y = y.view(shape)
+            r = r.view(shape) if residual is not None else r
+        return (y, r) if residual is not None else y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy, gr=None):
         r, w, rstd = ctx.saved_tensors
-        M, D = r.shape
-        need_x, need_w, need_res = ctx.needs_input_grad[:3]
-        shape = gy.shape if gy is not None else gr.shape if gr is not None else None
-        if shape is None:
-            return None, None, None, None
-        if gy is None:                       # only the sum was used
-            return (gr if need_x else None), (torch.zeros_like(w) if need_w else None), (gr if need_res else None), None
-        dev = r.device
-        with torch.cuda.device(dev):
-            gy = gy.reshape(M, D).contiguous()
-            gy = gy if gy.data_ptr() % 16 == 0 else gy.clone()
+        need_x, need_w, need_res, _ = ctx.needs_input_grad
+        if gy is None:                       # only the sum was used, or nothing
+            gw = torch.zeros_like(w) if need_w and gr is not None else None
+            return (gr if need_x else None), gw, (gr if need_res else None), None
+        D = w.shape[0]
+        dev = w.device
+        with on_device(dev):
+            r = r if r.dim() == 2 else r.view(-1, D)
+            M = r.shape[0]
+            gy = aligned(gy if gy.is_contiguous() else gy.contiguous())
             if gr is not None:
-                gr = gr.reshape(M, D).contiguous()
-                gr = gr if gr.data_ptr() % 16 == 0 else gr.clone()
+                gr = aligned(gr if gr.is_contiguous() else gr.contiguous())
             gx = torch.empty((M, D), dtype=r.dtype, device=dev)
             gw = torch.empty_like(w) if need_w else None
             if M > 0:
-                nbytes = int(lib.momoe_rms_norm_backward_workspace_bytes(M, D)) if need_w else 0
+                nbytes = _lib.rms_norm_backward_workspace_bytes(M, D) if need_w else 0
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if need_w else None
-                ops._call("momoe_rms_norm_backward", 2 if need_w else 1, lib.momoe_rms_norm_backward, ptr(gy), ptr(gr),
-                          ptr(r), pitch(r), ptr(w), ptr(rstd), _lib.TYPES[r.dtype], _lib.TYPES[w.dtype], M, D, ptr(gx),
-                          ptr(gw), ptr(ws), nbytes, stream_ptr())
+                ops._call("momoe_rms_norm_backward", 2 if need_w else 1, lib.momoe_rms_norm_backward, gy.data_ptr(),
+                          gr.data_ptr() if gr is not None else None, r.data_ptr(), pitch(r), w.data_ptr(),
+                          rstd.data_ptr(), _lib.TYPES[r.dtype], _lib.TYPES[w.dtype], M, D, gx.data_ptr(),
+                          gw.data_ptr() if need_w else None, ws.data_ptr() if need_w else None, nbytes, raw_stream(dev))
             elif need_w:
                 gw.zero_()
-        gx = gx.view(shape)
+        if len(ctx.shape) != 2:
+            gx = gx.view(ctx.shape)
         return (gx if need_x else None), gw, (gx if need_res else None), None
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """x [..., D] (bfloat16, float16 or float32; D a multiple of 8 up to 16384), weight [D] in x's type or float32.
     Returns y, or (y, x + residual) when a residual (like x) is given.  Differentiable in x, weight and residual."""
-    return RMSNormFunction.apply(x, weight, residual, float(eps))
+    dev = _check(x, weight, residual)
+    if _learns(x, weight, residual):
+        return RMSNormFunction.apply(x, weight, residual, float(eps))
+    with on_device(dev):
+        r, _, y, _, _ = _forward(x.detach(), weight.detach(), residual.detach() if residual is not None else None,
+                                 float(eps), False, False)
+    if x.dim() != 2:
+        y, r = y.view(x.shape), (r.view(x.shape) if residual is not None else r)
+    return (y, r) if residual is not None else y
 
 
 class Fp8Norm(NamedTuple):
@@ -116,14 +132,15 @@ class Fp8Norm(NamedTuple):
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
     """`rms_norm` that also gives y as 8-bit rows (converted from the 32-bit value, not from the rounded y).  Forward only."""
-    dev, D = _check(x, weight, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    dev = _check(x, weight, residual)
+    if _learns(x, weight, residual):
         raise RuntimeError("rms_norm_fp8 has no backward pass: call it under torch.no_grad()")
-    with torch.cuda.device(dev):
-        r, y, _, q, scale = _forward(as_rows(x.detach()), _weight(weight),
-                                     as_rows(residual.detach()) if residual is not None else None, float(eps), True, True,
-                                     False)
-    return Fp8Norm(y.view(x.shape), Fp8Rows(q, scale), r.view(x.shape) if r is not None else None)
+    with on_device(dev):
+        r, _, y, _, rows = _forward(x.detach(), weight.detach(), residual.detach() if residual is not None else None,
+                                    float(eps), True, False)
+    if x.dim() != 2:
+        y, r = y.view(x.shape), (r.view(x.shape) if residual is not None else r)
+    return Fp8Norm(y, rows, r if residual is not None else None)
 
 
 class RMSNorm(nn.Module):
