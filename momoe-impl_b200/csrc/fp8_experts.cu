@@ -1,12 +1,10 @@
-// Around the 8-bit expert GEMMs: the weights' conversion, the row gather that converts on the way, and one call that runs
-// the whole forward pass (permutation, gather, two GEMMs, combine) out of one workspace.
+// Around the 8-bit expert GEMMs: the weights' conversion, the dispatch of token rows into expert-major order (which converts
+// them on the way), and one call that runs the whole forward pass (dispatch, two GEMMs, combine) out of one workspace.
 #include "fp8.cuh"
 #include "internal.h"
 #include "../../include/momoe_b200.h"
 
 namespace momoe {
-
-int fp8_check_plan(const momoe_plan_t* p);
 
 __device__ __forceinline__ float f8_value(float v) { return v; }
 __device__ __forceinline__ float f8_value(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -58,25 +56,160 @@ __global__ void __launch_bounds__(256) fp8_quantize_weights_kernel(const T* __re
     }
 }
 
+// ------------------------------------------------------------------------------------------------ dispatch
+// Expert-major layout and row conversion in one pass over the tokens.  A thread block has a chunk of tokens; it needs, for
+// each expert, the pairs of all tokens (where the expert's 128-row tiles start) and a row number inside the expert that no
+// other block hands out.
+//   up to DISPATCH_SMALL_PAIRS pairs: every block counts all pairs itself, so the pass is one launch (an id costs a few
+//       cycles, a launch several microseconds);
+//   more: a first kernel counts each chunk and reserves its rows with one atomic for each (chunk, expert).
+// Rows inside an expert are handed out by atomics, in no fixed order.  No result depends on it: a row's values do not
+// depend on its place, and a token's K rows are added in the order of k.
+constexpr int DISPATCH_SMALL_PAIRS = 4096;
+constexpr int DISPATCH_MAX_EXPERTS = 1024;
+constexpr int DISPATCH_MAX_TOPK = 32;
+
+struct DispatchArgs {
+    const void* x;              // bf16 [M, D], or e4m3 with x_scale
+    const uint8_t* x_scale;
+    const int* topk_idx;
+    const float* topk_w;
+    int M, N, K, D;
+    int chunk;                  // tokens of a block
+    int* total;                 // large: pairs of each expert [N]
+    int* chunk_base;            // large: rows reserved before a chunk's own [n_chunks, N]
+    long long* sizes;
+    int* tile_expert;
+    int* pair_info;
+    int* sched;
+    int* row_token;
+    float* row_weight;
+    int* pos;
+    uint8_t* dst;
+    uint8_t* dst_scale;
+    int* status;
+};
+
+__device__ __forceinline__ int dispatch_expert(const DispatchArgs& a, int i, bool report) {
+    const int e = __ldg(a.topk_idx + i);
+    if (e >= 0 && e < a.N) return e;
+    if (report) atomicCAS(a.status, 0, DEV_BAD_EXPERT_ID);
+    return 0;                   // stay in bounds: the pair goes to expert 0, and the report says so
+}
+
+__global__ void __launch_bounds__(256) fp8_count_kernel(const DispatchArgs a) {
+    __shared__ int s_cnt[DISPATCH_MAX_EXPERTS];
+    for (int e = threadIdx.x; e < a.N; e += 256) s_cnt[e] = 0;
+    __syncthreads();
+    const int m0 = blockIdx.x * a.chunk, m1 = min(a.M, m0 + a.chunk);
+    for (int i = m0 * a.K + threadIdx.x; i < m1 * a.K; i += 256) atomicAdd(&s_cnt[dispatch_expert(a, i, true)], 1);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.N; e += 256)
+        if (s_cnt[e] != 0) a.chunk_base[static_cast<size_t>(blockIdx.x) * a.N + e] = atomicAdd(a.total + e, s_cnt[e]);
+}
+
+// 16 columns of a row as e4m3, scaled by `inv`.
+__device__ __forceinline__ uint4 fp8_convert16(const float (&v)[16], float inv) {
+    uint4 o;
+    o.x = fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    o.y = fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+    o.z = fp8_pack4(v[8] * inv, v[9] * inv, v[10] * inv, v[11] * inv);
+    o.w = fp8_pack4(v[12] * inv, v[13] * inv, v[14] * inv, v[15] * inv);
+    return o;
+}
+
 // One warp a token: its row is read once, converted (ROWS8: copied) and stored to the K expert-major rows of its experts,
 // the scales in the blocks the GEMMs read.  A lane holds 16 columns, 8 lanes a block of 128, the warp the 512 columns
 // whose four scale bytes make one word.  Bound by HBM: M D (2 + K) bytes from 16-bit rows, M D (1 + K) from 8-bit ones.
-// Padding rows are left as they are.  A token that names an expert twice would have both copies in one row: reported.
-template <bool ROWS8>
-__global__ void __launch_bounds__(256) fp8_gather_kernel(const void* __restrict__ x, const uint8_t* __restrict__ x_scale,
-                                                         const int* __restrict__ pos_MK, int M, int K, int D,
-                                                         uint8_t* __restrict__ dst, uint8_t* __restrict__ dst_scale,
-                                                         int* status) {
+// Padding rows of dst are left as they are.
+template <bool ROWS8, bool SMALL>
+__global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a) {
+    __shared__ int s_next[DISPATCH_MAX_EXPERTS];     // next row of each expert for this block
+    __shared__ int s_total[DISPATCH_MAX_EXPERTS];
+    __shared__ unsigned s_first[DISPATCH_MAX_EXPERTS];    // first tile | first pair << 16 of each expert
+    __shared__ unsigned s_warp[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int m0 = blockIdx.x * a.chunk, m1 = min(a.M, m0 + a.chunk);
+    const bool first = blockIdx.x == 0;
+    if constexpr (SMALL) {
+        for (int e = tid; e < a.N; e += 256) s_next[e] = s_total[e] = 0;
+        __syncthreads();
+        const int before = m0 * a.K;
+        for (int i = tid; i < a.M * a.K; i += 256) {
+            const int e = dispatch_expert(a, i, first);
+            atomicAdd(&s_total[e], 1);
+            if (i < before) atomicAdd(&s_next[e], 1);
+        }
+    } else {
+        // experts that the chunk does not name have no entry in chunk_base: what is read there is not used
+        for (int e = tid; e < a.N; e += 256) {
+            s_total[e] = __ldg(a.total + e);
+            s_next[e] = __ldg(a.chunk_base + static_cast<size_t>(blockIdx.x) * a.N + e);
+        }
+    }
+    __syncthreads();
+    // exclusive scan of tiles (low half) and tile pairs (high half) over the experts, four of them a thread
+    unsigned mine[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int e = tid * 4 + j;
+        const unsigned nt = e < a.N ? static_cast<unsigned>(s_total[e] + TILE_M - 1) / TILE_M : 0u;
+        mine[j] = sum;
+        sum += nt | ((nt + 1) / 2) << 16;
+    }
+    unsigned incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    unsigned base = incl - sum, all = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i < warp) base += s_warp[i];
+        all += s_warp[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (tid * 4 + j < a.N) s_first[tid * 4 + j] = base + mine[j];
+    __syncthreads();
+    if (first && tid == 0) {
+        a.sched[SCHED_N_TILES] = static_cast<int>(all & 0xFFFFu);
+        a.sched[SCHED_N_SAVED_TILES] = 0;
+        a.sched[SCHED_PAD_ROWS] = static_cast<int>((all & 0xFFFFu) * TILE_M);
+        a.sched[SCHED_N_PAIRS] = static_cast<int>(all >> 16);
+    }
+    // the tables of the tiles, and token -1 on padding rows: the experts are shared out among the blocks
+    for (int e = blockIdx.x * 8 + warp; e < a.N; e += gridDim.x * 8) {
+        const int cnt = s_total[e], t0 = static_cast<int>(s_first[e] & 0xFFFFu), p0 = static_cast<int>(s_first[e] >> 16);
+        const int nt = (cnt + TILE_M - 1) / TILE_M;
+        for (int t = lane; t < nt; t += 32) {
+            a.tile_expert[t0 + t] = e;
+            if ((t & 1) == 0) a.pair_info[p0 + t / 2] = (t0 + t) * 2 + (t + 1 < nt ? 1 : 0);
+        }
+        for (int r = cnt + lane; r < nt * TILE_M; r += 32) {
+            a.row_token[t0 * TILE_M + r] = -1;
+            a.row_weight[t0 * TILE_M + r] = 0.0f;
+        }
+        if (lane == 0) a.sizes[e] = cnt;
+    }
+
     constexpr int U = 4;             // groups of 512 columns in flight
-    const int lane = threadIdx.x & 31;
-    const int warps_total = gridDim.x * 8;
-    const int n_chunks = D >> 4;
-    const int n_blocks = (D + FP8_BLOCK - 1) / FP8_BLOCK;
+    const int n_chunks = a.D >> 4;
+    const int n_blocks = (a.D + FP8_BLOCK - 1) / FP8_BLOCK;
     const int n_groups = (n_blocks + FP8_GROUP - 1) / FP8_GROUP;
-    for (int m = blockIdx.x * 8 + (threadIdx.x >> 5); m < M; m += warps_total) {
-        const int p = lane < K ? __ldg(pos_MK + static_cast<size_t>(m) * K + lane) : -1 - lane;
-        const unsigned same = __match_any_sync(0xffffffffu, p);
-        if ((same & (same - 1u)) != 0u) atomicCAS(status, 0, DEV_REPEATED_EXPERT);
+    for (int m = m0 + warp; m < m1; m += 8) {
+        int p = 0;
+        if (lane < a.K) {
+            const int i = m * a.K + lane;
+            const int e = dispatch_expert(a, i, false);
+            p = static_cast<int>(s_first[e] & 0xFFFFu) * TILE_M + atomicAdd(&s_next[e], 1);
+            a.pos[i] = p;
+            a.row_token[p] = m;
+            a.row_weight[p] = __ldg(a.topk_w + i);
+        }
         for (int g0 = 0; g0 < n_groups; g0 += U) {
             uint4 lo[U], hi[U];
             uint32_t byte[U];
@@ -87,10 +220,10 @@ __global__ void __launch_bounds__(256) fp8_gather_kernel(const void* __restrict_
                 byte[u] = 127u;
                 if (c < n_chunks) {
                     if constexpr (ROWS8) {
-                        lo[u] = __ldg(static_cast<const uint4*>(x) + static_cast<size_t>(m) * n_chunks + c);
-                        byte[u] = __ldg(x_scale + static_cast<size_t>(m) * n_blocks + (c >> 3));
+                        lo[u] = __ldg(static_cast<const uint4*>(a.x) + static_cast<size_t>(m) * n_chunks + c);
+                        byte[u] = __ldg(a.x_scale + static_cast<size_t>(m) * n_blocks + (c >> 3));
                     } else {
-                        const uint4* src = static_cast<const uint4*>(x) + (static_cast<size_t>(m) * n_chunks + c) * 2;
+                        const uint4* src = static_cast<const uint4*>(a.x) + (static_cast<size_t>(m) * n_chunks + c) * 2;
                         lo[u] = __ldg(src);
                         hi[u] = __ldg(src + 1);
                     }
@@ -114,28 +247,29 @@ __global__ void __launch_bounds__(256) fp8_gather_kernel(const void* __restrict_
 #pragma unroll
                     for (int d = 4; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
                     byte[u] = fp8_scale_byte(top);
-                    const float inv = fp8_inv_scale(byte[u]);
-                    o.x = fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-                    o.y = fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-                    o.z = fp8_pack4(v[8] * inv, v[9] * inv, v[10] * inv, v[11] * inv);
-                    o.w = fp8_pack4(v[12] * inv, v[13] * inv, v[14] * inv, v[15] * inv);
+                    o = fp8_convert16(v, fp8_inv_scale(byte[u]));
                 }
                 const uint32_t word = __reduce_or_sync(0xffffffffu, (lane & 7) == 0 ? byte[u] << lane : 0u);
-                if (lane < K)
-                    *reinterpret_cast<uint32_t*>(dst_scale + fp8_atom_offset(p, g0 + u, n_groups)) = word;
-                for (int k = 0; k < K; ++k) {
+                if (lane < a.K)
+                    *reinterpret_cast<uint32_t*>(a.dst_scale + fp8_atom_offset(p, g0 + u, n_groups)) = word;
+                for (int k = 0; k < a.K; ++k) {
                     const size_t row = static_cast<size_t>(__shfl_sync(0xffffffffu, p, k));
-                    if (c < n_chunks) *reinterpret_cast<uint4*>(dst + row * D + static_cast<size_t>(c) * 16) = o;
+                    if (c < n_chunks) *reinterpret_cast<uint4*>(a.dst + row * a.D + static_cast<size_t>(c) * 16) = o;
                 }
             }
         }
     }
 }
 
+static bool dispatch_small(int M, int K) { return static_cast<long long>(M) * K <= DISPATCH_SMALL_PAIRS; }
+// Tokens of a block: one a warp where every block counts all pairs anyway, four a warp where a chunk has a set-up of its own.
+static int dispatch_chunk(int M, int K) { return dispatch_small(M, K) ? 8 : 32; }
+
 // Parts of the workspace of a whole forward pass, each on a 256-byte boundary.
 struct Fp8Workspace {
-    size_t cumsums, idx, which, pad_off, tile_expert, pair_info, sched, row_token, row_weight, pos, perm, x_scale, h,
-        h_scale, rows, bytes;
+    size_t tile_expert, pair_info, sched, row_token, row_weight, pos, dispatch, dispatch_bytes, x_scale, h, h_scale, rows,
+        bytes;
+    long long tiles;
 };
 static Fp8Workspace fp8_workspace(int M, int N, int K, int D, int H) {
     Fp8Workspace w;
@@ -145,19 +279,18 @@ static Fp8Workspace fp8_workspace(int M, int N, int K, int D, int H) {
         at += (bytes + 255) & ~static_cast<size_t>(255);
         return o;
     };
-    const size_t tiles = static_cast<size_t>(momoe_tile_capacity(M, K, N)), rows = tiles * TILE_M;
     const size_t msum = static_cast<size_t>(M) * K;
-    w.cumsums = take((N + 1) * 4);
-    w.idx = take(msum * 4);
-    w.which = take(msum * 4);
-    w.pad_off = take((N + 1) * 4);
+    // an expert without a token has no tile: fewer than momoe_tile_capacity when there are fewer pairs than experts
+    const size_t tiles = (msum + TILE_M - 1) / TILE_M + (msum < static_cast<size_t>(N) ? msum : N), rows = tiles * TILE_M;
+    w.tiles = static_cast<long long>(tiles);
     w.tile_expert = take(tiles * 4);
     w.pair_info = take(tiles * 4);
     w.sched = take(SCHED_WORDS * 4);
     w.row_token = take(rows * 4);
     w.row_weight = take(rows * 4);
     w.pos = take(msum * 4);
-    w.perm = take(momoe_permutation_workspace_bytes(M, N, K));
+    w.dispatch_bytes = momoe_fp8_dispatch_workspace_bytes(M, N, K);
+    w.dispatch = take(w.dispatch_bytes);
     w.x_scale = take(tiles * ((D + 511) / 512) * FP8_ATOM);
     w.h = take(rows * H);
     w.h_scale = take(tiles * ((H + 511) / 512) * FP8_ATOM);
@@ -188,24 +321,55 @@ MOMOE_API int momoe_fp8_quantize_weights(const void* W, int32_t type, int32_t N,
     return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
 
-MOMOE_API int momoe_fp8_gather_rows(const momoe_plan_t* plan, const void* x, const uint8_t* x_scale, uint8_t* dst_sorted,
-                                    uint8_t* dst_scale, momoe_stream_t stream) {
-    int rc = fp8_check_plan(plan);
-    if (rc != MOMOE_OK) return rc;
-    if (x == nullptr || dst_sorted == nullptr || dst_scale == nullptr) return MOMOE_ERR_ARG;
+MOMOE_API size_t momoe_fp8_dispatch_workspace_bytes(int32_t M, int32_t N, int32_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || dispatch_small(M, K)) return 0;
+    const int c = dispatch_chunk(M, K);
+    return (1 + static_cast<size_t>((M + c - 1) / c)) * N * 4;
+}
+
+MOMOE_API int momoe_fp8_dispatch_rows(const void* x, const uint8_t* x_scale, const int32_t* topk_idx_MK,
+                                      const float* topk_w_MK, int32_t M, int32_t N, int32_t K, int32_t D,
+                                      int64_t* sizes_N, int32_t* tile_expert, int32_t* pair_info, int32_t* sched,
+                                      int32_t* row_token, float* row_weight, int32_t* pos_MK, int64_t rows_capacity,
+                                      void* workspace, size_t workspace_bytes, uint8_t* dst_sorted, uint8_t* dst_scale,
+                                      int32_t* status, momoe_stream_t stream) {
+    if (x == nullptr || topk_idx_MK == nullptr || topk_w_MK == nullptr || sizes_N == nullptr || tile_expert == nullptr ||
+        pair_info == nullptr || sched == nullptr || row_token == nullptr || row_weight == nullptr || pos_MK == nullptr ||
+        dst_sorted == nullptr || dst_scale == nullptr || status == nullptr)
+        return MOMOE_ERR_ARG;
+    if (M <= 0 || N <= 0 || K <= 0 || K > N || D <= 0) return MOMOE_ERR_ARG;
+    if (D % 16 != 0) return MOMOE_ERR_UNSUPPORTED;
+    if (N > DISPATCH_MAX_EXPERTS || K > DISPATCH_MAX_TOPK) return MOMOE_ERR_TOO_LARGE;
+    // tiles and pairs share a word in the scan
+    const int64_t msum = static_cast<int64_t>(M) * K, tiles = (msum + TILE_M - 1) / TILE_M + (msum < N ? msum : N);
+    if (tiles > 0xFFFF) return MOMOE_ERR_TOO_LARGE;
+    if (rows_capacity < tiles * TILE_M) return MOMOE_ERR_ARG;
     if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(dst_sorted) |
           reinterpret_cast<uintptr_t>(dst_scale)) & 15) != 0)
         return MOMOE_ERR_ARG;
-    if (plan->K > 32) return MOMOE_ERR_TOO_LARGE;
-    const int want = (plan->M + 7) / 8, cap = sm_count() * 8;
-    const int grid = want < cap ? want : cap;
+    const size_t need = momoe_fp8_dispatch_workspace_bytes(M, N, K);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return MOMOE_ERR_ARG;
+    DispatchArgs a;
+    a.x = x; a.x_scale = x_scale; a.topk_idx = topk_idx_MK; a.topk_w = topk_w_MK;
+    a.M = M; a.N = N; a.K = K; a.D = D;
+    a.chunk = dispatch_chunk(M, K);
+    a.total = static_cast<int*>(workspace);
+    a.chunk_base = need > 0 ? a.total + N : nullptr;
+    a.sizes = reinterpret_cast<long long*>(sizes_N);
+    a.tile_expert = tile_expert; a.pair_info = pair_info; a.sched = sched;
+    a.row_token = row_token; a.row_weight = row_weight; a.pos = pos_MK;
+    a.dst = dst_sorted; a.dst_scale = dst_scale; a.status = status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (x_scale != nullptr)
-        fp8_gather_kernel<true><<<grid, 256, 0, st>>>(x, x_scale, plan->pos_MK, plan->M, plan->K, plan->D, dst_sorted,
-                                                      dst_scale, plan->status);
-    else
-        fp8_gather_kernel<false><<<grid, 256, 0, st>>>(x, x_scale, plan->pos_MK, plan->M, plan->K, plan->D, dst_sorted,
-                                                       dst_scale, plan->status);
+    const int grid = (M + a.chunk - 1) / a.chunk;
+    if (need == 0) {
+        if (x_scale != nullptr) fp8_dispatch_kernel<true, true><<<grid, 256, 0, st>>>(a);
+        else fp8_dispatch_kernel<false, true><<<grid, 256, 0, st>>>(a);
+    } else {
+        if (cudaMemsetAsync(a.total, 0, static_cast<size_t>(N) * 4, st) != cudaSuccess) return MOMOE_ERR_CUDA;
+        fp8_count_kernel<<<grid, 256, 0, st>>>(a);
+        if (x_scale != nullptr) fp8_dispatch_kernel<true, false><<<grid, 256, 0, st>>>(a);
+        else fp8_dispatch_kernel<false, false><<<grid, 256, 0, st>>>(a);
+    }
     return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
 
@@ -215,13 +379,14 @@ MOMOE_API size_t momoe_fp8_experts_workspace_bytes(int32_t M, int32_t N, int32_t
 }
 
 MOMOE_API int momoe_fp8_experts_launches(int32_t M, int32_t N, int32_t K) {
-    return momoe_permutation_launches(M, N, K) + 4;
+    (void)N;
+    return dispatch_small(M, K) ? 4 : 5;
 }
 
 MOMOE_API int momoe_fp8_experts_forward(const void* x_MD, const uint8_t* x_scale, const int32_t* topk_idx_MK,
                                         const float* topk_w_MK, int32_t M, int32_t N, int32_t K, int32_t D, int32_t H,
                                         const uint8_t* W1_N2HD, const uint8_t* S1, const uint8_t* W2_NDH,
-                                        const uint8_t* S2, int32_t decode_max_avg_rows, void* y_MD, int64_t* sizes_N,
+                                        const uint8_t* S2, int32_t stream_max_avg_rows, void* y_MD, int64_t* sizes_N,
                                         void* workspace, size_t workspace_bytes, int32_t* status,
                                         momoe_stream_t stream) {
     if (M <= 0 || N <= 0 || K <= 0 || D <= 0 || H <= 0) return MOMOE_ERR_ARG;
@@ -235,23 +400,22 @@ MOMOE_API int momoe_fp8_experts_forward(const void* x_MD, const uint8_t* x_scale
     auto u8 = [&](size_t at) { return reinterpret_cast<uint8_t*>(ws + at); };
     momoe_plan_t plan;
     plan.M = M; plan.N = N; plan.K = K; plan.D = D; plan.H = H; plan.reserved = 0;
-    plan.rows_capacity = momoe_sorted_rows_capacity(M, K, N);
+    plan.rows_capacity = l.tiles * TILE_M;
     plan.sched = i32(l.sched);
     plan.tile_expert = i32(l.tile_expert);
-    plan.pad_off = i32(l.pad_off);
+    plan.pad_off = nullptr;
     plan.row_token = i32(l.row_token);
     plan.row_weight = reinterpret_cast<float*>(ws + l.row_weight);
     plan.pos_MK = i32(l.pos);
     plan.status = status;
     plan.pair_info = i32(l.pair_info);
-    int rc = momoe_build_permutation(topk_idx_MK, topk_w_MK, M, N, K, 0, sizes_N, i32(l.cumsums), i32(l.idx),
-                                     i32(l.which), i32(l.pad_off), i32(l.tile_expert), i32(l.pair_info), i32(l.sched),
-                                     i32(l.row_token), reinterpret_cast<float*>(ws + l.row_weight), i32(l.pos),
-                                     plan.rows_capacity, ws + l.perm, l.x_scale - l.perm, status, stream);
+    int rc = momoe_fp8_dispatch_rows(x_MD, x_scale, topk_idx_MK, topk_w_MK, M, N, K, D, sizes_N, i32(l.tile_expert),
+                                     i32(l.pair_info), i32(l.sched), i32(l.row_token),
+                                     reinterpret_cast<float*>(ws + l.row_weight), i32(l.pos), plan.rows_capacity,
+                                     ws + l.dispatch, l.dispatch_bytes, u8(l.rows), u8(l.x_scale), status, stream);
     if (rc != MOMOE_OK) return rc;
-    if ((rc = momoe_fp8_gather_rows(&plan, x_MD, x_scale, u8(l.rows), u8(l.x_scale), stream)) != MOMOE_OK) return rc;
-    // as for 16-bit experts: with few rows an expert, the kernels that stream the weights
-    const bool decode = static_cast<int64_t>(M) * K <= static_cast<int64_t>(decode_max_avg_rows) * N;
+    // with few rows an expert, the kernels that stream the weights
+    const bool decode = static_cast<int64_t>(M) * K <= static_cast<int64_t>(stream_max_avg_rows) * N;
     rc = decode ? momoe_fp8_up_swiglu_decode(&plan, u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream)
                 : momoe_fp8_up_swiglu(&plan, u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream);
     if (rc != MOMOE_OK) return rc;

@@ -74,7 +74,9 @@ _PROTOS = {
     "momoe_balance_loss_backward": (C.c_int, [c_vp, c_i32, c_vp, c_i32, c_vp, c_i32, c_i32, c_i32, c_i32, C.c_float,
                                               c_vp, c_vp, c_vp, c_vp]),
     "momoe_fp8_quantize_weights": (C.c_int, [c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp]),
-    "momoe_fp8_gather_rows": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "momoe_fp8_dispatch_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
+    "momoe_fp8_dispatch_rows": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                          c_vp, c_vp, c_i64, c_vp, c_sz, c_vp, c_vp, c_vp, c_vp]),
     "momoe_fp8_up_swiglu": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "momoe_fp8_up_swiglu_decode": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "momoe_fp8_down_scale": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),

@@ -13,6 +13,8 @@ from . import _lib, ops
 from ._lib import aligned, as_rows, lib, on_device, pitch, ptr, raw_stream
 
 BLOCK = 128                      # values that share a scale
+# Calls with at most this many rows per expert on average stream the weights past the rows; more take the row-tile kernels.
+STREAM_MAX_AVG_ROWS = 96
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -101,10 +103,10 @@ def experts_forward(x, topk_idx_MK, topk_w_MK, experts):
     """Weighted sum of the K chosen experts' outputs for each token, in 8 bits.
 
     x: bfloat16 [M, D] (converted on the way; other float types are cast to bfloat16 first), or Fp8Rows;
-    topk_idx_MK int32 [M, K]: distinct expert ids; topk_w_MK float32 [M, K]; experts: Fp8Experts.  D, H multiples of 16,
+    topk_idx_MK int32 [M, K]: expert ids (one named twice counts with both weights); topk_w_MK float32 [M, K]; experts: Fp8Experts.  D, H multiples of 16,
     N <= 1024, K <= 32.  Returns (y bfloat16 [M, D], tokens_per_expert_N int64 [N]).  The hidden values are converted to
-    8-bit rows once, from 32 bits.  No host synchronisation: an expert id out of range (202) or a token that names an
-    expert twice (203) is reported through the device's status word like the other problems only the device can see."""
+    8-bit rows once, from 32 bits.  No host synchronisation: an expert id out of range (202) is reported through the
+    device's status word like the other problems only the device can see."""
     rows8 = isinstance(x, Fp8Rows)
     data = x.q if rows8 else x
     dev = _lib.require_one_device(data, x.scale if rows8 else None, topk_idx_MK, topk_w_MK, *experts)
@@ -152,7 +154,7 @@ def experts_forward(x, topk_idx_MK, topk_w_MK, experts):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         ops._call("momoe_fp8_experts_forward", _lib.fp8_experts_launches(M, N, K), lib.momoe_fp8_experts_forward,
                   data.data_ptr(), scale_ptr, idx.data_ptr(), w.data_ptr(), M, N, K, D, H, experts.W1_N2HD.data_ptr(),
-                  experts.S1.data_ptr(), experts.W2_NDH.data_ptr(), experts.S2.data_ptr(), ops.DECODE_MAX_AVG_ROWS,
+                  experts.S1.data_ptr(), experts.W2_NDH.data_ptr(), experts.S2.data_ptr(), STREAM_MAX_AVG_ROWS,
                   y.data_ptr(), sizes.data_ptr(), ws.data_ptr(), nbytes, ops.status_word(dev).data_ptr(),
                   raw_stream(dev))
     return y, sizes

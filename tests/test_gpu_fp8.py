@@ -23,6 +23,8 @@ SHAPES = [
     (257, 3, 1, 2176, 128, 0.0),
     (129, 1, 1, 128, 4096, 0.0),
     (640, 5, 3, 4096, 48, 0.0),
+    (90, 40, 6, 256, 144, 3.0),       # few rows on average, some experts with several 32-row blocks
+    (1400, 1000, 3, 64, 32, 1.0),     # many experts, more pairs than one launch dispatches
 ]
 
 
@@ -53,7 +55,7 @@ def value(q, scale):
     return q.double() * wide(scale.double(), q.shape[-1])
 
 
-def weights(fp8, N, D, H, seed):
+def weights(fp8, N, D, H, seed):      # channels of unlike size
     g = torch.Generator().manual_seed(seed)
     W1 = (torch.randn(N, D, 2 * H, generator=g) * torch.exp(torch.randn(N, D, 1, generator=g)) / D ** 0.5).bfloat16().cuda()
     W2 = (torch.randn(N, H, D, generator=g) / H ** 0.5).bfloat16().cuda()
@@ -134,39 +136,101 @@ def test_quantize_experts(fp8, N, D, H):
             assert torch.equal(q.float(), (w / step).float().to(torch.float8_e4m3fn).float())
 
 
-@pytest.mark.parametrize("decode", [False, True])
+class Stages:
+    """The tables and buffers of one forward pass, as the whole call carves them from its workspace."""
+
+    def __init__(self, M, N, K, D, H):
+        from momoe import _lib, ops
+        self.lib, self.ptr, self.st, self.status = _lib.lib, _lib.ptr, _lib.stream_ptr(), ops.status_word("cuda")
+        self.check = _lib.check
+        tiles = -(-M * K // 128) + min(N, M * K)
+        rows = tiles * 128
+        i32 = lambda n: torch.full((n,), 77, dtype=torch.int32, device="cuda")
+        u8 = lambda n: torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")
+        self.sizes = torch.empty(N, dtype=torch.int64, device="cuda")
+        self.tile_expert, self.pair_info, self.sched, self.row_token, self.pos = i32(tiles), i32(tiles), i32(8), i32(rows), i32(M * K)
+        self.row_weight = torch.full((rows,), float("nan"), device="cuda")
+        self.xs, self.xsc = u8(rows * D), u8(tiles * -(-D // 512) * 512)
+        self.hs, self.hsc = u8(rows * H), u8(tiles * -(-H // 512) * 512)
+        self.ys = torch.full((rows, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+        self.M, self.N, self.K, self.D, self.H, self.rows, self.tiles = M, N, K, D, H, rows, tiles
+        p = lambda t: t.data_ptr()
+        self.c = _lib.Plan(M=M, N=N, K=K, D=D, H=H, reserved=0, rows_capacity=rows, sched=p(self.sched),
+                           tile_expert=p(self.tile_expert), pad_off=0, row_token=p(self.row_token),
+                           row_weight=p(self.row_weight), pos_MK=p(self.pos), status=p(self.status), pair_info=p(self.pair_info))
+
+    def dispatch(self, x, scale, idx, w):
+        nbytes = self.lib.momoe_fp8_dispatch_workspace_bytes(self.M, self.N, self.K)
+        ws = torch.full((max(nbytes, 1),), 0x7F, dtype=torch.uint8, device="cuda")
+        p = self.ptr
+        self.check(self.lib.momoe_fp8_dispatch_rows(p(x), p(scale), p(idx), p(w), self.M, self.N, self.K, self.D,
+                                                    p(self.sizes), p(self.tile_expert), p(self.pair_info), p(self.sched),
+                                                    p(self.row_token), p(self.row_weight), p(self.pos), self.rows, p(ws),
+                                                    nbytes, p(self.xs), p(self.xsc), p(self.status), self.st), "dispatch")
+
+    def gemms(self, e, stream):
+        import ctypes
+        ref, p, L = ctypes.byref(self.c), self.ptr, self.lib
+        up, down = ((L.momoe_fp8_up_swiglu_decode, L.momoe_fp8_down_scale_decode) if stream
+                    else (L.momoe_fp8_up_swiglu, L.momoe_fp8_down_scale))
+        self.check(up(ref, p(self.xs), p(self.xsc), p(e.W1_N2HD), p(e.S1), p(self.hs), p(self.hsc), self.st), "up")
+        self.check(down(ref, p(self.hs), p(self.hsc), p(e.W2_NDH), p(e.S2), p(self.ys), self.st), "down")
+
+    def combine(self):
+        import ctypes
+        y = torch.empty(self.M, self.D, dtype=torch.bfloat16, device="cuda")
+        self.check(self.lib.momoe_combine_rows(ctypes.byref(self.c), self.ptr(self.ys), self.D, self.ptr(y), self.st), "combine")
+        return y
+
+
+def check_tables(s, idx, w):
+    """The layout against its definition: whole tiles of one expert each, every pair in a row of its own."""
+    sizes = torch.bincount(idx.flatten().long(), minlength=s.N)
+    assert torch.equal(s.sizes, sizes)
+    nt = -(-sizes // 128)
+    T = int(nt.sum())
+    assert s.sched.tolist()[:4] == [T, 0, T * 128, int((-(-nt // 2)).sum())]
+    assert torch.equal(s.tile_expert[:T].long(), torch.repeat_interleave(torch.arange(s.N, device="cuda"), nt))
+    pairs, t0 = [], 0
+    for n in nt.tolist():
+        pairs += [(t0 + j) * 2 + (1 if j + 1 < n else 0) for j in range(0, n, 2)]
+        t0 += n
+    assert s.pair_info[:len(pairs)].tolist() == pairs
+    tok, wt, pos = s.row_token[:T * 128], s.row_weight[:T * 128], s.pos.long()
+    assert len(pos.unique()) == s.M * s.K and int((tok >= 0).sum()) == s.M * s.K
+    assert torch.equal(tok[pos], torch.arange(s.M, device="cuda").int().repeat_interleave(s.K))
+    assert torch.equal(wt[pos], w.flatten()) and not wt[tok < 0].any()
+    assert torch.equal(s.tile_expert[pos // 128], idx.flatten())
+    first = torch.repeat_interleave((nt.cumsum(0) - nt) * 128, nt * 128)
+    at = torch.arange(T * 128, device="cuda") - first           # place inside the expert: real rows first
+    assert torch.equal(tok >= 0, at < torch.repeat_interleave(sizes, nt * 128))
+
+
+@pytest.mark.parametrize("stream", [False, True])
 @pytest.mark.parametrize("M,N,K,D,H,skew", SHAPES)
-def test_stages_against_64_bits(fp8, M, N, K, D, H, skew, decode):
-    from momoe import _lib, ops
-    lib, ptr, st = _lib.lib, _lib.ptr, _lib.stream_ptr()
+def test_stages_against_64_bits(fp8, monkeypatch, M, N, K, D, H, skew, stream):
+    from momoe import ops
     idx, w = routing(M, N, K, M + D, skew)
-    W1, W2 = weights(fp8, N, D, H, D + H)
-    e = fp8.quantize_experts(W1, W2)
-    plan = ops.RoutingPlan.from_topk(idx, w, N, D, H)
+    e = fp8.quantize_experts(*weights(fp8, N, D, H, D + H))
     g = torch.Generator().manual_seed(1)
     x = torch.randn(M, D, generator=g).bfloat16().cuda()
-    rows, tiles = plan.rows_capacity, plan.tile_capacity
-    u8 = lambda n: torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")
-    xs, xsc, hs, hsc = u8(rows * D), u8(tiles * -(-D // 512) * 512), u8(rows * H), u8(tiles * -(-H // 512) * 512)
-    ys = torch.full((rows, D), float("nan"), dtype=torch.bfloat16, device="cuda")
-    _lib.check(lib.momoe_fp8_gather_rows(plan.ref, ptr(x), None, ptr(xs), ptr(xsc), st), "gather")
-    up, down = ((lib.momoe_fp8_up_swiglu_decode, lib.momoe_fp8_down_scale_decode) if decode
-                else (lib.momoe_fp8_up_swiglu, lib.momoe_fp8_down_scale))
-    _lib.check(up(plan.ref, ptr(xs), ptr(xsc), ptr(e.W1_N2HD), ptr(e.S1), ptr(hs), ptr(hsc), st), "up")
-    _lib.check(down(plan.ref, ptr(hs), ptr(hsc), ptr(e.W2_NDH), ptr(e.S2), ptr(ys), st), "down")
+    s = Stages(M, N, K, D, H)
+    s.dispatch(x, None, idx, w)
+    s.gemms(e, stream)
     torch.cuda.synchronize()
     ops.check_status()
-    real = (plan.row_token >= 0).nonzero().flatten()
-    token = plan.row_token[real].long()
-    expert = plan.tile_expert[real // 128].long()
-    # gather: the converted row of each token, bit for bit
+    check_tables(s, idx, w)
+    real = s.pos.long()
+    token = torch.arange(M, device="cuda").repeat_interleave(K)
+    expert = idx.flatten().long()
+    # dispatch: the converted row of each token, bit for bit
     q, scale = rows_of(x.double())
-    xq = xs.view(torch.float8_e4m3fn).view(rows, D)[real]
+    xq = s.xs.view(torch.float8_e4m3fn).view(s.rows, D)[real]
     assert torch.equal(xq.float(), q[token].float())
-    assert torch.equal(unpack_scales(xsc, rows, -(-D // 128))[real], scale[token])
+    assert torch.equal(unpack_scales(s.xsc, s.rows, -(-D // 128))[real], scale[token])
     xv = value(xq, scale[token])
-    hq = hs.view(torch.float8_e4m3fn).view(rows, H)[real]
-    hscale = unpack_scales(hsc, rows, -(-H // 128))[real]
+    hq = s.hs.view(torch.float8_e4m3fn).view(s.rows, H)[real]
+    hscale = unpack_scales(s.hsc, s.rows, -(-H // 128))[real]
     hv = value(hq, hscale)
     W1v = block_values(e.W1_N2HD.view(N, 2, H, D), e.S1)
     W2v = block_values(e.W2_NDH, e.S2)
@@ -176,30 +240,27 @@ def test_stages_against_64_bits(fp8, M, N, K, D, H, skew, decode):
             continue
         a, b = xv[at] @ W1v[n, 0].T, xv[at] @ W1v[n, 1].T
         da, db = ACC * (xv[at].abs() @ W1v[n, 0].abs().T), ACC * (xv[at].abs() @ W1v[n, 1].abs().T)
-        s = torch.sigmoid(b)
-        h = a * b * s
+        sg = torch.sigmoid(b)
+        h = a * b * sg
         # |d(b sigmoid(b))/db| <= 1.1
-        dh = da * (b * s).abs() + 1.1 * db * a.abs() + 1.1 * da * db + 2.0 ** -20 * h.abs()
+        dh = da * (b * sg).abs() + 1.1 * db * a.abs() + 1.1 * da * db + 2.0 ** -20 * h.abs()
         top = torch.nn.functional.pad(h.abs(), (0, -H % 128)).unflatten(-1, (-1, 128)).amax(-1)
         dtop = torch.nn.functional.pad(dh, (0, -H % 128)).unflatten(-1, (-1, 128)).amax(-1)
         sc = hscale[at]
         assert (top - dtop <= 448 * sc).all() and (top + dtop >= 224 * sc).all()
         tol = torch.maximum((h.abs() + dh) * 2.0 ** -4, wide(sc, H) * 2.0 ** -10) + dh
         assert ((hv[at] - h).abs() <= tol).all(), "h of expert %d: %g" % (n, float(((hv[at] - h).abs() / tol).max()))
-        y = hv[at] @ W2v[n].T * plan.row_weight[real[at], None].double()
-        dy = ACC * (hv[at].abs() @ W2v[n].abs().T) * plan.row_weight[real[at], None].double()
-        off = (ys[real[at]].double() - y).abs()
+        wt = w.flatten()[at, None].double()
+        y = hv[at] @ W2v[n].T * wt
+        dy = ACC * (hv[at].abs() @ W2v[n].abs().T) * wt
+        off = (s.ys[real[at]].double() - y).abs()
         assert (off <= 2.0 ** -8 * (y.abs() + dy) + dy).all(), "y of expert %d" % n
     # the whole call is these stages and the combine, bit for bit, from 16-bit and from 8-bit rows
-    want = ops.combine_rows(plan, ys, D)
-    saved = ops.DECODE_MAX_AVG_ROWS
-    try:
-        ops.DECODE_MAX_AVG_ROWS = 2 ** 20 if decode else 0
-        for rows_in in (x, fp8.Fp8Rows(q, scale.to(torch.float8_e8m0fnu)), fp8.quantize_rows(x)):
-            y, sizes = fp8.experts_forward(rows_in, idx, w, e)
-            assert torch.equal(y, want) and torch.equal(sizes, plan.sizes)
-    finally:
-        ops.DECODE_MAX_AVG_ROWS = saved
+    want = s.combine()
+    monkeypatch.setattr(fp8, "STREAM_MAX_AVG_ROWS", 2 ** 20 if stream else 0)
+    for rows_in in (x, fp8.Fp8Rows(q, scale.to(torch.float8_e8m0fnu)), fp8.quantize_rows(x)):
+        y, sizes = fp8.experts_forward(rows_in, idx, w, e)
+        assert torch.equal(y, want) and torch.equal(sizes, s.sizes)
     ops.check_status()
 
 
@@ -257,16 +318,28 @@ def test_capture_other_stream_and_two_graphs(fp8):
     ops.check_status()
 
 
-def test_device_side_reports(fp8):
+def test_an_expert_named_twice_counts_twice_and_bad_ids_are_reported(fp8):
     from momoe import ops
     e = fp8.quantize_experts(*weights(fp8, 8, 64, 32, 1))
-    x = torch.randn(4, 64, device="cuda").bfloat16()
-    w = torch.full((4, 2), 0.5, device="cuda")
+    x = torch.randn(4, 64, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    w = torch.tensor([[0.5, 0.5], [1.0, 0.25], [0.75, 0.25], [0.0, 2.0]], device="cuda")
+    t = lambda ids: torch.tensor(ids, dtype=torch.int32, device="cuda")
     ops.check_status()
-    for ids, code in (([[0, 1], [2, 3], [4, 4], [5, 6]], "203"), ([[0, 1], [2, 8], [4, 5], [5, 6]], "202")):
-        fp8.experts_forward(x, torch.tensor(ids, dtype=torch.int32, device="cuda"), w, e)
-        with pytest.raises(RuntimeError, match=code):
+    y, sizes = fp8.experts_forward(x, t([[0, 1], [2, 3], [4, 4], [5, 6]]), w, e)
+    assert sizes.tolist() == [1, 1, 1, 1, 2, 1, 1, 0]
+    one, _ = fp8.experts_forward(x[2:3], t([[4]]), torch.ones(1, 1, device="cuda"), e)
+    # 0.75 o + 0.25 o: each product and their sum rounded to bfloat16, half a step each
+    assert ((y[2].double() - one[0].double()).abs() <= 3 * 2.0 ** -8 * one[0].double().abs()).all()
+    ops.check_status()
+    for ids in ([[0, 1], [2, 8], [4, 5], [5, 6]], [[0, 1], [2, 3], [4, -1], [5, 6]]):
+        fp8.experts_forward(x, t(ids), w, e)
+        with pytest.raises(RuntimeError, match="202"):
             ops.check_status()
+    many = t([[0, 1]]).expand(5000, 2).clone()               # the two-launch dispatch reports as well
+    many[4321, 1] = 99
+    fp8.experts_forward(x[:1].expand(5000, 64), many, torch.ones(5000, 2, device="cuda"), e)
+    with pytest.raises(RuntimeError, match="202"):
+        ops.check_status()
     ops.check_status()
 
 

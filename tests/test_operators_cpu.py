@@ -68,9 +68,18 @@ def test_fp8_arguments(lib):
     plan = lib.Plan(M=4, N=8, K=2, D=72, H=32, reserved=0, rows_capacity=128 * 9, sched=16, tile_expert=16,
                     pad_off=16, row_token=16, row_weight=16, pos_MK=16, status=16, pair_info=16)
     p = C.byref(plan)
-    assert L.momoe_fp8_gather_rows(p, ONE, None, ONE, ONE, None) == -2           # D not a multiple of 16
+    assert L.momoe_fp8_up_swiglu(p, ONE, ONE, ONE, ONE, ONE, ONE, None) == -2    # D not a multiple of 16
     plan.D = 64
-    assert L.momoe_fp8_gather_rows(p, ONE, None, None, ONE, None) == -1
+    def dispatch(x=ONE, M=4, N=8, K=2, D=64, rows=128 * 9, ws=ONE, n=None, dst=ONE):
+        n = L.momoe_fp8_dispatch_workspace_bytes(M, N, K) if n is None else n
+        return L.momoe_fp8_dispatch_rows(x, None, ONE, ONE, M, N, K, D, ONE, ONE, ONE, ONE, ONE, ONE, ONE, rows, ws, n, dst,
+                                         ONE, ONE, None)
+    assert dispatch(x=None) == -1 and dispatch(D=72) == -2 and dispatch(K=9) == -1 and dispatch(N=1025) == -4
+    assert dispatch(N=40, K=33) == -4 and dispatch(rows=128 * 8) == -1 and dispatch(dst=ODD) == -1
+    assert dispatch(M=5000, rows=1 << 20, n=8) == -1 and dispatch(M=5000, rows=1 << 20, ws=None) == -1
+    assert dispatch(M=8 << 20, rows=1 << 40) == -4                               # more tiles than a table entry counts
+    assert L.momoe_fp8_dispatch_workspace_bytes(4, 8, 2) == 0
+    assert L.momoe_fp8_dispatch_workspace_bytes(5000, 8, 2) == (1 + 157) * 8 * 4
     for f in (L.momoe_fp8_up_swiglu, L.momoe_fp8_up_swiglu_decode):
         assert f(p, ONE, ONE, ONE, None, ONE, ONE, None) == -1 and f(p, ODD, ONE, ONE, ONE, ONE, ONE, None) == -1
         assert f(None, ONE, ONE, ONE, ONE, ONE, ONE, None) == -1
