@@ -13,9 +13,9 @@
 //         the item's 128 columns (the scale of 8-bit rows): a warp reduction for each token and one meeting of four warps
 //   down  an item is 128 columns of y (NT = 32), or 256 in two MMAs, so that a row crosses from L2 half as often (NT = 128)
 //
-// One CTA (224 threads) an SM, persistent over items = (128-row tile, column block).  Warp 0 loads, warp 1 issues MMAs,
-// warps 2..5 are the epilogue (a thread has one weight column and 32 tokens at a time), warp 6 fills the ring of scale slots
-// (see the row-tile kernel for how scales travel).  With NT = 128 there is one accumulator: the MMAs of an item wait for
+// One CTA (320 threads) an SM, persistent over items = (128-row tile, column block).  Warp 0 loads, warp 1 issues MMAs,
+// warps 2..5 are the epilogue (a thread has one weight column and 32 tokens at a time), warps 6..9 write scales to TMEM
+// (see the row-tile kernel).  With NT = 128 there is one accumulator: the MMAs of an item wait for
 // the read-out of the item before, while the ring goes on filling; they need less than half of the time that the
 // weights take.
 #include <cstring>
@@ -29,11 +29,10 @@ namespace momoe {
 
 int fp8_check_plan(const momoe_plan_t* p);
 
-constexpr int D8_THREADS = 224;
+constexpr int D8_THREADS = 320;
 constexpr int D8_K = 128;                        // values of a k slice
 constexpr int D8_W = 128 * D8_K;                 // 16 KiB: 128 weight rows
 constexpr int D8_X = 32 * D8_K;                  // 4 KiB: 32 token rows
-constexpr int D8_SF_SLOTS = 4;
 
 template <bool UP, int NT>
 struct D8 {
@@ -42,8 +41,7 @@ struct D8 {
     static constexpr int SLICE = NW * D8_W + NT / 32 * D8_X;
     static constexpr int STAGE = SL * SLICE;
     static constexpr int STAGES = NT > 32 ? 4 : UP ? 6 : 5;
-    static constexpr int SF = (NW + 1) * FP8_ATOM;
-    static constexpr int SMEM = STAGES * STAGE + D8_SF_SLOTS * SF + 1024;
+    static constexpr int SMEM = STAGES * STAGE + 1024;
     static constexpr int BUFS = NT > 32 ? 1 : 2;             // accumulators
     static constexpr int SF_COL = 256;                       // TMEM: accumulators below, two copies of the scales from here
     static constexpr int TMEM_COLS = 512;
@@ -91,8 +89,8 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bar_full[C::STAGES];
     __shared__ uint64_t bar_empty[C::STAGES];
-    __shared__ uint64_t bar_sf_full[D8_SF_SLOTS];
-    __shared__ uint64_t bar_sf_empty[D8_SF_SLOTS];
+    __shared__ uint64_t bar_sf_full[2];
+    __shared__ uint64_t bar_sf_empty[2];
     __shared__ uint64_t bar_acc_full[C::BUFS];
     __shared__ uint64_t bar_acc_empty[C::BUFS];
     __shared__ uint64_t bar_meet;                    // up: the four epilogue warps have written their part of s_top
@@ -103,7 +101,6 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t stage_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sf_base = stage_base + C::STAGES * C::STAGE;
     const int total_items = __ldg(g.sched + SCHED_N_TILES) * g.n_cblk;
     if (total_items <= 0 || static_cast<int>(blockIdx.x) >= total_items) return;
     const int n_groups = (g.nkb + FP8_GROUP - 1) / FP8_GROUP;
@@ -114,9 +111,9 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
             mbar_init(smem_u32(&bar_full[s]), 1);
             mbar_init(smem_u32(&bar_empty[s]), 1);
         }
-        for (int s = 0; s < D8_SF_SLOTS; ++s) {
-            mbar_init(smem_u32(&bar_sf_full[s]), 1);
-            mbar_init(smem_u32(&bar_sf_empty[s]), 1);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&bar_sf_full[b]), 4);
+            mbar_init(smem_u32(&bar_sf_empty[b]), 1);
         }
         for (int b = 0; b < C::BUFS; ++b) {
             mbar_init(smem_u32(&bar_acc_full[b]), 1);
@@ -172,8 +169,11 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     } else if (warp == 1) {
         // ================================================================ MMAs
         if (lane == 0) {
+            // descriptor halves as in the row-tile kernels: only the start address changes from MMA to MMA
+            constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+            const uint32_t lo0 = ((stage_base >> 4) & 0x3FFFu) | (1u << 16);
             int stage = 0;
-            uint32_t phase = 0;
+            uint32_t phase = 0, lo = lo0;
             int it = 0, gi = 0;
             bool ok = true;
             for (int item = blockIdx.x; ok && item < total_items; item += gridDim.x) {
@@ -187,20 +187,10 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
                     tc_fence_after();
                     const uint32_t tmem_d = tmem_base + ab * (C::NW * NT);
                     for (int grp = 0; ok && grp < n_groups; ++grp, ++gi) {
-                        const int slot = gi % D8_SF_SLOTS;
                         const uint32_t sf = tmem_base + C::SF_COL + (gi & 1) * 16;
-                        ok = mbar_wait(smem_u32(&bar_sf_full[slot]), (gi / D8_SF_SLOTS) & 1u, abortp, g.status,
-                                       DEV_TIMEOUT_MMA);
-                        // the TMEM copy was last read by the MMAs of the group before the previous one
-                        if (ok && gi >= 2)
-                            ok = mbar_wait(smem_u32(&bar_sf_empty[(gi - 2) % D8_SF_SLOTS]),
-                                           ((gi - 2) / D8_SF_SLOTS) & 1u, abortp, g.status, DEV_TIMEOUT_MMA);
+                        ok = mbar_wait(smem_u32(&bar_sf_full[gi & 1]), (gi >> 1) & 1u, abortp, g.status, DEV_TIMEOUT_MMA);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t sf_smem = sf_base + slot * C::SF;
-#pragma unroll
-                        for (int i = 0; i <= C::NW; ++i)
-                            tmem_cp_scales(sf + 4 * i, scales_smem_desc(sf_smem + i * FP8_ATOM));
                         const int kb0 = grp * FP8_GROUP;
 #pragma unroll
                         for (int j = 0; j < FP8_GROUP; ++j) {
@@ -211,34 +201,35 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
                                 }
                                 if (ok) {
                                     const uint32_t idesc = umma_idesc_fp8(128, 0, j) | n_field;
-                                    const uint32_t sw = stage_base + stage * C::STAGE + j % C::SL * C::SLICE;
-                                    const uint64_t dx = umma_smem_desc(sw + C::NW * D8_W, 16, 1024);
+                                    const uint32_t w_lo = lo + (j % C::SL * C::SLICE >> 4);
+                                    const uint32_t x_lo = w_lo + (C::NW * D8_W >> 4);
 #pragma unroll
                                     for (int i = 0; i < C::NW; ++i) {
-                                        const uint64_t dw = umma_smem_desc(sw + i * D8_W, 16, 1024);
 #pragma unroll
                                         for (uint32_t k = 0; k < 4; ++k)
-                                            umma_fp8(tmem_d + i * NT, dw + k * 2u, dx + k * 2u, idesc, sf + 4 * i,
-                                                     sf + 4 * C::NW, (kb0 + j + static_cast<int>(k)) != 0 ? 1u : 0u);
+                                            umma_fp8_lohi(tmem_d + i * NT, w_lo + (i * D8_W >> 4) + k * 2u, desc_hi,
+                                                          x_lo + k * 2u, desc_hi, idesc, sf + 4 * i, sf + 4 * C::NW,
+                                                          (kb0 + j + static_cast<int>(k)) != 0 ? 1u : 0u);
                                     }
                                     if (j % C::SL == C::SL - 1 || kb0 + j + 1 == g.nkb) {
                                         umma_commit(smem_u32(&bar_empty[stage]));
-                                        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                                        lo += C::STAGE >> 4;
+                                        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; lo = lo0; }
                                     }
                                 }
                             }
                         }
-                        if (ok) umma_commit(smem_u32(&bar_sf_empty[slot]));
+                        if (ok) umma_commit(smem_u32(&bar_sf_empty[gi & 1]));
                     }
                     if (ok) umma_commit(smem_u32(&bar_acc_full[ab]));
                 }
             }
         }
-    } else if (warp == 6) {
-        // ================================================================ scales (whole warp)
-        int slot = 0;
-        uint32_t phase = 0;
+    } else if (warp >= 6) {
+        // ================================================================ scales (four whole warps)
+        int gi = 0;
         bool ok = true;
+        const uint32_t sf0 = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + C::SF_COL;
         const int w_blocks = UP ? g.n_cblk : (g.out_cols + 127) / 128;
         for (int item = blockIdx.x; ok && item < total_items; item += gridDim.x) {
             const D8Item w = d8_item<NT>(g, item);
@@ -254,7 +245,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
             }
             const uint8_t* xs = g.x_scale + static_cast<size_t>(w.tile) * n_groups * FP8_ATOM + lane * 16;
             for (int ps = 0; ok && ps < w.n_pass; ++ps) {
-                for (int grp = 0; grp < n_groups; ++grp) {
+                for (int grp = 0; grp < n_groups; ++grp, ++gi) {
                     uint4 xw;
                     if constexpr (NT == 32) {
                         // row ps * 32 + lane: word ps of the lane's 16 bytes
@@ -269,20 +260,19 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
                     word |= __shfl_xor_sync(0xffffffffu, word, 1);
                     word |= __shfl_xor_sync(0xffffffffu, word, 2);
                     const uint32_t w0 = __shfl_sync(0xffffffffu, word, 0), w1 = __shfl_sync(0xffffffffu, word, 4);
-                    int okw = 1;
-                    if (lane == 0)
-                        okw = mbar_wait(smem_u32(&bar_sf_empty[slot]), phase ^ 1u, abortp, g.status,
-                                        DEV_TIMEOUT_PRODUCER) ? 1 : 0;
-                    okw = __shfl_sync(0xffffffffu, okw, 0);
-                    if (okw == 0) { ok = false; break; }
-                    const uint32_t dst = sf_base + slot * C::SF + lane * 16;
-                    st_shared_v4(dst, w0, w0, w0, w0);
-                    if constexpr (C::NW == 2) st_shared_v4(dst + FP8_ATOM, w1, w1, w1, w1);
-                    st_shared_v4(dst + C::NW * FP8_ATOM, xw.x, xw.y, xw.z, xw.w);
-                    fence_proxy_async_smem();
+                    ok = mbar_wait(smem_u32(&bar_sf_empty[gi & 1]), ((gi >> 1) & 1u) ^ 1u, abortp, g.status,
+                                   DEV_TIMEOUT_PRODUCER);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t sf = sf0 + (gi & 1) * 16;
+                    tmem_st4(sf, w0, w0, w0, w0);
+                    if constexpr (C::NW == 2) tmem_st4(sf + 4, w1, w1, w1, w1);
+                    tmem_st4(sf + 4 * C::NW, xw.x, xw.y, xw.z, xw.w);
+                    tmem_st_wait();
+                    tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&bar_sf_full[slot]));
-                    if (++slot == D8_SF_SLOTS) { slot = 0; phase ^= 1u; }
+                    if (lane == 0) mbar_arrive(smem_u32(&bar_sf_full[gi & 1]));
                 }
             }
         }

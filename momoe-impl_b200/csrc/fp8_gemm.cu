@@ -11,11 +11,11 @@
 // CTA loads its 128 rows of A and half of B, ring of 3 stages of two 128-byte k slices (a slice is 128 values here), warp
 // 0 loads, warp 1 of the leader issues the MMAs, warps 2..9 are the epilogue.  What differs:
 //
-// Scales.  Warp 10 of each CTA fills a ring of four 1.5 KiB slots, each with the scales of four slices (512 k): one
-// 512-byte block for the CTA's 128 rows, copied as it lies in memory, and two for the 256 weight columns, one word each
-// repeated 128 times.  tcgen05.cp moves a slot to TMEM in front of the four slices' MMAs, which pick their byte of each
-// word through the scale ids of the instruction descriptor.  Two TMEM copies alternate; a copy is overwritten only after
-// the commit behind the MMAs that read it has arrived.
+// Scales.  Warps 10..13 of each CTA (one for each TMEM lane quarter) write the scales of four slices (512 k) straight into
+// TMEM: 4 columns for the CTA's 128 rows, 8 for the 256 weight columns (one word each, repeated).  The MMAs of the four
+// slices pick their byte of each word through the scale ids of the instruction descriptor.  Two TMEM copies alternate; a
+// copy is overwritten after the commit behind the MMAs that read it has arrived.  (Copies from shared memory by tcgen05.cp
+// sit between the MMAs in the tensor pipe: 536 against XXX us for the up GEMM of 16384 tokens, D2048 H1024, top-8 of 128.)
 //
 // TMEM.  Two accumulators of 256 columns and 24 columns of scales do not fit 512 columns, so the accumulators overlap: the
 // first takes columns 0..255, the second 224..479, the scales 480..503.  The epilogue reads the 32 shared columns of a
@@ -32,7 +32,8 @@
 namespace momoe {
 
 constexpr int F8_EPI_WARPS = 8;
-constexpr int F8_THREADS = 32 * (3 + F8_EPI_WARPS);
+constexpr int F8_SF_WARPS = 4;
+constexpr int F8_THREADS = 32 * (2 + F8_EPI_WARPS + F8_SF_WARPS);
 constexpr int F8_PAIR_N = 256;
 constexpr int F8_K = 128;                                 // values of a k slice (128 bytes)
 constexpr int F8_A_BYTES = TILE_M * F8_K;                 // 16 KiB
@@ -40,11 +41,11 @@ constexpr int F8_B_BYTES = F8_PAIR_N / 2 * F8_K;          // 16 KiB
 constexpr int F8_SLICE_BYTES = F8_A_BYTES + F8_B_BYTES;
 constexpr int F8_STAGE_BYTES = 2 * F8_SLICE_BYTES;
 constexpr int F8_STAGES = 3;
-constexpr int F8_SF_SLOTS = 4;
-constexpr int F8_SF_BYTES = 3 * FP8_ATOM;
-constexpr int F8_EPI_BYTES = 2048;                        // staging of one epilogue warp: 32 rows x 64 bytes
-constexpr int F8_SMEM_BYTES =
-    F8_STAGES * F8_STAGE_BYTES + F8_SF_SLOTS * F8_SF_BYTES + F8_EPI_WARPS * F8_EPI_BYTES + 1024;
+constexpr int F8_PIECE = 2048;                            // staging of results: 32 rows x 64 bytes
+template <bool UP>
+constexpr int F8_PIECES = UP ? 1 : 2;                     // pieces an epilogue warp has
+template <bool UP>
+constexpr int F8_SMEM_BYTES = F8_STAGES * F8_STAGE_BYTES + F8_EPI_WARPS * F8_PIECES<UP> * F8_PIECE + 1024;
 constexpr int F8_ACC1 = 224;                              // first column of the second accumulator
 constexpr int F8_SF_COL = 480;
 constexpr int F8_SF_COLS = 12;                            // 4 for A, 8 for B
@@ -62,7 +63,6 @@ struct Fp8Args {
     int b_blocks;               // down: ceil(D / 128)
     uint8_t* h_scale;           // up: scales of h, blocks of 512 bytes
     const float* row_weight;    // down
-    __nv_bfloat16* y;           // down
 };
 
 __device__ __forceinline__ uint32_t f8_pack_bf16(float lo, float hi) {
@@ -92,8 +92,8 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bar_full[F8_STAGES];
     __shared__ uint64_t bar_empty[F8_STAGES];
-    __shared__ uint64_t bar_sf_full[F8_SF_SLOTS];    // leader: both CTAs' scale warps have filled the slot
-    __shared__ uint64_t bar_sf_empty[F8_SF_SLOTS];   // both: the MMAs that use the slot's scales have completed
+    __shared__ uint64_t bar_sf_full[2];              // leader: both CTAs' scale warps have written this copy
+    __shared__ uint64_t bar_sf_empty[2];             // both: the MMAs that read this copy have completed
     __shared__ uint64_t bar_acc_full[2];
     __shared__ uint64_t bar_acc_empty[2];            // leader
     __shared__ uint64_t bar_ovl;                     // leader: the shared columns of the latest tile have been read
@@ -108,8 +108,7 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     const int cluster_id = blockIdx.x >> 1;
     const int n_clusters = gridDim.x >> 1;
     const uint32_t stage_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sf_base = stage_base + F8_STAGES * F8_STAGE_BYTES;
-    const uint32_t epi_base = sf_base + F8_SF_SLOTS * F8_SF_BYTES;
+    const uint32_t epi_base = stage_base + F8_STAGES * F8_STAGE_BYTES;
 
     const int total_items = __ldg(g.sched + SCHED_N_PAIRS) * g.n_nblk;
     if (total_items <= 0 || cluster_id >= total_items) return;   // both CTAs of the cluster leave together
@@ -121,11 +120,9 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             mbar_init(smem_u32(&bar_full[s]), 1);
             mbar_init(smem_u32(&bar_empty[s]), 1);
         }
-        for (int s = 0; s < F8_SF_SLOTS; ++s) {
-            mbar_init(smem_u32(&bar_sf_full[s]), 2);
-            mbar_init(smem_u32(&bar_sf_empty[s]), 1);
-        }
         for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&bar_sf_full[b]), 2 * F8_SF_WARPS);
+            mbar_init(smem_u32(&bar_sf_empty[b]), 1);
             mbar_init(smem_u32(&bar_acc_full[b]), 1);
             mbar_init(smem_u32(&bar_acc_empty[b]), 2 * F8_EPI_WARPS);
         }
@@ -193,20 +190,10 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 tc_fence_after();
                 const uint32_t tmem_d = tmem_base + ab * F8_ACC1;
                 for (int grp = 0; ok && grp < n_groups; ++grp, ++gi) {
-                    const int slot = gi % F8_SF_SLOTS;
                     const uint32_t sf = tmem_base + F8_SF_COL + (gi & 1) * F8_SF_COLS;
-                    ok = mbar_wait_cluster(smem_u32(&bar_sf_full[slot]), (gi / F8_SF_SLOTS) & 1u, abortp, g.status,
-                                           DEV_TIMEOUT_MMA);
-                    // the TMEM copy was last read by the MMAs of the group before the previous one
-                    if (ok && gi >= 2)
-                        ok = mbar_wait(smem_u32(&bar_sf_empty[(gi - 2) % F8_SF_SLOTS]), ((gi - 2) / F8_SF_SLOTS) & 1u,
-                                       abortp, g.status, DEV_TIMEOUT_MMA);
+                    ok = mbar_wait(smem_u32(&bar_sf_full[gi & 1]), (gi >> 1) & 1u, abortp, g.status, DEV_TIMEOUT_MMA);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sf_smem = sf_base + slot * F8_SF_BYTES;
-                    tmem_cp_scales_pair(sf, scales_smem_desc(sf_smem));
-                    tmem_cp_scales_pair(sf + 4, scales_smem_desc(sf_smem + FP8_ATOM));
-                    tmem_cp_scales_pair(sf + 8, scales_smem_desc(sf_smem + 2 * FP8_ATOM));
                     const int kb0 = grp * FP8_GROUP;
 #pragma unroll
                     for (int j = 0; j < FP8_GROUP; ++j) {
@@ -230,17 +217,17 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                             }
                         }
                     }
-                    if (ok) umma_commit_pair(smem_u32(&bar_sf_empty[slot]), 3);
+                    if (ok) umma_commit_pair(smem_u32(&bar_sf_empty[gi & 1]), 3);
                 }
                 if (ok) umma_commit_pair(smem_u32(&bar_acc_full[ab]), 3);
             }
         }
-    } else if (warp == 2 + F8_EPI_WARPS) {
-        // ================================================================ scales (both CTAs, whole warp)
-        int slot = 0;
-        uint32_t phase = 0;
+    } else if (warp >= 2 + F8_EPI_WARPS) {
+        // ================================================================ scales (both CTAs, four whole warps)
+        int gi = 0;
         bool ok = true;
         const uint32_t full0 = mapa_shared(smem_u32(&bar_sf_full[0]), 0);
+        const uint32_t sf0 = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + F8_SF_COL;
         for (int item = cluster_id; ok && item < total_items; item += n_clusters) {
             const Fp8Work w = f8_work(g, item, cta_rank);
             const int tile = w.valid ? w.tile : w.tile - 1;     // a missing half reads its partner's scales
@@ -256,7 +243,7 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 bs = g.b_scale + (static_cast<size_t>(w.e) * g.b_blocks + w.nb * 2 + i) * g.nkb;
                 have = w.nb * 2 + i < g.b_blocks;
             }
-            for (int grp = 0; grp < n_groups; ++grp) {
+            for (int grp = 0; grp < n_groups; ++grp, ++gi) {
                 const uint4 a = __ldg(src + grp * 32 + lane);
                 const int kb = grp * FP8_GROUP + (lane & 3);
                 uint32_t word = have && kb < g.nkb ? __ldg(bs + kb) : 127u;
@@ -264,20 +251,19 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 word |= __shfl_xor_sync(0xffffffffu, word, 1);
                 word |= __shfl_xor_sync(0xffffffffu, word, 2);
                 const uint32_t b0 = __shfl_sync(0xffffffffu, word, 0), b1 = __shfl_sync(0xffffffffu, word, 4);
-                int okw = 1;
-                if (lane == 0)
-                    okw = mbar_wait(smem_u32(&bar_sf_empty[slot]), phase ^ 1u, abortp, g.status, DEV_TIMEOUT_PRODUCER)
-                              ? 1 : 0;
-                okw = __shfl_sync(0xffffffffu, okw, 0);
-                if (okw == 0) { ok = false; break; }
-                const uint32_t dst = sf_base + slot * F8_SF_BYTES + lane * 16;
-                st_shared_v4(dst, a.x, a.y, a.z, a.w);
-                st_shared_v4(dst + FP8_ATOM, b0, b0, b0, b0);
-                st_shared_v4(dst + 2 * FP8_ATOM, b1, b1, b1, b1);
-                fence_proxy_async_smem();
+                ok = mbar_wait(smem_u32(&bar_sf_empty[gi & 1]), ((gi >> 1) & 1u) ^ 1u, abortp, g.status,
+                               DEV_TIMEOUT_PRODUCER);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t sf = sf0 + (gi & 1) * F8_SF_COLS;
+                tmem_st4(sf, a.x, a.y, a.z, a.w);
+                tmem_st4(sf + 4, b0, b0, b0, b0);
+                tmem_st4(sf + 8, b1, b1, b1, b1);
+                tmem_st_wait();
+                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(full0 + static_cast<uint32_t>(slot * sizeof(uint64_t)));
-                if (++slot == F8_SF_SLOTS) { slot = 0; phase ^= 1u; }
+                if (lane == 0) mbar_arrive_cluster_relaxed(full0 + static_cast<uint32_t>((gi & 1) * sizeof(uint64_t)));
             }
         }
     } else {
@@ -287,10 +273,11 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const int half = (warp - 2) >> 2;
         const uint32_t acc_empty_leader = mapa_shared(smem_u32(&bar_acc_empty[0]), 0);
         const uint32_t ovl_leader = mapa_shared(smem_u32(&bar_ovl), 0);
-        const uint32_t stage_area = epi_base + (warp - 2) * F8_EPI_BYTES;
+        constexpr int PIECES = F8_PIECES<UP>;
+        const uint32_t stage_area = epi_base + (warp - 2) * PIECES * F8_PIECE;
         int it = 0;
         bool ok = true;
-        bool stored = false;
+        int n_stored = 0;                  // pieces handed to TMA stores so far (lane 0 owns the bulk groups)
         for (int item = cluster_id; ok && item < total_items; item += n_clusters, ++it) {
             const Fp8Work w = f8_work(g, item, cta_rank);
             const int ab = it & 1;
@@ -300,12 +287,12 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             auto hand_back_shared = [&]() {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(ovl_leader);
+                if (lane == 0) mbar_arrive_cluster_relaxed(ovl_leader);
             };
             auto hand_back_all = [&]() {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(acc_empty_leader + ab * static_cast<uint32_t>(sizeof(uint64_t)));
+                if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + ab * static_cast<uint32_t>(sizeof(uint64_t)));
             };
             float wgt = 0.0f;
             const size_t grow = static_cast<size_t>(w.tile) * TILE_M + row;
@@ -357,10 +344,11 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                         g.h_scale[fp8_atom_offset(grow, w.nb >> 2, (g.n_nblk + 3) >> 2) + (w.nb & 3)] =
                             static_cast<uint8_t>(byte);
                     if (col0 < g.out_cols) {
-                        if (stored && lane == 0) bulk_wait_read<0>();
+                        const uint32_t slot = stage_area + n_stored % PIECES * F8_PIECE;
+                        if (n_stored >= PIECES && lane == 0) bulk_wait_read<PIECES - 1>();
                         __syncwarp();
                         // [32 rows x 64 bytes], 64-byte swizzle: 16-byte chunk j of row r at chunk j ^ ((r >> 1) & 3)
-                        const uint32_t base = stage_area + lane * 64;
+                        const uint32_t base = slot + lane * 64;
                         const uint32_t x = (lane >> 1) & 3;
                         uint32_t p[8];
 #pragma unroll
@@ -377,39 +365,48 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) {
-                            tma_store_2d(&tmO, stage_area, col0 / 2, w.tile * TILE_M + q * 32);
+                            tma_store_2d(&tmO, slot, col0 / 2, w.tile * TILE_M + q * 32);
                             bulk_commit();
                         }
-                        stored = true;
+                        ++n_stored;
                     }
                 }
             } else {
-                uint32_t r[32];
+                // results leave through shared memory by TMA: with one row a thread, stores straight from registers touch
+                // 32 sectors an instruction and take longer than the tile's MMAs (XXX us against YYY)
 #pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
                     // half 1 starts with the last chunk, which may be the shared one
                     const int c = half == 0 ? i : 4 + ((i + 3) & 3);
+                    uint32_t r[32];
                     tmem_ld32(taddr + c * 32, r);
                     tmem_ld_wait();
                     if (i == 0 && shares) hand_back_shared();
                     if (i == 3) hand_back_all();
                     const int col0 = w.nb * F8_PAIR_N + c * 32;
                     if (w.valid && col0 < g.out_cols) {
-                        __nv_bfloat16* dst = g.y + grow * g.out_cols + col0;
+                        const uint32_t slot = stage_area + n_stored % PIECES * F8_PIECE;
+                        if (n_stored >= PIECES && lane == 0) bulk_wait_read<PIECES - 1>();
+                        __syncwarp();
+                        // [32 rows x 64 bytes], 64-byte swizzle: 16-byte chunk j of row r at chunk j ^ ((r >> 1) & 3)
+                        const uint32_t base = slot + lane * 64;
+                        const uint32_t x = (lane >> 1) & 3;
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            if (col0 + j * 16 < g.out_cols) {     // D is a multiple of 16: 32-byte pieces are whole
-                                uint32_t v[8];
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t v[4];
 #pragma unroll
-                                for (int u = 0; u < 8; ++u)
-                                    v[u] = f8_pack_bf16(__uint_as_float(r[j * 16 + 2 * u]) * wgt,
-                                                        __uint_as_float(r[j * 16 + 2 * u + 1]) * wgt);
-                                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + j * 16),
-                                             "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
-                                             "r"(v[6]), "r"(v[7])
-                                             : "memory");
-                            }
+                            for (int u = 0; u < 4; ++u)
+                                v[u] = f8_pack_bf16(__uint_as_float(r[j * 8 + 2 * u]) * wgt,
+                                                    __uint_as_float(r[j * 8 + 2 * u + 1]) * wgt);
+                            st_shared_v4(base + ((j ^ x) << 4), v[0], v[1], v[2], v[3]);
                         }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&tmO, slot, col0, w.tile * TILE_M + q * 32);   // columns past D are not written
+                            bulk_commit();
+                        }
+                        ++n_stored;
                     }
                 }
             }
@@ -441,7 +438,7 @@ static int f8_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUten
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MOMOE_ERR_CUDA;
     if (!attr_set[dev]) {
         if (cudaFuncSetAttribute(fp8_grouped_gemm_kernel<UP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 F8_SMEM_BYTES) != cudaSuccess)
+                                 F8_SMEM_BYTES<UP>) != cudaSuccess)
             return MOMOE_ERR_CUDA;
         attr_set[dev] = true;
     }
@@ -450,7 +447,7 @@ static int f8_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUten
         memset(&cfg, 0, sizeof(cfg));
         cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
         cfg.blockDim = dim3(F8_THREADS);
-        cfg.dynamicSmemBytes = F8_SMEM_BYTES;
+        cfg.dynamicSmemBytes = F8_SMEM_BYTES<UP>;
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = 2;
@@ -465,7 +462,7 @@ static int f8_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUten
         }
         pairs[dev] = n < sm_count() / 2 ? n : sm_count() / 2;
     }
-    fp8_grouped_gemm_kernel<UP><<<2 * pairs[dev], F8_THREADS, F8_SMEM_BYTES, stream>>>(tmA, tmB, tmO, g);
+    fp8_grouped_gemm_kernel<UP><<<2 * pairs[dev], F8_THREADS, F8_SMEM_BYTES<UP>, stream>>>(tmA, tmB, tmO, g);
     return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
 
@@ -525,9 +522,10 @@ MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_so
         !f8_aligned(y_sorted, 32))
         return MOMOE_ERR_ARG;
     const int D = plan->D, H = plan->H;
-    CUtensorMap tmA, tmB;
+    CUtensorMap tmA, tmB, tmO;
     if ((rc = encode_tmap_2d(&tmA, h_sorted, plan->rows_capacity, H / 2, TILE_M, F8_K / 2)) != MOMOE_OK) return rc;
     if ((rc = encode_tmap_3d(&tmB, W2_NDH, plan->N, D, H / 2, 128, F8_K / 2)) != MOMOE_OK) return rc;
+    if ((rc = encode_tmap_2d(&tmO, y_sorted, plan->rows_capacity, D, 32, 32, TMAP_SWIZZLE_64B)) != MOMOE_OK) return rc;
     Fp8Args g;
     memset(&g, 0, sizeof(g));
     g.sched = plan->sched;
@@ -541,6 +539,5 @@ MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_so
     g.b_scale = S2;
     g.b_blocks = f8_cdiv(D, 128);
     g.row_weight = plan->row_weight;
-    g.y = static_cast<__nv_bfloat16*>(y_sorted);
-    return f8_launch<false>(tmA, tmB, tmA, g, static_cast<cudaStream_t>(stream));
+    return f8_launch<false>(tmA, tmB, tmO, g, static_cast<cudaStream_t>(stream));
 }

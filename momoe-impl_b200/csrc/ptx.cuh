@@ -186,6 +186,12 @@ __device__ __forceinline__ void cluster_sync_all() {   // every thread of both C
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same without release semantics, for an arrival that hands back TMEM and publishes no memory: a release at cluster
+// scope first waits for the thread's earlier global stores, about 2000 cycles behind an epilogue's.  What the arrival
+// orders, tcgen05.ld, has completed before it by tcgen05.wait::ld.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // TMA loads issued by either CTA of a pair into its OWN shared memory; the transaction bytes are credited to the
 // mbarrier at `bar_cluster_addr`, which may live in the pair's leader CTA.  Each load has a single destination.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* m, uint32_t bar_cluster_addr, int c0,
@@ -277,13 +283,17 @@ __device__ __forceinline__ void umma_fp8_pair_lohi(uint32_t tmem_d, uint32_t a_l
           "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void umma_fp8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
-                                         uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
+__device__ __forceinline__ void umma_fp8_lohi(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                              uint32_t idesc, uint32_t tmem_sfa, uint32_t tmem_sfb,
+                                              uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %8, 0;\n\t"
+        "mov.b64 da, {%1, %2};\n\t"
+        "mov.b64 db, {%3, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %5, [%6], [%7], p;\n\t}"
+        ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb),
+          "r"(accumulate)
         : "memory");
 }
 // Instruction descriptor of kind::mxf8f6f4 with e4m3 operands (type 0), both K-major, e8m0 scales (bit 23):
@@ -292,48 +302,13 @@ __host__ __device__ constexpr uint32_t umma_idesc_fp8(int m, int n, int scale_id
     return (static_cast<uint32_t>(scale_id) << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
            (static_cast<uint32_t>(m >> 7) << 27) | (static_cast<uint32_t>(scale_id) << 29);
 }
-// 512 bytes of shared memory (32 lanes x 16 bytes) into 4 TMEM columns, repeated in all four lane quarters.  The pair
-// form copies, in each CTA of the pair, from that CTA's shared memory into its own TMEM.  Executes before any MMA that
-// the same thread issues later.
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+// Scales reach TMEM by tcgen05.st: each of four warps (one a lane quarter) stores the same 32 lanes x 4 columns into its
+// quarter, since the tensor core expects them repeated there.
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
 }
-__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-// Descriptor of such a 512-byte block: no swizzle, 8-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t scales_smem_desc(uint32_t saddr) {
-    return static_cast<uint64_t>((saddr >> 4) & 0x3FFF) | (static_cast<uint64_t>(128 >> 4) << 16) |
-           (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
-}
-// A wait whose arrivals come from both CTAs of a pair and publish shared memory written there (cluster scope).
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                                  int code) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    const long long t0 = clock64();
-    for (uint32_t spin = 1;; ++spin) {
-        if (mbar_try_wait_cluster(bar, parity)) return true;
-        if ((spin & 0x3F) == 0) {
-            if (*abort_flag) return false;
-            if (clock64() - t0 > kWaitLimitCycles) {
-                *abort_flag = 1;
-                atomicCAS(status, 0, code);
-                return false;
-            }
-        }
-    }
-}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---------------------------------------------------------------- UMMA descriptors
 // Shared-memory operand descriptor (64 bit): start address>>4 in [0,14), leading byte offset>>4 in [16,30),
