@@ -1,6 +1,6 @@
-"""Builds libmomoe_b200.so (sm_100a only) in-tree with nvcc.
+"""Builds libmomoe_b200.so (sm_100a only) in-tree with nvcc, and _native.so, its binding for torch tensors, with g++.
 
-    python momoe-impl_b200/build.py            # product library -> momoe-impl_b200/momoe/libmomoe_b200.so
+    python momoe-impl_b200/build.py            # -> momoe-impl_b200/momoe/libmomoe_b200.so, momoe-impl_b200/momoe/_native.so
 
 nvcc cross-compiles, so this runs on machines without a GPU.  The library links cudart statically and
 resolves the one driver entry point it needs at run time, so it also loads without a driver.
@@ -8,6 +8,7 @@ resolves the one driver entry point it needs at run time, so it also loads witho
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -18,6 +19,11 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--threads", "4",
 ]
+
+
+BINDING = os.path.join(CSRC, "binding.cpp")
+BINDING_PATH = os.path.join(HERE, "momoe", "_native.so")
+HEADER = os.path.join(HERE, "..", "include", "momoe_b200.h")
 
 
 def _stale(out, deps):
@@ -31,11 +37,18 @@ def build(out=LIB_PATH, extra_flags=(), force=False, verbose=False):
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]
-    deps.append(os.path.join(HERE, "..", "include", "momoe_b200.h"))
+    deps.append(HEADER)
+    if out == LIB_PATH:
+        build_binding(force=force, verbose=verbose)
     if not force and not _stale(out, deps):
         return out
+    _run([nvcc, "-shared", "-o"], NVCC_FLAGS + list(extra_flags) + srcs, out, verbose)
+    return out
+
+
+def _run(head, tail, out, verbose):
     tmp = out + ".tmp%d" % os.getpid()     # written beside the target, then renamed: readers never see a partial file
-    cmd = [nvcc, "-shared", "-o", tmp] + NVCC_FLAGS + list(extra_flags) + srcs
+    cmd = head + [tmp] + tail
     if verbose:
         print(" ".join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -43,10 +56,29 @@ def build(out=LIB_PATH, extra_flags=(), force=False, verbose=False):
         sys.stderr.write(res.stdout + res.stderr)
         if os.path.exists(tmp):
             os.remove(tmp)
-        raise RuntimeError("nvcc failed building " + out)
+        raise RuntimeError("%s failed building %s" % (os.path.basename(head[0]), out))
     os.replace(tmp, out)
     if verbose:
         sys.stderr.write(res.stdout + res.stderr)
+
+
+def build_binding(out=BINDING_PATH, force=False, verbose=False):
+    """The torch binding; it takes the entry points from the loaded library at run time, so neither links the other."""
+    if not force and not _stale(out, [BINDING, HEADER]):
+        return out
+    import torch
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")))
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_native",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    includes = ["-isystem" + p for p in (os.path.join(home, "include"), os.path.join(cuda, "include"),
+                                         os.path.join(home, "include", "torch", "csrc", "api", "include"),
+                                         sysconfig.get_paths()["include"])]
+    libs = ["-L" + os.path.join(home, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+            "-ltorch_python"]
+    # the compiler on PATH and the C++ runtime that torch has loaded: a toolchain that links its own copy statically (CXX
+    # may name one) puts two runtimes into the process, and the first error message crashes it
+    _run(["g++", "-shared", "-o"], flags + includes + [BINDING] + libs + ["-l:libstdc++.so.6"], out, verbose)
     return out
 
 

@@ -25,11 +25,6 @@ constexpr int BAL_THREADS = 256;
 constexpr int BAL_WARPS = BAL_THREADS / 32;
 constexpr int BAL_MAX_EXPERTS = 1024;
 
-__device__ __forceinline__ float bal_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 __device__ __forceinline__ float bal_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -46,45 +41,59 @@ struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) BalVec {
     T v[V];
 };
 
-// Lane l holds the logits (l + 32 i) V .. + V - 1 of its row, i < NV; columns from Ng on count as -inf.
-template <typename T, int V, int NV>
-__device__ __forceinline__ void bal_load(const T* row, int N, int Ng, int lane, float (&x)[NV * V]) {
+// How a row of N logits lies in a warp: L lanes a row (32 / L rows side by side), lane l of them holds the logits
+// (l + i L) V .. + V - 1, i < NV.  Few lanes a row keep the reductions short, which is what a row costs; V = 8 needs rows
+// that are a multiple of 8 long.
+template <typename T, int L, int V, int NV>
+struct BalRow {
+    static constexpr int C = V * NV;
+
+    static __device__ __forceinline__ int column(int l, int i) { return (l + i * L) * V; }
+
+    // columns from Ng on, and the whole row where `in` is false, count as -inf
+    static __device__ __forceinline__ void load(const T* row, bool in, int N, int Ng, int l, float (&x)[C]) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int j = (lane + i * 32) * V;
-        if (j < N) {
-            const BalVec<T, V> q = *reinterpret_cast<const BalVec<T, V>*>(row + j);
+        for (int i = 0; i < NV; ++i) {
+            const int j = column(l, i);
+            BalVec<T, V> q;
+            if (in && j < N) q = *reinterpret_cast<const BalVec<T, V>*>(row + j);
 #pragma unroll
-            for (int u = 0; u < V; ++u) x[i * V + u] = j + u < Ng ? bal_to_float(q.v[u]) : -INFINITY;
-        } else {
-#pragma unroll
-            for (int u = 0; u < V; ++u) x[i * V + u] = -INFINITY;
+            for (int u = 0; u < V; ++u) x[i * V + u] = in && j + u < Ng ? bal_to_float(q.v[u]) : -INFINITY;
         }
     }
-}
-// x -> probabilities; returns the log of the sum (0, and p = 0, where every logit is -inf).
-template <int C>
-__device__ __forceinline__ float bal_softmax(float (&x)[C]) {
-    float mx = x[0];
+    static __device__ __forceinline__ float max(float v) {
 #pragma unroll
-    for (int i = 1; i < C; ++i) mx = fmaxf(mx, x[i]);
-    mx = bal_max(mx);
-    const bool dead = mx == -INFINITY;
-    const float base = dead ? 0.0f : mx;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-        x[i] = __expf(x[i] - base);
-        sum += x[i];
+        for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
     }
-    sum = bal_sum(sum);
-    // a NaN among the logits is lost by the maximum, not by the sum: sum > 0 fails for it, so it reaches the result
-    if (dead && sum == 0.0f) return 0.0f;
-    const float inv = 1.0f / sum;
+    static __device__ __forceinline__ float sum(float v) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) x[i] *= inv;
-    return base + logf(sum);
-}
+        for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+    // x -> probabilities; returns the log of the sum (0, and p = 0, where every logit is -inf).
+    static __device__ __forceinline__ float softmax(float (&x)[C]) {
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < C; ++i) mx = fmaxf(mx, x[i]);
+        mx = max(mx);
+        const bool dead = mx == -INFINITY;
+        const float base = dead ? 0.0f : mx;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            x[i] = __expf(x[i] - base);
+            s += x[i];
+        }
+        s = sum(s);
+        // a NaN among the logits is lost by the maximum, not by the sum: it is not 0, so it reaches the result
+        const bool none = dead && s == 0.0f;
+        const float inv = none ? 0.0f : 1.0f / s;
+#pragma unroll
+        for (int i = 0; i < C; ++i) x[i] *= inv;
+        return none ? 0.0f : base + logf(s);
+    }
+};
 
 // The B sequences of M rows: a table of B + 1 row numbers, or (null) consecutive sequences of S rows.
 struct BalSeqs {
@@ -126,12 +135,14 @@ struct BalArgs {
     float* g;            // [B, N]
 };
 
-template <typename T, int V, int NV>
+template <typename T, int L, int V, int NV>
 __global__ void __launch_bounds__(BAL_THREADS) balance_partial_kernel(const BalArgs a) {
+    using Row = BalRow<T, L, V, NV>;
+    constexpr int SIDE = 32 / L;                // rows side by side in a warp
     extern __shared__ float sm[];               // [8 warps, N] sums, then N counters
     __shared__ float s_z[BAL_WARPS];
     int* s_cnt = reinterpret_cast<int*>(sm + BAL_WARPS * a.N);
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, l = lane % L;
     const int c = blockIdx.x;
     const int row0 = c * a.R, row1 = min(a.M, row0 + a.R);
     if (c == 0 && threadIdx.x == 0) *a.ticket = 0u;
@@ -139,7 +150,7 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_partial_kernel(const BalA
     const int Ng = a.N - a.Ks;
     int b = a.seq.of(row0);
     if (b < 0) b = 0;
-    for (; b < a.B; ++b) {
+    for (; b < a.seq.B; ++b) {
         const int start = a.seq.bound(b);
         if (start >= row1) break;
         const int lo = max(start, row0), hi = min(a.seq.bound(b + 1), row1);
@@ -150,23 +161,33 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_partial_kernel(const BalA
             const int e = __ldg(a.topk + static_cast<size_t>(lo) * a.K + i);
             if (e >= 0 && e < a.N) atomicAdd(&s_cnt[e], 1);
         }
-        float acc[NV * V], z = 0.0f;
+        float acc[Row::C], z = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV * V; ++i) acc[i] = 0.0f;
-        for (int m = lo + w; m < hi; m += BAL_WARPS) {
-            float x[NV * V];
-            bal_load<T, V, NV>(logits + static_cast<size_t>(m) * a.N, a.N, Ng, lane, x);
-            const float lse = bal_softmax(x);
+        for (int i = 0; i < Row::C; ++i) acc[i] = 0.0f;
+        for (int m0 = lo + w * SIDE; m0 < hi; m0 += BAL_WARPS * SIDE) {
+            const int m = m0 + lane / L;
+            float x[Row::C];
+            Row::load(logits + static_cast<size_t>(m) * a.N, m < hi, a.N, Ng, l, x);
+            const float lse = Row::softmax(x);
 #pragma unroll
-            for (int i = 0; i < NV * V; ++i) acc[i] += x[i];
+            for (int i = 0; i < Row::C; ++i) acc[i] += x[i];
             z = fmaf(lse, lse, z);
         }
+        // rows side by side, then the warps
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = (lane + i * 32) * V;
+        for (int o = 16; o >= L; o >>= 1) {
 #pragma unroll
-            for (int u = 0; u < V; ++u)
-                if (j + u < a.N) sm[w * a.N + j + u] = acc[i * V + u];
+            for (int i = 0; i < Row::C; ++i) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+            z += __shfl_xor_sync(0xffffffffu, z, o);
+        }
+        if (lane < L) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int j = Row::column(l, i);
+#pragma unroll
+                for (int u = 0; u < V; ++u)
+                    if (j + u < a.N) sm[w * a.N + j + u] = acc[i * V + u];
+            }
         }
         if (lane == 0) s_z[w] = z;
         __syncthreads();
@@ -282,55 +303,75 @@ __global__ void __launch_bounds__(1024) balance_finish_kernel(const BalArgs a) {
     }
 }
 
-// One warp a row.  `add` (may be null, may be `out` itself): a gradient of the logits from elsewhere, added in 32 bits.
-template <typename T, int V, int NV>
+// `add` (may be null, may be `out` itself): a gradient of the logits from elsewhere, added in 32 bits.  A warp takes RW
+// consecutive rows, so that the coefficients of their sequence are mostly read once.
+template <typename T, int L, int V, int NV>
 __global__ void __launch_bounds__(BAL_THREADS)
-balance_backward_kernel(const T* __restrict__ logits, const BalSeqs seq, const float* __restrict__ g, int N, int Ks,
+balance_backward_kernel(const T* __restrict__ logits, const BalSeqs seq, const float* __restrict__ g, int N, int Ks, int RW,
                         float z_coef, const float* __restrict__ up, const T* add, T* out) {
-    const int lane = threadIdx.x & 31;
-    const int m = blockIdx.x * BAL_WARPS + (threadIdx.x >> 5);
-    if (m >= seq.M) return;
+    using Row = BalRow<T, L, V, NV>;
+    constexpr int SIDE = 32 / L;
+    const int lane = threadIdx.x & 31, l = lane % L;
+    const int first_row = (blockIdx.x * BAL_WARPS + (threadIdx.x >> 5)) * RW;
+    const int end_row = min(seq.M, first_row + RW);
+    if (first_row >= end_row) return;
     const int Ng = N - Ks;
-    const int b = seq.of(m);
     const int first = seq.bound(0), last = seq.bound(seq.B);
-    const bool real = b >= 0 && m < last;
-    float x[NV * V];
-    if (real) {
-        const float scale = __ldg(up);
-        bal_load<T, V, NV>(logits + static_cast<size_t>(m) * N, N, Ng, lane, x);
-        const float lse = bal_softmax(x);
-        const float zt = 2.0f * z_coef / static_cast<float>(max(last - first, 1)) * lse;
-        float gv[NV * V], dot = 0.0f;
+    const float scale = __ldg(up);
+    const float zt = 2.0f * z_coef / static_cast<float>(max(last - first, 1));
+    int b = -1;                                 // sequence whose coefficients gv holds
+    float gv[Row::C];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = (lane + i * 32) * V;
+    for (int i = 0; i < Row::C; ++i) gv[i] = 0.0f;
+    for (int m0 = first_row; m0 < end_row; m0 += SIDE) {
+        const int m = m0 + lane / L;
+        const bool here = m < end_row;
+        const bool real = here && m >= first && m < last;
+        float x[Row::C];
+        Row::load(logits + static_cast<size_t>(m) * N, real, N, Ng, l, x);
+        if (real && (b < 0 || m >= seq.bound(b + 1))) {
+            b = seq.of(m);
 #pragma unroll
-            for (int u = 0; u < V; ++u) {
-                gv[i * V + u] = j + u < Ng ? __ldg(g + static_cast<size_t>(b) * N + j + u) : 0.0f;
-                dot = fmaf(gv[i * V + u], x[i * V + u], dot);
+            for (int i = 0; i < NV; ++i) {
+                const int j = Row::column(l, i);
+                if (V % 4 == 0) {
+#pragma unroll
+                    for (int u = 0; u < V; u += 4)
+                        if (j + u < N) {
+                            const float4 q = __ldg(reinterpret_cast<const float4*>(g + static_cast<size_t>(b) * N + j + u));
+                            gv[i * V + u] = q.x;
+                            gv[i * V + (u + 1) % V] = q.y;
+                            gv[i * V + (u + 2) % V] = q.z;
+                            gv[i * V + (u + 3) % V] = q.w;
+                        }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < V; ++u)
+                        if (j + u < N) gv[i * V + u] = __ldg(g + static_cast<size_t>(b) * N + j + u);
+                }
             }
         }
-        dot = bal_sum(dot);
+        const float lse = Row::softmax(x);
+        float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV * V; ++i) x[i] *= scale * (gv[i] - dot + zt);
-    } else {
+        for (int i = 0; i < Row::C; ++i) dot = fmaf(gv[i], x[i], dot);     // x is 0 in columns without a coefficient
+        dot = Row::sum(dot) - zt * lse;
+        if (!here) continue;
+        const size_t row = static_cast<size_t>(m) * N;
 #pragma unroll
-        for (int i = 0; i < NV * V; ++i) x[i] = 0.0f;
-    }
-    const size_t row = static_cast<size_t>(m) * N;
+        for (int i = 0; i < NV; ++i) {
+            const int j = Row::column(l, i);
+            if (j >= N) continue;
+            BalVec<T, V> q;
+            if (add != nullptr) q = *reinterpret_cast<const BalVec<T, V>*>(add + row + j);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int j = (lane + i * 32) * V;
-        if (j >= N) continue;
-        BalVec<T, V> q;
-        if (add != nullptr) q = *reinterpret_cast<const BalVec<T, V>*>(add + row + j);
-#pragma unroll
-        for (int u = 0; u < V; ++u) {
-            float v = j + u < Ng ? x[i * V + u] : 0.0f;
-            if (add != nullptr) v += bal_to_float(q.v[u]);
-            bal_from_float(v, q.v[u]);
+            for (int u = 0; u < V; ++u) {
+                float v = real && j + u < Ng ? x[i * V + u] * scale * (gv[i * V + u] - dot) : 0.0f;
+                if (add != nullptr) v += bal_to_float(q.v[u]);
+                bal_from_float(v, q.v[u]);
+            }
+            *reinterpret_cast<BalVec<T, V>*>(out + row + j) = q;
         }
-        *reinterpret_cast<BalVec<T, V>*>(out + row + j) = q;
     }
 }
 
@@ -367,18 +408,22 @@ static bool bal_uniform(const int32_t* cu, int32_t seq_len, int32_t M, int32_t B
     return cu != nullptr || (seq_len > 0 && B == (M - 1) / seq_len + 1);
 }
 
-// Width of a lane's accesses: the widest of 8 and 4 logits that the row length allows and that keeps every lane busy.
+// 16 logits a lane in accesses of 8 where the row length allows it (32 above 512 experts), else one by one across a warp.
 #define BAL_DISPATCH(T, CALL)                                   \
-    if (N % 8 == 0 && N > 512) { CALL(T, 8, 4); }               \
-    else if (N % 8 == 0 && N > 256) { CALL(T, 8, 2); }          \
-    else if (N % 8 == 0 && N > 128) { CALL(T, 8, 1); }          \
-    else if (N % 4 == 0 && N > 64 && N <= 128) { CALL(T, 4, 1); } \
-    else if (N <= 32) { CALL(T, 1, 1); }                        \
-    else if (N <= 64) { CALL(T, 1, 2); }                        \
-    else if (N <= 128) { CALL(T, 1, 4); }                       \
-    else if (N <= 256) { CALL(T, 1, 8); }                       \
-    else if (N <= 512) { CALL(T, 1, 16); }                      \
-    else { CALL(T, 1, 32); }
+    if (N % 8 == 0) {                                           \
+        if (N <= 32) { CALL(T, 2, 8, 2); }                      \
+        else if (N <= 64) { CALL(T, 4, 8, 2); }                 \
+        else if (N <= 128) { CALL(T, 8, 8, 2); }                \
+        else if (N <= 256) { CALL(T, 16, 8, 2); }               \
+        else if (N <= 512) { CALL(T, 32, 8, 2); }               \
+        else { CALL(T, 32, 8, 4); }                             \
+    }                                                           \
+    else if (N <= 32) { CALL(T, 32, 1, 1); }                    \
+    else if (N <= 64) { CALL(T, 32, 1, 2); }                    \
+    else if (N <= 128) { CALL(T, 32, 1, 4); }                   \
+    else if (N <= 256) { CALL(T, 32, 1, 8); }                   \
+    else if (N <= 512) { CALL(T, 32, 1, 16); }                  \
+    else { CALL(T, 32, 1, 32); }
 
 }  // namespace momoe
 
@@ -427,7 +472,7 @@ MOMOE_API int momoe_balance_loss(const void* logits_MN, int32_t type, const int3
     a.g = grad_BN;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const size_t smem = static_cast<size_t>(BAL_WARPS + 1) * N * 4;   // 36 KiB at most
-#define BAL_PARTIAL(T, V, NV) balance_partial_kernel<T, V, NV><<<a.n_blk, BAL_THREADS, smem, st>>>(a)
+#define BAL_PARTIAL(T, L, V, NV) balance_partial_kernel<T, L, V, NV><<<a.n_blk, BAL_THREADS, smem, st>>>(a)
     if (type == 0) { BAL_DISPATCH(__nv_bfloat16, BAL_PARTIAL) }
     else { BAL_DISPATCH(float, BAL_PARTIAL) }
 #undef BAL_PARTIAL
@@ -445,13 +490,16 @@ MOMOE_API int momoe_balance_loss_backward(const void* logits_MN, int32_t type, c
     if (logits_MN == nullptr || grad_BN == nullptr || grad_loss == nullptr || G_logits_MN == nullptr)
         return MOMOE_ERR_ARG;
     if (((reinterpret_cast<uintptr_t>(logits_MN) | reinterpret_cast<uintptr_t>(add_MN) |
-          reinterpret_cast<uintptr_t>(G_logits_MN)) & 15) != 0)
+          reinterpret_cast<uintptr_t>(G_logits_MN) | reinterpret_cast<uintptr_t>(grad_BN)) & 15) != 0)
         return MOMOE_ERR_ARG;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int grid = (M + BAL_WARPS - 1) / BAL_WARPS;
-#define BAL_BACKWARD(T, V, NV)                                                                                  \
-    balance_backward_kernel<T, V, NV><<<grid, BAL_THREADS, 0, st>>>(                                            \
-        static_cast<const T*>(logits_MN), BalSeqs{cu_seqlens, seq_len, B, M}, grad_BN, N, Ks, z_coef, grad_loss,      \
+    // rows of a warp: four blocks an SM, at least the rows that lie side by side in a warp
+    int RW = (M + sm_count() * 4 * BAL_WARPS - 1) / (sm_count() * 4 * BAL_WARPS);
+    RW = RW < 8 ? 8 : RW;
+    const int grid = ((M + RW - 1) / RW + BAL_WARPS - 1) / BAL_WARPS;
+#define BAL_BACKWARD(T, L, V, NV)                                                                               \
+    balance_backward_kernel<T, L, V, NV><<<grid, BAL_THREADS, 0, st>>>(                                         \
+        static_cast<const T*>(logits_MN), BalSeqs{cu_seqlens, seq_len, B, M}, grad_BN, N, Ks, RW, z_coef, grad_loss,  \
         static_cast<const T*>(add_MN), static_cast<T*>(G_logits_MN))
     if (type == 0) { BAL_DISPATCH(__nv_bfloat16, BAL_BACKWARD) }
     else { BAL_DISPATCH(float, BAL_BACKWARD) }

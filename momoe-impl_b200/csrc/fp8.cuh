@@ -42,35 +42,65 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
 }
 __device__ __forceinline__ uint8_t fp8_one(float a) { return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3); }
 
-// Eight consecutive values of a row in 32 bits.
+// Eight consecutive values of a row as they lie in memory, read past L1 (each is used once), and in 32 bits.
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+    uint4 q;
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
+    return q;
+}
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]);
+struct Raw8;
 template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+struct Raw8<float> {
+    uint4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = ld_stream(p);
+        b = ld_stream(p + 4);
     }
-}
-template <>
-__device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+    __device__ __forceinline__ void unpack(float (&v)[8]) const {
+        v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+        v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
     }
+};
+template <>
+struct Raw8<__nv_bfloat16> {
+    uint4 q;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { q = ld_stream(p); }
+    __device__ __forceinline__ void unpack(float (&v)[8]) const {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+template <>
+struct Raw8<__half> {
+    uint4 q;
+    __device__ __forceinline__ void load(const __half* p) { q = ld_stream(p); }
+    __device__ __forceinline__ void unpack(float (&v)[8]) const {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+};
+// The same through L1, for what other threads read as well.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    Raw8<T> r;
+    const uint4* q = reinterpret_cast<const uint4*>(p);
+    if constexpr (sizeof(T) == 4) {
+        r.a = __ldg(q);
+        r.b = __ldg(q + 1);
+    } else {
+        r.q = __ldg(q);
+    }
+    r.unpack(v);
 }
 // Rounds the eight values to T, stores them and leaves the rounded values in v.
 template <typename T>

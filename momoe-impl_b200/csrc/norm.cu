@@ -9,8 +9,9 @@
 //   gy * xhat.  gx is the gradient of x and of the residual alike.
 //
 // Everything is bound by HBM: each tensor crosses it once, a row lives in registers between its two uses.  A row belongs
-// to TPR threads that hold up to 4 chunks of 8 columns each (16-byte accesses): one warp up to 1024 columns, one thread
-// block of 128, 256 or 512 threads up to 4096, 8192, 16384.  Sums are 32-bit.
+// to a warp up to 512 columns and to a thread block above; a thread holds 2 chunks of 8 columns (4 above 8192 columns), so
+// that a block has few idle threads at widths between powers of two and enough blocks fit an SM to keep 60 KiB and more
+// in flight.  Sums are 32-bit.
 #include <cmath>
 
 #include "fp8.cuh"
@@ -19,25 +20,36 @@
 
 namespace momoe {
 
-constexpr int NORM_CH = 4;             // chunks of 8 columns a thread holds
-constexpr int NORM_MAX_D = 512 * NORM_CH * 8;
+constexpr int NORM_MAX_THREADS = 512;
+constexpr int NORM_MAX_D = NORM_MAX_THREADS * 4 * 8;
+
+// How a row of n chunks is shared out: chunks a thread holds, threads of a row, rows of a block.
+struct NormShape {
+    int ch, tpr, rows;
+};
+static NormShape norm_shape(int D) {
+    const int n = D >> 3;
+    if (n <= 64) return {2, 32, 4};
+    const int ch = n <= 2 * NORM_MAX_THREADS ? 2 : 4;
+    return {ch, ((n + ch - 1) / ch + 31) / 32 * 32, 1};
+}
 
 __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// Sum over the TPR threads of a row; every one of them gets it.  `buf` is written again only after the next barrier.
-template <int TPR>
+// Sum over the threads of a row (a warp, or the whole block); every one of them gets it.  `buf` is written again only
+// after the next barrier.
+template <bool BLOCK>
 __device__ __forceinline__ float row_sum(float v, float* buf) {
     v = lanes_sum(v);
-    if constexpr (TPR > 32) {
+    if constexpr (BLOCK) {
+        const int n = blockDim.x >> 5, lane = threadIdx.x & 31;
         __syncthreads();
-        if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+        if (lane == 0) buf[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = 0.0f;
-#pragma unroll
-        for (int i = 0; i < TPR / 32; ++i) v += buf[i];
+        v = lanes_sum(lane < n ? buf[lane] : 0.0f);
     }
     return v;
 }
@@ -64,49 +76,56 @@ __device__ __forceinline__ void load_weight8(const void* w, int w_fp32, int col,
     else load8(static_cast<const T*>(w) + col, v);
 }
 
-template <typename T, int TPR>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const NormArgs<T> g) {
-    __shared__ float buf[TPR > 32 ? TPR / 32 : 1];
-    constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
-    const int t = threadIdx.x % TPR;
-    const int m = blockIdx.x * ROWS + threadIdx.x / TPR;
-    if (m >= g.M) return;                       // ROWS > 1 only with TPR = 32: whole warps leave
+template <typename T, int CH, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 128) rms_norm_kernel(const NormArgs<T> g) {
+    __shared__ float buf[32];
+    const int TPR = BLOCK ? blockDim.x : 32;
+    const int t = BLOCK ? threadIdx.x : threadIdx.x & 31;
+    const int m = BLOCK ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (m >= g.M) return;                       // whole warps leave, and only where a row is a warp's
     const int n_chunks = g.D >> 3;
     const T* x = g.x + m * g.x_stride;
-    float v[NORM_CH][8];
-    float sq = 0.0f;
+    Raw8<T> rx[CH], re[CH];
 #pragma unroll
-    for (int i = 0; i < NORM_CH; ++i) {
+    for (int i = 0; i < CH; ++i) {
         const int c = t + i * TPR;
-        if (c < n_chunks) load8(x + c * 8, v[i]);
+        if (c < n_chunks) rx[i].load(x + c * 8);
     }
     if (g.res != nullptr) {
         const T* res = g.res + m * g.res_stride;
-        T* r = g.r + static_cast<size_t>(m) * g.D;
 #pragma unroll
-        for (int i = 0; i < NORM_CH; ++i) {
+        for (int i = 0; i < CH; ++i) {
             const int c = t + i * TPR;
-            if (c < n_chunks) {
-                float a[8];
-                load8(res + c * 8, a);
+            if (c < n_chunks) re[i].load(res + c * 8);
+        }
+    }
+    float v[CH][8];
+    float sq = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] += a[j];
-                store8(r + c * 8, v[i]);        // leaves the rounded sum in v
-            }
+    for (int i = 0; i < CH; ++i) {
+        const int c = t + i * TPR;
+        if (c >= n_chunks) continue;
+        rx[i].unpack(v[i]);
+        if (g.res != nullptr) {
+            float a[8];
+            re[i].unpack(a);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] += a[j];
+            store8(g.r + static_cast<size_t>(m) * g.D + c * 8, v[i]);        // leaves the rounded sum in v
         }
     }
 #pragma unroll
-    for (int i = 0; i < NORM_CH; ++i)
+    for (int i = 0; i < CH; ++i)
         if (t + i * TPR < n_chunks) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) sq = fmaf(v[i][j], v[i][j], sq);
         }
-    sq = row_sum<TPR>(sq, buf);
+    sq = row_sum<BLOCK>(sq, buf);
     const float rstd = 1.0f / sqrtf(sq / static_cast<float>(g.D) + g.eps);
     if (t == 0 && g.rstd != nullptr) g.rstd[m] = rstd;
     const int n_blocks = (g.D + FP8_BLOCK - 1) / FP8_BLOCK;
 #pragma unroll
-    for (int i = 0; i < NORM_CH; ++i) {
+    for (int i = 0; i < CH; ++i) {
         const int c = t + i * TPR;
         if (c - (t & 31) >= n_chunks) break;    // the whole warp is past the row's end
         const bool in = c < n_chunks;
@@ -140,7 +159,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_kernel(const N
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// Every group of TPR threads walks rows g, g + G, g + 2G, ... and keeps the weight's gradient of its columns in
+// Every group (a warp or a block) walks rows g, g + G, g + 2G, ... and keeps the weight's gradient of its columns in
 // registers; the groups' partial sums go to `part` [G, D] and a second kernel adds them in a fixed order, so the result
 // does not depend on timing.
 template <typename T>
@@ -157,61 +176,71 @@ struct NormBwdArgs {
     float* part;         // null: no weight gradient
 };
 
-template <typename T, int TPR>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_backward_kernel(const NormBwdArgs<T> g) {
-    __shared__ float buf[TPR > 32 ? TPR / 32 : 1];
-    constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
-    const int t = threadIdx.x % TPR;
-    const int group = blockIdx.x * ROWS + threadIdx.x / TPR;
+template <typename T, int CH, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 128) rms_norm_backward_kernel(const NormBwdArgs<T> g) {
+    __shared__ float buf[32];
+    const int TPR = BLOCK ? blockDim.x : 32;
+    const int t = BLOCK ? threadIdx.x : threadIdx.x & 31;
+    const int group = BLOCK ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
     if (group >= g.G) return;
     const int n_chunks = g.D >> 3;
     const float inv_d = 1.0f / static_cast<float>(g.D);
-    float gw[NORM_CH][8];
+    float gw[CH][8];
 #pragma unroll
-    for (int i = 0; i < NORM_CH; ++i)
+    for (int i = 0; i < CH; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) gw[i][j] = 0.0f;
+#pragma unroll 1
     for (int m = group; m < g.M; m += g.G) {
         const T* gy = g.gy + static_cast<size_t>(m) * g.D;
+        const T* gr = g.gr + static_cast<size_t>(m) * g.D;
         const T* r = g.r + m * g.r_stride;
-        const float rstd = g.rstd[m];
-        float a[NORM_CH][8], b[NORM_CH][8];
+        // all three tensors are asked for before the first is used (with 4 chunks there is no room to hold the third)
+        Raw8<T> ry[CH], rr[CH], re[CH];
 #pragma unroll
-        for (int i = 0; i < NORM_CH; ++i) {
+        for (int i = 0; i < CH; ++i) {
             const int c = t + i * TPR;
             if (c < n_chunks) {
-                load8(gy + c * 8, a[i]);
-                load8(r + c * 8, b[i]);
+                ry[i].load(gy + c * 8);
+                rr[i].load(r + c * 8);
+                if (CH <= 2 && g.gr != nullptr) re[i].load(gr + c * 8);
             }
         }
+        const float rstd = g.rstd[m];
         float dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NORM_CH; ++i) {
+        for (int i = 0; i < CH; ++i) {
             const int c = t + i * TPR;
             if (c < n_chunks) {
-                float w[8];
+                float w[8], a[8], b[8];
                 load_weight8<T>(g.w, g.w_fp32, c * 8, w);
+                ry[i].unpack(a);
+                rr[i].unpack(b);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    b[i][j] *= rstd;                              // xhat
-                    gw[i][j] = fmaf(a[i][j], b[i][j], gw[i][j]);
-                    a[i][j] *= w[j];                              // gh
-                    dot = fmaf(a[i][j], b[i][j], dot);
+                    b[j] *= rstd;                              // xhat
+                    gw[i][j] = fmaf(a[j], b[j], gw[i][j]);
+                    dot = fmaf(a[j] * w[j], b[j], dot);        // gh * xhat
                 }
             }
         }
-        dot = row_sum<TPR>(dot, buf) * inv_d;
+        dot = row_sum<BLOCK>(dot, buf) * inv_d;
         T* gx = g.gx + static_cast<size_t>(m) * g.D;
 #pragma unroll
-        for (int i = 0; i < NORM_CH; ++i) {
+        for (int i = 0; i < CH; ++i) {
             const int c = t + i * TPR;
             if (c < n_chunks) {
-                float o[8];
+                // gh and xhat again from the values as they were read: cheaper than registers to keep them
+                float w[8], a[8], b[8], o[8];
+                load_weight8<T>(g.w, g.w_fp32, c * 8, w);
+                ry[i].unpack(a);
+                rr[i].unpack(b);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = rstd * (a[i][j] - b[i][j] * dot);
+                for (int j = 0; j < 8; ++j) o[j] = rstd * (a[j] * w[j] - b[j] * rstd * dot);
                 if (g.gr != nullptr) {
                     float e[8];
-                    load8(g.gr + static_cast<size_t>(m) * g.D + c * 8, e);
+                    if (CH > 2) re[i].load(gr + c * 8);
+                    re[i].unpack(e);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) o[j] += e[j];
                 }
@@ -222,7 +251,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) rms_norm_backward_kerne
     if (g.part != nullptr) {
         float* part = g.part + static_cast<size_t>(group) * g.D;
 #pragma unroll
-        for (int i = 0; i < NORM_CH; ++i) {
+        for (int i = 0; i < CH; ++i) {
             const int c = t + i * TPR;
             if (c < n_chunks) store8(part + c * 8, gw[i]);
         }
@@ -236,8 +265,10 @@ __global__ void __launch_bounds__(1024) rms_norm_weight_grad_kernel(const float*
     __shared__ float s[32][33];
     const int d = blockIdx.x * 32 + threadIdx.x;
     float v = 0.0f;
-    if (d < D)
+    if (d < D) {
+#pragma unroll 8
         for (int i = threadIdx.y; i < G; i += 32) v += part[static_cast<size_t>(i) * D + d];
+    }
     s[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
     v = lanes_sum(s[threadIdx.x][threadIdx.y]);
@@ -281,32 +312,30 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Groups of the backward pass: enough of them to fill the GPU (three blocks of 128 threads or one of 512 an SM at the
-// kernel's registers), no more, since each leaves a row of partial sums.
+// Groups of the backward pass: as many as are resident at 80 registers a thread, no more, since each leaves a row of
+// partial sums.
 static int norm_groups(int M, int D) {
-    const int n = D >> 3;
-    const int sms = sm_count();
-    const int groups = n <= 32 * NORM_CH ? sms * 12 : n <= 128 * NORM_CH ? sms * 3 : n <= 256 * NORM_CH ? sms * 2 : sms;
+    const NormShape s = norm_shape(D);
+    const int groups = sm_count() * (768 / s.tpr > 0 ? 768 / s.tpr : 1);
     return M < groups ? M : groups;
 }
 
+#define NORM_DISPATCH(KERNEL, ROWS)                                                                            \
+    if (s.rows > 1) KERNEL<T, 2, false><<<((ROWS) + 3) / 4, 128, 0, st>>>(g);                                  \
+    else if (s.ch == 2) KERNEL<T, 2, true><<<(ROWS), s.tpr, 0, st>>>(g);                                       \
+    else KERNEL<T, 4, true><<<(ROWS), s.tpr, 0, st>>>(g);
+
 template <typename T>
 static int norm_launch(const NormArgs<T>& g, cudaStream_t st) {
-    const int n = g.D >> 3;
-    if (n <= 32 * NORM_CH) rms_norm_kernel<T, 32><<<(g.M + 3) / 4, 128, 0, st>>>(g);
-    else if (n <= 128 * NORM_CH) rms_norm_kernel<T, 128><<<g.M, 128, 0, st>>>(g);
-    else if (n <= 256 * NORM_CH) rms_norm_kernel<T, 256><<<g.M, 256, 0, st>>>(g);
-    else rms_norm_kernel<T, 512><<<g.M, 512, 0, st>>>(g);
+    const NormShape s = norm_shape(g.D);
+    NORM_DISPATCH(rms_norm_kernel, g.M)
     return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
 
 template <typename T>
 static int norm_backward_launch(const NormBwdArgs<T>& g, void* gw, cudaStream_t st) {
-    const int n = g.D >> 3;
-    if (n <= 32 * NORM_CH) rms_norm_backward_kernel<T, 32><<<(g.G + 3) / 4, 128, 0, st>>>(g);
-    else if (n <= 128 * NORM_CH) rms_norm_backward_kernel<T, 128><<<g.G, 128, 0, st>>>(g);
-    else if (n <= 256 * NORM_CH) rms_norm_backward_kernel<T, 256><<<g.G, 256, 0, st>>>(g);
-    else rms_norm_backward_kernel<T, 512><<<g.G, 512, 0, st>>>(g);
+    const NormShape s = norm_shape(g.D);
+    NORM_DISPATCH(rms_norm_backward_kernel, g.G)
     if (gw != nullptr) {
         const dim3 grid((g.D + 31) / 32), block(32, 32);
         if (g.w_fp32) rms_norm_weight_grad_kernel<<<grid, block, 0, st>>>(g.part, g.G, g.D, static_cast<float*>(gw));

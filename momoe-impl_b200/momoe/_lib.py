@@ -1,10 +1,10 @@
-"""ctypes binding of libmomoe_b200.so (the C ABI declared in include/momoe_b200.h).
+"""ctypes binding of libmomoe_b200.so (the C ABI declared in include/momoe_b200.h), and the compiled binding `native` of
+the operators around the expert layer (csrc/binding.cpp), whose calls are too short for Python on the way.
 
 There is no fallback: if the library is missing, importing this module raises with the build command.
 """
 import contextlib
 import ctypes as C
-import functools
 import os
 
 import torch
@@ -18,6 +18,12 @@ if not os.path.exists(LIB_PATH):
         "There is no CPU or PyTorch fallback for the MoMoE kernels.")
 
 lib = C.CDLL(LIB_PATH)
+
+if not os.path.exists(os.path.join(_HERE, "_native.so")):
+    raise ImportError("_native.so is not built; run `python momoe-impl_b200/build.py` (needs g++ and torch's headers)")
+from . import _native as native      # noqa: E402  (torch tensors in, the same library underneath)
+
+native.bind(LIB_PATH)
 
 c_i32, c_i64, c_vp, c_sz, c_u32 = C.c_int32, C.c_int64, C.c_void_p, C.c_size_t, C.c_uint32
 
@@ -187,10 +193,3 @@ def as_rows(t):
 def pitch(r):
     """Row pitch in elements of a tensor from as_rows."""
     return r.stride(0) if r.shape[0] > 1 else r.shape[1]
-
-
-# Sizes that a shape asks for, remembered: a call into the library costs more than the look-up.
-rms_norm_backward_workspace_bytes = functools.lru_cache(4096)(lib.momoe_rms_norm_backward_workspace_bytes)
-balance_loss_workspace_bytes = functools.lru_cache(4096)(lib.momoe_balance_loss_workspace_bytes)
-fp8_experts_workspace_bytes = functools.lru_cache(4096)(lib.momoe_fp8_experts_workspace_bytes)
-fp8_experts_launches = functools.lru_cache(4096)(lib.momoe_fp8_experts_launches)

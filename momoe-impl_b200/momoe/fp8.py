@@ -10,7 +10,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, ops
-from ._lib import aligned, as_rows, lib, on_device, pitch, ptr, raw_stream
+from ._lib import as_rows, lib, native, on_device, pitch, ptr, raw_stream
 
 BLOCK = 128                      # values that share a scale
 # Calls with at most this many rows per expert on average stream the weights past the rows; more take the row-tile kernels.
@@ -93,14 +93,6 @@ def quantize_experts(Wl1_ND2H, Wl2_NHD):
     return Fp8Experts(W1, S1, W2, S2.view(N, _blocks(D), _blocks(H)))
 
 
-def _check_tensor(t, name, shape, dtype):
-    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
-        raise RuntimeError("%s must be a contiguous %s of shape %s, but got: %s of shape %s, strides %s"
-                           % (name, dtype, list(shape), t.dtype, list(t.shape), list(t.stride())))
-    if t.data_ptr() % 16 != 0:
-        raise RuntimeError("%s must start on a 16-byte boundary" % name)
-
-
 def experts_forward(x, topk_idx_MK, topk_w_MK, experts):
     """Weighted sum of the K chosen experts' outputs for each token, in 8 bits.
 
@@ -109,54 +101,8 @@ def experts_forward(x, topk_idx_MK, topk_w_MK, experts):
     N <= 1024, K <= 32.  Returns (y bfloat16 [M, D], tokens_per_expert_N int64 [N]).  The hidden values are converted to
     8-bit rows once, from 32 bits.  No host synchronisation: an expert id out of range (202) is reported through the
     device's status word like the other problems only the device can see."""
-    rows8 = isinstance(x, Fp8Rows)
-    data = x.q if rows8 else x
-    dev = _lib.require_one_device(data, x.scale if rows8 else None, topk_idx_MK, topk_w_MK, *experts)
-    if torch.is_grad_enabled() and (data.requires_grad or topk_w_MK.requires_grad):
-        raise RuntimeError("8-bit experts have no backward pass: call them under torch.no_grad()")
-    if experts.W2_NDH.dim() != 3 or data.dim() != 2 or topk_idx_MK.dim() != 2 or topk_idx_MK.shape[0] != data.shape[0]:
-        raise RuntimeError("x must be [M, D], topk_idx_MK [M, K] and the weights [N, 2H, D] and [N, D, H], but got: %s, %s, "
-                           "%s and %s" % (list(data.shape), list(topk_idx_MK.shape), list(experts.W1_N2HD.shape),
-                                          list(experts.W2_NDH.shape)))
-    N, D, H = experts.sizes
-    M, K = topk_idx_MK.shape
-    if D % 16 != 0 or H % 16 != 0 or D == 0 or H == 0:
-        raise RuntimeError("8-bit experts need D and H in multiples of 16, but got: D = %d, H = %d" % (D, H))
-    _check_tensor(experts.W1_N2HD, "W1_N2HD", (N, 2 * H, D), E4M3)
-    _check_tensor(experts.W2_NDH, "W2_NDH", (N, D, H), E4M3)
-    _check_tensor(experts.S1, "S1", (N, 2, _blocks(H), _blocks(D)), E8M0)
-    _check_tensor(experts.S2, "S2", (N, _blocks(D), _blocks(H)), E8M0)
-    if K == 0 or K > N:
-        raise RuntimeError("each token needs 1 to N = %d experts, but got K = %d" % (N, K))
-    if topk_w_MK.shape != topk_idx_MK.shape:
-        raise RuntimeError("topk_w_MK must be like topk_idx_MK, %s, but got: %s"
-                           % (list(topk_idx_MK.shape), list(topk_w_MK.shape)))
-    if data.shape[1] != D or not data.is_floating_point():
-        raise RuntimeError("x must be floating-point [M, %d], but got: %s %s" % (D, data.dtype, list(data.shape)))
-    with on_device(dev):
-        scale_ptr = None
-        if rows8:
-            data, scale = aligned(data.contiguous()), x.scale.contiguous()
-            _check_tensor(data, "x.q", (M, D), E4M3)
-            if scale.shape != (M, _blocks(D)) or scale.dtype != E8M0:
-                raise RuntimeError("x.scale must be %s of shape %s, but got: %s of shape %s"
-                                   % (E8M0, [M, _blocks(D)], scale.dtype, list(scale.shape)))
-            scale_ptr = scale.data_ptr()
-        else:
-            if data.dtype != torch.bfloat16:
-                data = data.detach().to(torch.bfloat16)
-            data = aligned(data.contiguous())
-        idx = (topk_idx_MK if topk_idx_MK.dtype == torch.int32 else topk_idx_MK.to(torch.int32)).contiguous()
-        w = (topk_w_MK if topk_w_MK.dtype == torch.float32 else topk_w_MK.detach().to(torch.float32)).contiguous()
-        y = torch.empty((M, D), dtype=torch.bfloat16, device=dev)
-        if M == 0:
-            return y, torch.zeros(N, dtype=torch.int64, device=dev)
-        sizes = torch.empty(N, dtype=torch.int64, device=dev)
-        nbytes = _lib.fp8_experts_workspace_bytes(M, N, K, D, H)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        ops._call("momoe_fp8_experts_forward", _lib.fp8_experts_launches(M, N, K), lib.momoe_fp8_experts_forward,
-                  data.data_ptr(), scale_ptr, idx.data_ptr(), w.data_ptr(), M, N, K, D, H, experts.W1_N2HD.data_ptr(),
-                  experts.S1.data_ptr(), experts.W2_NDH.data_ptr(), experts.S2.data_ptr(), STREAM_MAX_AVG_ROWS,
-                  y.data_ptr(), sizes.data_ptr(), ws.data_ptr(), nbytes, ops.status_word(dev).data_ptr(),
-                  raw_stream(dev))
+    q, scale = x if isinstance(x, Fp8Rows) else (x, None)
+    _lib.require_cuda(q)
+    y, sizes = native.experts_forward(q, scale, topk_idx_MK, topk_w_MK, *experts, STREAM_MAX_AVG_ROWS,
+                                      ops.status_word(q.device))
     return y, sizes

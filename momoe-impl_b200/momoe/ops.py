@@ -18,6 +18,11 @@ KERNEL_EVENTS = None
 NVTX = os.environ.get("MOMOE_B200_NVTX", "0") == "1"   # one NVTX range per C-ABI call, for timeline tools
 
 
+def launch_count():
+    """Kernels queued so far, through ctypes (LAUNCHES) and through the compiled binding."""
+    return LAUNCHES + _lib.native.launches()
+
+
 def _call(name, n_kernels, fn, *args):
     global LAUNCHES
     ev = KERNEL_EVENTS

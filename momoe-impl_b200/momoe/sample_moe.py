@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import balance, fp8, ops
-from ._lib import require_cuda
+from ._lib import native, require_cuda
 from .momoe import MoMoE, _CHECK, compact_routing_of
 from .topk_router import TopKRouter
 
@@ -45,7 +45,7 @@ class FusedMoEFunction(torch.autograd.Function):
                                                           inference=not any(ctx.needs_input_grad))
             ctx.aux = balance_coef != 0 or z_coef != 0
             if ctx.aux:
-                aux_loss, _, g_BN = balance._loss(logits_MN, topk_idx, Ks, balance_coef, z_coef, None, S, B)
+                aux_loss, _, g_BN = native.balance_forward(logits_MN, topk_idx, Ks, balance_coef, z_coef, None, S, B)
         ctx.plan = plan
         ctx.shape = (B, S, D)
         ctx.Ks = Ks
@@ -81,7 +81,7 @@ class FusedMoEFunction(torch.autograd.Function):
             if ctx.aux:
                 # the experts' share of the logits' gradient is in 16 bits already; the sum is formed in 32 and rounded
                 # once more, like every gradient that reaches the two gate GEMMs
-                G_L = balance._loss_backward(saved[6], saved[7], ctx.Ks, ctx.z_coef, None, S, B, G_aux, add=G_L)
+                G_L = native.balance_backward(saved[6], saved[7], ctx.Ks, ctx.z_coef, None, S, G_aux, G_L)
             G_x = torch.addmm(G_x, G_L, Wg.T)
             G_Wg = x_MD.T @ G_L
         ops.status_post(dev)
