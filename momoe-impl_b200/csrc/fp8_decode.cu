@@ -16,6 +16,10 @@
 // warps 2..5 are the epilogue (a thread has one weight column and 32 tokens at a time), warps 6..9 write scales to TMEM
 // (see the row-tile kernel).  There is one accumulator: the MMAs of an item wait for the read-out of the item before, while
 // the ring goes on filling; they need less than half of the time that the weights take.
+//
+// With so few items that half of the SMs would idle (one token), two CTAs of a cluster share an item's k axis: the second
+// stores its accumulators into the first one's shared memory, which adds them and goes on (XXX against YYY us for both GEMMs
+// of one token, D2048 H768 top-8).
 #include <cstring>
 
 #include "fp8.cuh"
@@ -35,7 +39,8 @@ constexpr int D8_X = 32 * D8_K;                  // 4 KiB: 32 token rows
 constexpr int D8_NT = 128;                       // tokens of a tile, columns of an accumulator
 constexpr int D8_STAGE = 2 * D8_W + D8_NT / 32 * D8_X;       // one k slice: two blocks of 128 weight rows, the token rows
 constexpr int D8_STAGES = 4;
-constexpr int D8_SMEM = D8_STAGES * D8_STAGE + 1024;
+template <int SPLIT>
+constexpr int D8_SMEM = D8_STAGES * D8_STAGE + (SPLIT > 1 ? 4 * 64 * 32 * 4 : 0) + 1024;
 constexpr int D8_SF_COL = 256;                   // TMEM: accumulators in columns 0..255, two copies of the scales behind
 constexpr int D8_TMEM_COLS = 512;
 
@@ -45,6 +50,7 @@ struct Fp8DecArgs {
     const int* row_token;
     const float* row_weight;
     int* status;
+    int tile_cap;            // entries of tile_expert, and 1 / 128 of those of row_token
     int n_cblk;
     int nkb;
     int out_cols;
@@ -63,14 +69,122 @@ __device__ __forceinline__ D8Item d8_item(const Fp8DecArgs& g, int item) {
     D8Item w;
     w.tile = item / g.n_cblk;
     w.cb = item - w.tile * g.n_cblk;
-    w.e = __ldg(g.tile_expert + w.tile);
+    w.e = __ldcg(g.tile_expert + w.tile);
     const int* rt = g.row_token + static_cast<size_t>(w.tile) * TILE_M;
-    const int r1 = __ldg(rt + 32), r2 = __ldg(rt + 64), r3 = __ldg(rt + 96);
+    const int r1 = __ldcg(rt + 32), r2 = __ldcg(rt + 64), r3 = __ldcg(rt + 96);
     w.n_sub = 1 + (r1 >= 0) + (r2 >= 0) + (r3 >= 0);
     return w;
 }
 
-template <bool UP>
+// What an epilogue warp keeps between read-outs.
+struct D8Epi {
+    uint32_t bar_acc_empty, bar_meet, bar_part_full, bar_part_free;
+    uint32_t part;           // split: this lane's place in the buffer of the first CTA
+    uint32_t* s_top;         // up: [2][4 quarters][32 tokens]
+    volatile int* abortp;
+    int rank;
+    int meet, parts;
+};
+
+template <int T>
+__device__ __forceinline__ void d8_tmem_ld(uint32_t taddr, uint32_t (&r)[T]) {
+    if constexpr (T == 8) tmem_ld8(taddr, r);
+    else tmem_ld32(taddr, r);
+}
+
+// The first T tokens of a 32-row block out of the accumulators (columns taddr and taddr + D8_NT), by the four epilogue
+// warps; `last`: hand the accumulators back.  False when a wait was abandoned.
+template <bool UP, int SPLIT, int T>
+__device__ __forceinline__ bool d8_read_out(const Fp8DecArgs& g, D8Epi& c, const D8Item& w, size_t row0, uint32_t taddr,
+                                            bool last) {
+    const int lane = threadIdx.x & 31, q = (threadIdx.x >> 5) & 3;
+    float wgt = 0.0f;
+    if constexpr (!UP) wgt = __ldcg(g.row_weight + row0 + lane);   // lane t holds the weight of token t
+    uint32_t r[T], rb[T];
+    d8_tmem_ld<T>(taddr, r);
+    d8_tmem_ld<T>(taddr + D8_NT, rb);
+    tmem_ld_wait();
+    if (last) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c.bar_acc_empty);
+    }
+    if constexpr (SPLIT > 1) {
+        // [quarter][T columns of both accumulators][lane] floats in the first CTA's shared memory
+        if (c.rank != 0) {
+            bool ok = mbar_wait_cluster(c.bar_part_free, (c.parts & 1u) ^ 1u, c.abortp, g.status, DEV_TIMEOUT_EPILOGUE);
+            if (!__all_sync(0xffffffffu, ok)) return false;
+            const uint32_t dst = mapa_shared(c.part, 0);
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                st_cluster_f32(dst + t * 128, r[t]);
+                st_cluster_f32(dst + (T + t) * 128, rb[t]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(c.bar_part_full, 0));
+            ++c.parts;
+            return true;
+        }
+        bool ok = mbar_wait_cluster(c.bar_part_full, c.parts & 1u, c.abortp, g.status, DEV_TIMEOUT_EPILOGUE);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        ++c.parts;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            r[t] = __float_as_uint(__uint_as_float(r[t]) + ld_shared_f32(c.part + t * 128));
+            rb[t] = __float_as_uint(__uint_as_float(rb[t]) + ld_shared_f32(c.part + (T + t) * 128));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(c.bar_part_free, 1));
+    }
+    if constexpr (UP) {
+        const int col = w.cb * 128 + q * 32 + lane;
+        float v[T];
+        uint32_t mine = 0u;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const float b = __uint_as_float(rb[t]);
+            v[t] = b * __fdividef(1.0f, 1.0f + __expf(-b)) * __uint_as_float(r[t]);
+            // columns past H have zero weights, so v is zero there
+            const uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(v[t]));
+            if (lane == t) mine = top;
+        }
+        const int mb = c.meet & 1;
+        uint32_t* s_top = c.s_top + mb * 128;
+        s_top[q * 32 + lane] = mine;
+        // this half of s_top is written again two meetings later, after every warp has been at the next one
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c.bar_meet);
+        bool ok = mbar_wait(c.bar_meet, static_cast<uint32_t>(mb), c.abortp, g.status, DEV_TIMEOUT_EPILOGUE);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        ++c.meet;
+        mine = max(max(s_top[lane], s_top[32 + lane]), max(s_top[64 + lane], s_top[96 + lane]));
+        const uint32_t byte = fp8_scale_byte(mine);
+        const float inv = fp8_inv_scale(byte);
+        if (q == 0 && lane < T)
+            g.h_scale[fp8_atom_offset(row0 + lane, w.cb >> 2, (g.n_cblk + 3) >> 2) + (w.cb & 3)] = static_cast<uint8_t>(byte);
+        uint8_t* dst = g.h + row0 * g.out_cols + col;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const float s = __shfl_sync(0xffffffffu, inv, t);
+            if (col < g.out_cols) dst[static_cast<size_t>(t) * g.out_cols] = fp8_one(v[t] * s);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int col = w.cb * 256 + i * 128 + q * 32 + lane;
+            __nv_bfloat16* dst = g.y + row0 * g.out_cols + col;
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const float s = __shfl_sync(0xffffffffu, wgt, t);
+                if (col < g.out_cols)
+                    dst[static_cast<size_t>(t) * g.out_cols] = __float2bfloat16_rn(__uint_as_float(i == 0 ? r[t] : rb[t]) * s);
+            }
+        }
+    }
+    return true;
+}
+
+template <bool UP, int SPLIT>
 __global__ void __launch_bounds__(D8_THREADS, 1)
 fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Fp8DecArgs g) {
     extern __shared__ uint8_t smem_raw[];
@@ -82,15 +196,21 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     __shared__ uint64_t bar_acc_empty;
     __shared__ uint64_t bar_meet;                    // up: the four epilogue warps have written their part of s_top
     __shared__ uint32_t s_top[UP ? 2 : 1][UP ? 4 : 1][UP ? 32 : 1];
+    __shared__ uint64_t bar_part_full[4];            // split: the other CTA's part of a quarter's accumulators has arrived
+    __shared__ uint64_t bar_part_free[4];            // split, other CTA: its buffer has been read
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t stage_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const int total_items = __ldg(g.sched + SCHED_N_TILES) * g.n_cblk;
-    if (total_items <= 0 || static_cast<int>(blockIdx.x) >= total_items) return;
     const int n_groups = (g.nkb + FP8_GROUP - 1) / FP8_GROUP;
+    // this CTA's part of the k axis, in groups of four slices
+    const int rank = SPLIT > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int grp0 = n_groups * rank / SPLIT, grp1 = n_groups * (rank + 1) / SPLIT;
+    const int kb_lo = grp0 * FP8_GROUP, kb_hi = min(g.nkb, grp1 * FP8_GROUP);
+    const int first_item = blockIdx.x / SPLIT, step_item = gridDim.x / SPLIT;
+    grid_launch_dependents();
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -105,6 +225,10 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         mbar_init(smem_u32(&bar_acc_full), 1);
         mbar_init(smem_u32(&bar_acc_empty), 4);
         mbar_init(smem_u32(&bar_meet), 4);
+        for (int w = 0; w < 4; ++w) {
+            mbar_init(smem_u32(&bar_part_full[w]), 1);
+            mbar_init(smem_u32(&bar_part_free[w]), 1);
+        }
         fence_mbar_init();
         tma_prefetch_desc(&tmW);
         tma_prefetch_desc(&tmX);
@@ -115,9 +239,16 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (SPLIT > 1) cluster_sync_all();     // the other CTA's barriers exist before anything arrives on them
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
     volatile int* abortp = &abort_flag;
+    // everything above ran beside the tail of the kernel before; from here on its results are read
+    grid_wait();
+    // the first item's entries are asked for together with the schedule (and clamped to the tables, which may be shorter)
+    const int n_tiles = __ldcg(g.sched + SCHED_N_TILES);
+    const D8Item first = d8_item(g, min(first_item, g.tile_cap * g.n_cblk - 1));
+    const int total_items = n_tiles * g.n_cblk;
 
     if (warp == 0) {
         // ================================================================ loads
@@ -125,9 +256,9 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int item = blockIdx.x; ok && item < total_items; item += gridDim.x) {
-                const D8Item w = d8_item(g, item);
-                for (int kb = 0; kb < g.nkb; ++kb) {
+            for (int item = first_item; ok && item < total_items; item += step_item) {
+                const D8Item w = item == first_item ? first : d8_item(g, item);
+                for (int kb = kb_lo; kb < kb_hi; ++kb) {
                     ok = mbar_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, abortp, g.status, DEV_TIMEOUT_PRODUCER);
                     if (!ok) break;
                     const uint32_t full = smem_u32(&bar_full[stage]);
@@ -155,13 +286,13 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
             uint32_t phase = 0, lo = lo0;
             int it = 0, gi = 0;
             bool ok = true;
-            for (int item = blockIdx.x; ok && item < total_items; item += gridDim.x, ++it) {
-                const D8Item w = d8_item(g, item);
+            for (int item = first_item; ok && item < total_items; item += step_item, ++it) {
+                const D8Item w = item == first_item ? first : d8_item(g, item);
                 const uint32_t n_field = static_cast<uint32_t>(w.n_sub * 32 >> 3) << 17;
                 ok = mbar_wait(smem_u32(&bar_acc_empty), (it & 1u) ^ 1u, abortp, g.status, DEV_TIMEOUT_MMA);
                 if (!ok) break;
                 tc_fence_after();
-                for (int grp = 0; ok && grp < n_groups; ++grp, ++gi) {
+                for (int grp = grp0; ok && grp < grp1; ++grp, ++gi) {
                     const uint32_t sf = tmem_base + D8_SF_COL + (gi & 1) * 16;
                     ok = mbar_wait(smem_u32(&bar_sf_full[gi & 1]), (gi >> 1) & 1u, abortp, g.status, DEV_TIMEOUT_MMA);
                     if (!ok) break;
@@ -169,7 +300,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
                     const int kb0 = grp * FP8_GROUP;
 #pragma unroll
                     for (int j = 0; j < FP8_GROUP; ++j) {
-                        if (ok && kb0 + j < g.nkb) {
+                        if (ok && kb0 + j < kb_hi) {
                             ok = mbar_wait(smem_u32(&bar_full[stage]), phase, abortp, g.status, DEV_TIMEOUT_MMA);
                             if (ok) {
                                 tc_fence_after();
@@ -180,7 +311,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
                                     for (uint32_t k = 0; k < 4; ++k)
                                         umma_fp8_lohi(tmem_base + i * D8_NT, lo + (i * D8_W >> 4) + k * 2u, desc_hi,
                                                       lo + (2 * D8_W >> 4) + k * 2u, desc_hi, idesc, sf + 4 * i, sf + 8,
-                                                      (kb0 + j + static_cast<int>(k)) != 0 ? 1u : 0u);
+                                                      (kb0 - kb_lo + j + static_cast<int>(k)) != 0 ? 1u : 0u);
                                 }
                                 umma_commit(smem_u32(&bar_empty[stage]));
                                 lo += D8_STAGE >> 4;
@@ -199,15 +330,15 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         bool ok = true;
         const uint32_t sf0 = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + D8_SF_COL;
         const int w_blocks = UP ? g.n_cblk : (g.out_cols + 127) / 128;
-        for (int item = blockIdx.x; ok && item < total_items; item += gridDim.x) {
-            const D8Item w = d8_item(g, item);
+        for (int item = first_item; ok && item < total_items; item += step_item) {
+            const D8Item w = item == first_item ? first : d8_item(g, item);
             const int i = (lane >> 2) & 1;
             const int wb = UP ? w.cb : w.cb * 2 + i;
             const bool have = wb < w_blocks;
             const uint8_t* ws = g.w_scale + ((static_cast<size_t>(w.e) * (UP ? 2 : 1) + (UP ? i : 0)) * w_blocks + wb) * g.nkb;
             const uint4* xs = reinterpret_cast<const uint4*>(g.x_scale + static_cast<size_t>(w.tile) * n_groups * FP8_ATOM);
-            for (int grp = 0; grp < n_groups; ++grp, ++gi) {
-                const uint4 xw = __ldg(xs + grp * 32 + lane);
+            for (int grp = grp0; grp < grp1; ++grp, ++gi) {
+                const uint4 xw = __ldcg(xs + grp * 32 + lane);
                 const int kb = grp * FP8_GROUP + (lane & 3);
                 uint32_t word = have && kb < g.nkb ? __ldg(ws + kb) : 127u;
                 word <<= 8 * (lane & 3);
@@ -233,75 +364,31 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         // ================================================================ epilogue (warps 2..5)
         const int q = warp & 3;
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-        int it = 0, meet = 0;
+        D8Epi c;
+        c.bar_acc_empty = smem_u32(&bar_acc_empty);
+        c.bar_meet = smem_u32(&bar_meet);
+        c.bar_part_full = smem_u32(&bar_part_full[q]);
+        c.bar_part_free = smem_u32(&bar_part_free[q]);
+        c.part = stage_base + D8_STAGES * D8_STAGE + (q * 64 * 32 + lane) * 4;
+        c.s_top = &s_top[0][0][0];
+        c.abortp = abortp;
+        c.rank = rank;
+        c.meet = c.parts = 0;
+        int it = 0;
         bool ok = true;
-        for (int item = blockIdx.x; ok && item < total_items; item += gridDim.x, ++it) {
-            const D8Item w = d8_item(g, item);
+        for (int item = first_item; ok && item < total_items; item += step_item, ++it) {
+            const D8Item w = item == first_item ? first : d8_item(g, item);
             ok = mbar_wait(smem_u32(&bar_acc_full), it & 1u, abortp, g.status, DEV_TIMEOUT_EPILOGUE);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            auto hand_back = [&]() {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&bar_acc_empty));
-            };
-#pragma unroll 1
-            for (int sub = 0; sub < w.n_sub; ++sub) {
+            for (int sub = 0; ok && sub < w.n_sub; ++sub) {
                 const size_t row0 = static_cast<size_t>(w.tile) * TILE_M + sub * 32;
-                uint32_t r[32], rb[32];
-                tmem_ld32(taddr + sub * 32, r);
-                tmem_ld32(taddr + D8_NT + sub * 32, rb);
-                tmem_ld_wait();
-                if (sub + 1 == w.n_sub) hand_back();
-                if constexpr (UP) {
-                    const int col = w.cb * 128 + q * 32 + lane;
-                    float v[32];
-                    uint32_t mine = 0u;
-#pragma unroll
-                    for (int t = 0; t < 32; ++t) {
-                        const float b = __uint_as_float(rb[t]);
-                        v[t] = b * __fdividef(1.0f, 1.0f + __expf(-b)) * __uint_as_float(r[t]);
-                        // columns past H have zero weights, so v is zero there
-                        const uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(v[t]));
-                        if (lane == t) mine = top;
-                    }
-                    const int mb = meet & 1;
-                    s_top[mb][q][lane] = mine;
-                    // s_top[mb] is written again two meetings later, after every warp has been at the next one
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&bar_meet));
-                    ok = mbar_wait(smem_u32(&bar_meet), static_cast<uint32_t>(mb), abortp, g.status, DEV_TIMEOUT_EPILOGUE);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    ++meet;
-                    mine = max(max(s_top[mb][0][lane], s_top[mb][1][lane]), max(s_top[mb][2][lane], s_top[mb][3][lane]));
-                    const uint32_t byte = fp8_scale_byte(mine);
-                    const float inv = fp8_inv_scale(byte);
-                    if (q == 0)
-                        g.h_scale[fp8_atom_offset(row0 + lane, w.cb >> 2, (g.n_cblk + 3) >> 2) + (w.cb & 3)] =
-                            static_cast<uint8_t>(byte);
-                    uint8_t* dst = g.h + row0 * g.out_cols + col;
-#pragma unroll
-                    for (int t = 0; t < 32; ++t) {
-                        const float s = __shfl_sync(0xffffffffu, inv, t);
-                        if (col < g.out_cols) dst[static_cast<size_t>(t) * g.out_cols] = fp8_one(v[t] * s);
-                    }
-                } else {
-                    const float wgt = __ldg(g.row_weight + row0 + lane);   // lane t holds the weight of token t
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int col = w.cb * 256 + i * 128 + q * 32 + lane;
-                        __nv_bfloat16* dst = g.y + row0 * g.out_cols + col;
-#pragma unroll
-                        for (int t = 0; t < 32; ++t) {
-                            const float s = __shfl_sync(0xffffffffu, wgt, t);
-                            if (col < g.out_cols)
-                                dst[static_cast<size_t>(t) * g.out_cols] =
-                                    __float2bfloat16_rn(__uint_as_float(i == 0 ? r[t] : rb[t]) * s);
-                        }
-                    }
-                }
+                const bool last = sub + 1 == w.n_sub;
+                // real rows come first; a token more costs a reduction and a store, so a few rows take the short form
+                const int real = __popc(__ballot_sync(0xffffffffu, __ldcg(g.row_token + row0 + lane) >= 0));
+                ok = real <= 8 ? d8_read_out<UP, SPLIT, 8>(g, c, w, row0, taddr + sub * 32, last)
+                               : d8_read_out<UP, SPLIT, 32>(g, c, w, row0, taddr + sub * 32, last);
             }
         }
     }
@@ -313,25 +400,33 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000LL) __nanosleep(1000);
     }
+    if constexpr (SPLIT > 1) cluster_sync_all();     // the other CTA may still write here
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem_base, D8_TMEM_COLS);
     }
 }
 
-template <bool UP>
+template <bool UP, int SPLIT>
 static int d8_launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const Fp8DecArgs& g, cudaStream_t stream) {
     static bool attr_set[64] = {false};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MOMOE_ERR_CUDA;
     if (!attr_set[dev]) {
-        if (cudaFuncSetAttribute(fp8_decode_kernel<UP>, cudaFuncAttributeMaxDynamicSharedMemorySize, D8_SMEM) !=
-            cudaSuccess)
+        if (cudaFuncSetAttribute(fp8_decode_kernel<UP, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 D8_SMEM<SPLIT>) != cudaSuccess)
             return MOMOE_ERR_CUDA;
         attr_set[dev] = true;
     }
-    fp8_decode_kernel<UP><<<sm_count(), D8_THREADS, D8_SMEM, stream>>>(tmW, tmX, g);
-    return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
+    return launch_dependent(fp8_decode_kernel<UP, SPLIT>, sm_count() / SPLIT * SPLIT, D8_THREADS, D8_SMEM<SPLIT>, stream,
+                            SPLIT, tmW, tmX, g) == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
+}
+
+// Whether the items leave half of the SMs idle: then two CTAs share an item's k axis.
+static bool d8_split(const momoe_plan_t* p, const Fp8DecArgs& g) {
+    const long long msum = static_cast<long long>(p->M) * p->K;
+    const long long tiles = msum / TILE_M + (msum < p->N ? msum : p->N);      // an upper bound
+    return tiles * g.n_cblk * 2 <= sm_count() && g.nkb > FP8_GROUP;
 }
 
 static void d8_args(const momoe_plan_t* p, Fp8DecArgs& g) {
@@ -341,6 +436,7 @@ static void d8_args(const momoe_plan_t* p, Fp8DecArgs& g) {
     g.row_token = p->row_token;
     g.row_weight = p->row_weight;
     g.status = p->status;
+    g.tile_cap = static_cast<int>(p->rows_capacity / TILE_M);
 }
 static inline bool d8_aligned(const void* p) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -372,7 +468,8 @@ MOMOE_API int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const uint8_t
     g.w_scale = S1;
     g.h = h_sorted;
     g.h_scale = h_scale;
-    return d8_launch<true>(tmW, tmX, g, static_cast<cudaStream_t>(stream));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return d8_split(plan, g) ? d8_launch<true, 2>(tmW, tmX, g, st) : d8_launch<true, 1>(tmW, tmX, g, st);
 }
 
 MOMOE_API int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
@@ -394,5 +491,6 @@ MOMOE_API int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const uint8_
     g.x_scale = h_scale;
     g.w_scale = S2;
     g.y = static_cast<__nv_bfloat16*>(y_sorted);
-    return d8_launch<false>(tmW, tmX, g, static_cast<cudaStream_t>(stream));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return d8_split(plan, g) ? d8_launch<false, 2>(tmW, tmX, g, st) : d8_launch<false, 1>(tmW, tmX, g, st);
 }

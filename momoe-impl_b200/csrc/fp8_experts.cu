@@ -2,6 +2,7 @@
 // them on the way), and one call that runs the whole forward pass (dispatch, two GEMMs, combine) out of one workspace.
 #include "fp8.cuh"
 #include "internal.h"
+#include "ptx.cuh"
 #include "../../include/momoe_b200.h"
 
 namespace momoe {
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(256) fp8_quantize_weights_kernel(const T* __re
 //   more: a first kernel counts each chunk and reserves its rows with one atomic for each (chunk, expert).
 // Rows inside an expert are handed out by atomics, in no fixed order.  No result depends on it: a row's values do not
 // depend on its place, and a token's K rows are added in the order of k.
-constexpr int DISPATCH_SMALL_PAIRS = 4096;
+constexpr int DISPATCH_SMALL_PAIRS = 16384;
 constexpr int DISPATCH_MAX_EXPERTS = 1024;
 constexpr int DISPATCH_MAX_TOPK = 32;
 
@@ -131,6 +132,33 @@ __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int m0 = blockIdx.x * a.chunk, m1 = min(a.M, m0 + a.chunk);
     const bool first = blockIdx.x == 0;
+    grid_launch_dependents();
+    constexpr int U = 4;             // groups of 512 columns in flight
+    const int n_chunks = a.D >> 4;
+    const int n_blocks = (a.D + FP8_BLOCK - 1) / FP8_BLOCK;
+    const int n_groups = (n_blocks + FP8_GROUP - 1) / FP8_GROUP;
+    uint4 lo[U], hi[U];
+    uint32_t byte[U];
+    auto fetch = [&](int m, int g0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = (g0 + u) * 32 + lane;
+            lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
+            byte[u] = 127u;
+            if (c < n_chunks) {
+                if constexpr (ROWS8) {
+                    lo[u] = __ldg(static_cast<const uint4*>(a.x) + static_cast<size_t>(m) * n_chunks + c);
+                    byte[u] = __ldg(a.x_scale + static_cast<size_t>(m) * n_blocks + (c >> 3));
+                } else {
+                    const uint4* src = static_cast<const uint4*>(a.x) + (static_cast<size_t>(m) * n_chunks + c) * 2;
+                    lo[u] = __ldg(src);
+                    hi[u] = __ldg(src + 1);
+                }
+            }
+        }
+    };
+    // the first token's row is on its way while the layout is worked out
+    if (m0 + warp < m1) fetch(m0 + warp, 0);
     if constexpr (SMALL) {
         for (int e = tid; e < a.N; e += 256) s_next[e] = s_total[e] = 0;
         __syncthreads();
@@ -196,10 +224,6 @@ __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a)
         if (lane == 0) a.sizes[e] = cnt;
     }
 
-    constexpr int U = 4;             // groups of 512 columns in flight
-    const int n_chunks = a.D >> 4;
-    const int n_blocks = (a.D + FP8_BLOCK - 1) / FP8_BLOCK;
-    const int n_groups = (n_blocks + FP8_GROUP - 1) / FP8_GROUP;
     for (int m = m0 + warp; m < m1; m += 8) {
         int p = 0;
         if (lane < a.K) {
@@ -211,24 +235,7 @@ __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a)
             a.row_weight[p] = __ldg(a.topk_w + i);
         }
         for (int g0 = 0; g0 < n_groups; g0 += U) {
-            uint4 lo[U], hi[U];
-            uint32_t byte[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int c = (g0 + u) * 32 + lane;
-                lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
-                byte[u] = 127u;
-                if (c < n_chunks) {
-                    if constexpr (ROWS8) {
-                        lo[u] = __ldg(static_cast<const uint4*>(a.x) + static_cast<size_t>(m) * n_chunks + c);
-                        byte[u] = __ldg(a.x_scale + static_cast<size_t>(m) * n_blocks + (c >> 3));
-                    } else {
-                        const uint4* src = static_cast<const uint4*>(a.x) + (static_cast<size_t>(m) * n_chunks + c) * 2;
-                        lo[u] = __ldg(src);
-                        hi[u] = __ldg(src + 1);
-                    }
-                }
-            }
+            if (g0 != 0 || m != m0 + warp) fetch(m, g0);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (g0 + u >= n_groups) break;
@@ -262,8 +269,11 @@ __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a)
 }
 
 static bool dispatch_small(int M, int K) { return static_cast<long long>(M) * K <= DISPATCH_SMALL_PAIRS; }
-// Tokens of a block: one a warp where every block counts all pairs anyway, four a warp where a chunk has a set-up of its own.
-static int dispatch_chunk(int M, int K) { return dispatch_small(M, K) ? 8 : 32; }
+// Tokens of a block: one a warp, more where there are more than four blocks an SM (a block has a set-up of its own).
+static int dispatch_chunk(int M) {
+    const int want = (M + 4 * sm_count() - 1) / (4 * sm_count());
+    return (want + 7) / 8 * 8;
+}
 
 // Parts of the workspace of a whole forward pass, each on a 256-byte boundary.
 struct Fp8Workspace {
@@ -323,7 +333,7 @@ MOMOE_API int momoe_fp8_quantize_weights(const void* W, int32_t type, int32_t N,
 
 MOMOE_API size_t momoe_fp8_dispatch_workspace_bytes(int32_t M, int32_t N, int32_t K) {
     if (M <= 0 || N <= 0 || K <= 0 || dispatch_small(M, K)) return 0;
-    const int c = dispatch_chunk(M, K);
+    const int c = dispatch_chunk(M);
     return (1 + static_cast<size_t>((M + c - 1) / c)) * N * 4;
 }
 
@@ -352,7 +362,7 @@ MOMOE_API int momoe_fp8_dispatch_rows(const void* x, const uint8_t* x_scale, con
     DispatchArgs a;
     a.x = x; a.x_scale = x_scale; a.topk_idx = topk_idx_MK; a.topk_w = topk_w_MK;
     a.M = M; a.N = N; a.K = K; a.D = D;
-    a.chunk = dispatch_chunk(M, K);
+    a.chunk = dispatch_chunk(M);
     a.total = static_cast<int*>(workspace);
     a.chunk_base = need > 0 ? a.total + N : nullptr;
     a.sizes = reinterpret_cast<long long*>(sizes_N);
@@ -422,5 +432,7 @@ MOMOE_API int momoe_fp8_experts_forward(const void* x_MD, const uint8_t* x_scale
     rc = decode ? momoe_fp8_down_scale_decode(&plan, u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, stream)
                 : momoe_fp8_down_scale(&plan, u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, stream);
     if (rc != MOMOE_OK) return rc;
-    return momoe_combine_rows(&plan, ws + l.rows, D, y_MD, stream);
+    // launched early beside the tile kernel its blocks wait there for long and slow it down (1124 against 1098 us at 16384
+    // tokens, D2048 H1024, top-8 of 128); behind the streaming kernel it saves a launch gap (30.7 against 32.5 us, 1 token)
+    return combine_rows(&plan, ws + l.rows, D, y_MD, stream, decode);
 }

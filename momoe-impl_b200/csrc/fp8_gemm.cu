@@ -78,10 +78,10 @@ struct Fp8Work {
 __device__ __forceinline__ Fp8Work f8_work(const Fp8Args& g, int item, uint32_t cta_rank) {
     Fp8Work w;
     w.nb = item % g.n_nblk;
-    const int info = __ldg(g.pair_info + item / g.n_nblk);
+    const int info = __ldcg(g.pair_info + item / g.n_nblk);
     w.tile = (info >> 1) + static_cast<int>(cta_rank);
     w.valid = cta_rank == 0 || (info & 1) != 0;
-    w.e = __ldg(g.tile_expert + (info >> 1));
+    w.e = __ldcg(g.tile_expert + (info >> 1));
     return w;
 }
 
@@ -110,9 +110,8 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     const uint32_t stage_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t epi_base = stage_base + F8_STAGES * F8_STAGE_BYTES;
 
-    const int total_items = __ldg(g.sched + SCHED_N_PAIRS) * g.n_nblk;
-    if (total_items <= 0 || cluster_id >= total_items) return;   // both CTAs of the cluster leave together
     const int n_groups = (g.nkb + FP8_GROUP - 1) / FP8_GROUP;
+    grid_launch_dependents();
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
@@ -142,6 +141,9 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
     volatile int* abortp = &abort_flag;
+    // everything above ran beside the tail of the kernel before; from here on its results are read
+    grid_wait();
+    const int total_items = __ldcg(g.sched + SCHED_N_PAIRS) * g.n_nblk;
 
     if (warp == 0) {
         // ================================================================ loads
@@ -244,7 +246,7 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 have = w.nb * 2 + i < g.b_blocks;
             }
             for (int grp = 0; grp < n_groups; ++grp, ++gi) {
-                const uint4 a = __ldg(src + grp * 32 + lane);
+                const uint4 a = __ldcg(src + grp * 32 + lane);
                 const int kb = grp * FP8_GROUP + (lane & 3);
                 uint32_t word = have && kb < g.nkb ? __ldg(bs + kb) : 127u;
                 word <<= 8 * (lane & 3);
@@ -296,7 +298,7 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             };
             float wgt = 0.0f;
             const size_t grow = static_cast<size_t>(w.tile) * TILE_M + row;
-            if constexpr (!UP) wgt = w.valid ? __ldg(g.row_weight + grow) : 0.0f;
+            if constexpr (!UP) wgt = w.valid ? __ldcg(g.row_weight + grow) : 0.0f;
             ok = mbar_wait(smem_u32(&bar_acc_full[ab]), (it >> 1) & 1u, abortp, g.status, DEV_TIMEOUT_EPILOGUE) &&
                  *abortp == 0;
             ok = __all_sync(0xffffffffu, ok);
@@ -462,8 +464,9 @@ static int f8_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUten
         }
         pairs[dev] = n < sm_count() / 2 ? n : sm_count() / 2;
     }
-    fp8_grouped_gemm_kernel<UP><<<2 * pairs[dev], F8_THREADS, F8_SMEM_BYTES<UP>, stream>>>(tmA, tmB, tmO, g);
-    return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
+    // (the cluster shape is the kernel's own attribute)
+    return launch_dependent(fp8_grouped_gemm_kernel<UP>, 2 * pairs[dev], F8_THREADS, F8_SMEM_BYTES<UP>, stream, 1, tmA, tmB,
+                            tmO, g) == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
 
 int fp8_check_plan(const momoe_plan_t* p) {

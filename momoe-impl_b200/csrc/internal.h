@@ -51,6 +51,28 @@ static inline void share_sm_with_gemm() {
         done[dev] = true;
     }
 }
+// Launch as a programmatic dependent of the kernel before it in the stream, in clusters of `cluster` blocks.  The kernel
+// calls grid_wait before it reads or writes anything that an earlier kernel touches.
+template <typename... P, typename... A>
+static inline cudaError_t launch_dependent(void (*kernel)(P...), int grid, int block, size_t smem, cudaStream_t stream,
+                                           int cluster, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(static_cast<unsigned>(block));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Shared-memory swizzle of a tensor map: the byte span inside which TMA permutes 16-byte chunks.
 enum TmapSwizzle : int { TMAP_SWIZZLE_128B = 0, TMAP_SWIZZLE_64B = 1, TMAP_SWIZZLE_32B = 2 };
 int encode_tmap_2d(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
@@ -61,4 +83,10 @@ int encode_tmap_3d(CUtensorMap* m, const void* base, uint64_t d2, uint64_t rows,
 int encode_tmap(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
                 const uint32_t* box, int swizzle);
 
+}  // namespace momoe
+
+struct momoe_plan;
+namespace momoe {
+// momoe_combine_rows; `dependent`: launched as a programmatic dependent of the kernel before it in the stream.
+int combine_rows(const momoe_plan* plan, const void* src_sorted, int32_t cols, void* dst, void* stream, bool dependent);
 }  // namespace momoe

@@ -24,7 +24,8 @@ SHAPES = [
     (129, 1, 1, 128, 4096, 0.0),
     (640, 5, 3, 4096, 48, 0.0),
     (90, 40, 6, 256, 144, 3.0),       # few rows on average, some experts with several 32-row blocks
-    (1400, 1000, 3, 64, 32, 1.0),     # many experts, more pairs than one launch dispatches
+    (1400, 1000, 3, 64, 32, 1.0),     # many experts
+    (6000, 40, 3, 96, 64, 1.0),       # more pairs than one launch dispatches
 ]
 
 
@@ -335,9 +336,9 @@ def test_an_expert_named_twice_counts_twice_and_bad_ids_are_reported(fp8):
         fp8.experts_forward(x, t(ids), w, e)
         with pytest.raises(RuntimeError, match="202"):
             ops.check_status()
-    many = t([[0, 1]]).expand(5000, 2).clone()               # the two-launch dispatch reports as well
+    many = t([[0, 1]]).expand(9000, 2).clone()               # the two-launch dispatch reports as well
     many[4321, 1] = 99
-    fp8.experts_forward(x[:1].expand(5000, 64), many, torch.ones(5000, 2, device="cuda"), e)
+    fp8.experts_forward(x[:1].expand(9000, 64), many, torch.ones(9000, 2, device="cuda"), e)
     with pytest.raises(RuntimeError, match="202"):
         ops.check_status()
     ops.check_status()
