@@ -280,33 +280,35 @@ int momoe_fp8_quantize_weights(const void* W, int32_t type, int32_t N, int32_t K
 
 /* Token-major rows -> expert-major 8-bit rows, with the tables of momoe_plan_t that the 8-bit GEMMs read, from a compact
  * routing: x is bf16 [M, D] (x_scale NULL) or e4m3 [M, D] with scales [M, ceil(D / 128)].  Experts without a token have no
- * tile, so rows_capacity is 128 * (ceil(M * K / 128) + min(N, M * K)) at least; tables as in momoe_plan_t.  Inside an
- * expert the rows are in no particular order (no result of a forward pass depends on it), and a token may name an expert
- * twice.  Padding rows of dst keep whatever the buffer held.  An id outside [0, N) sets *status to 202.  D a multiple of
- * 16, N <= 1024, K <= 32. */
+ * tile, so rows_capacity is 128 * (ceil(M * K / 128) + min(N, M * K)) at least; tables as in momoe_plan_t, and tile_rows
+ * int32[rows_capacity / 128]: the real rows of each tile, which come first in it.  Inside an expert the rows are in no
+ * particular order (no result of a forward pass depends on it), and a token may name an expert twice.  Padding rows of dst
+ * and row_weight keep whatever the buffers held.  An id outside [0, N) sets *status to 202.  D a multiple of 16, N <= 1024,
+ * K <= 32. */
 size_t momoe_fp8_dispatch_workspace_bytes(int32_t M, int32_t N, int32_t K);
 int momoe_fp8_dispatch_rows(const void* x, const uint8_t* x_scale, const int32_t* topk_idx_MK, const float* topk_w_MK,
                             int32_t M, int32_t N, int32_t K, int32_t D, int64_t* sizes_N, int32_t* tile_expert,
-                            int32_t* pair_info, int32_t* sched, int32_t* row_token, float* row_weight, int32_t* pos_MK,
+                            int32_t* pair_info, int32_t* sched, int32_t* tile_rows, float* row_weight, int32_t* pos_MK,
                             int64_t rows_capacity, void* workspace, size_t workspace_bytes, uint8_t* dst_sorted,
                             uint8_t* dst_scale, int32_t* status, momoe_stream_t stream);
 
 /* Up/gate GEMM + SwiGLU on 8-bit operands: a, b = x W1[e]^T (fp32), h = b sigmoid(b) a as 8-bit rows (rounded once, from
  * fp32).  W1 [N, 2H, D], S1 [N, 2, ceil(H / 128), ceil(D / 128)].  The second form streams the weights past a few rows an
- * expert.  Padding rows of the results are not defined.  D and H multiples of 16. */
+ * expert.  Of the plan they read sched, tile_expert, pair_info (first form) and row_weight (down).  Padding rows of the
+ * results are not defined.  D and H multiples of 16. */
 int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const uint8_t* x_sorted, const uint8_t* x_scale,
                         const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
                         momoe_stream_t stream);
-int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const uint8_t* x_sorted, const uint8_t* x_scale,
-                               const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
+int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* x_sorted,
+                               const uint8_t* x_scale, const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
                                momoe_stream_t stream);
 
 /* Down GEMM on 8-bit operands: y_sorted[r, :] = bf16(w[r] * (h[r, :] W2[e]^T)).  W2 [N, D, H],
  * S2 [N, ceil(D / 128), ceil(H / 128)]; y_sorted 32-byte aligned. */
 int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
                          const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, momoe_stream_t stream);
-int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
-                                const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, momoe_stream_t stream);
+int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* h_sorted,
+                                const uint8_t* h_scale, const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, momoe_stream_t stream);
 
 /* The whole forward pass of 8-bit experts from a compact routing: dispatch, up, down, combine, out of one workspace
  * (256-byte aligned).  x as for momoe_fp8_dispatch_rows; y_MD bf16 [M, D]; sizes_N int64 [N].  Calls with at

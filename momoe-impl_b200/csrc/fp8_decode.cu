@@ -47,10 +47,10 @@ constexpr int D8_TMEM_COLS = 512;
 struct Fp8DecArgs {
     const int* sched;
     const int* tile_expert;
-    const int* row_token;
+    const int* tile_rows;
     const float* row_weight;
     int* status;
-    int tile_cap;            // entries of tile_expert, and 1 / 128 of those of row_token
+    int tile_cap;            // entries of tile_expert and tile_rows
     int n_cblk;
     int nkb;
     int out_cols;
@@ -63,16 +63,16 @@ struct Fp8DecArgs {
 
 struct D8Item {
     int tile, cb, e;
-    int n_sub;       // 32-row blocks of the tile that hold real rows (which come first)
+    int rows;        // real rows of the tile (they come first)
+    int n_sub;       // 32-row blocks that hold them
 };
 __device__ __forceinline__ D8Item d8_item(const Fp8DecArgs& g, int item) {
     D8Item w;
     w.tile = item / g.n_cblk;
     w.cb = item - w.tile * g.n_cblk;
     w.e = __ldcg(g.tile_expert + w.tile);
-    const int* rt = g.row_token + static_cast<size_t>(w.tile) * TILE_M;
-    const int r1 = __ldcg(rt + 32), r2 = __ldcg(rt + 64), r3 = __ldcg(rt + 96);
-    w.n_sub = 1 + (r1 >= 0) + (r2 >= 0) + (r3 >= 0);
+    w.rows = __ldcg(g.tile_rows + w.tile);
+    w.n_sub = (w.rows + 31) >> 5;
     return w;
 }
 
@@ -385,9 +385,8 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
             for (int sub = 0; ok && sub < w.n_sub; ++sub) {
                 const size_t row0 = static_cast<size_t>(w.tile) * TILE_M + sub * 32;
                 const bool last = sub + 1 == w.n_sub;
-                // real rows come first; a token more costs a reduction and a store, so a few rows take the short form
-                const int real = __popc(__ballot_sync(0xffffffffu, __ldcg(g.row_token + row0 + lane) >= 0));
-                ok = real <= 8 ? d8_read_out<UP, SPLIT, 8>(g, c, w, row0, taddr + sub * 32, last)
+                // a token more costs a reduction and a store, so a few rows take the short form
+                ok = w.rows - sub * 32 <= 8 ? d8_read_out<UP, SPLIT, 8>(g, c, w, row0, taddr + sub * 32, last)
                                : d8_read_out<UP, SPLIT, 32>(g, c, w, row0, taddr + sub * 32, last);
             }
         }
@@ -429,11 +428,11 @@ static bool d8_split(const momoe_plan_t* p, const Fp8DecArgs& g) {
     return tiles * g.n_cblk * 2 <= sm_count() && g.nkb > FP8_GROUP;
 }
 
-static void d8_args(const momoe_plan_t* p, Fp8DecArgs& g) {
+static void d8_args(const momoe_plan_t* p, const int32_t* tile_rows, Fp8DecArgs& g) {
     memset(&g, 0, sizeof(g));
     g.sched = p->sched;
     g.tile_expert = p->tile_expert;
-    g.row_token = p->row_token;
+    g.tile_rows = tile_rows;
     g.row_weight = p->row_weight;
     g.status = p->status;
     g.tile_cap = static_cast<int>(p->rows_capacity / TILE_M);
@@ -446,12 +445,12 @@ using namespace momoe;
 
 #define MOMOE_API extern "C" __attribute__((visibility("default")))
 
-MOMOE_API int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const uint8_t* x_sorted, const uint8_t* x_scale,
-                                         const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted,
+MOMOE_API int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* x_sorted,
+                                         const uint8_t* x_scale, const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted,
                                          uint8_t* h_scale, momoe_stream_t stream) {
     int rc = fp8_check_plan(plan);
     if (rc != MOMOE_OK) return rc;
-    if (!d8_aligned(x_sorted) || !d8_aligned(x_scale) || !d8_aligned(W1_N2HD) || S1 == nullptr ||
+    if (tile_rows == nullptr || !d8_aligned(x_sorted) || !d8_aligned(x_scale) || !d8_aligned(W1_N2HD) || S1 == nullptr ||
         !d8_aligned(h_sorted) || !d8_aligned(h_scale))
         return MOMOE_ERR_ARG;
     const int D = plan->D, H = plan->H;
@@ -460,7 +459,7 @@ MOMOE_API int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const uint8_t
         return rc;
     if ((rc = encode_tmap_2d(&tmX, x_sorted, plan->rows_capacity, D / 2, 32, D8_K / 2)) != MOMOE_OK) return rc;
     Fp8DecArgs g;
-    d8_args(plan, g);
+    d8_args(plan, tile_rows, g);
     g.n_cblk = (H + 127) / 128;
     g.nkb = (D + D8_K - 1) / D8_K;
     g.out_cols = H;
@@ -472,19 +471,19 @@ MOMOE_API int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const uint8_t
     return d8_split(plan, g) ? d8_launch<true, 2>(tmW, tmX, g, st) : d8_launch<true, 1>(tmW, tmX, g, st);
 }
 
-MOMOE_API int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
-                                          const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted,
+MOMOE_API int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* h_sorted,
+                                          const uint8_t* h_scale, const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted,
                                           momoe_stream_t stream) {
     int rc = fp8_check_plan(plan);
     if (rc != MOMOE_OK) return rc;
-    if (!d8_aligned(h_sorted) || !d8_aligned(h_scale) || !d8_aligned(W2_NDH) || S2 == nullptr || !d8_aligned(y_sorted))
+    if (tile_rows == nullptr || !d8_aligned(h_sorted) || !d8_aligned(h_scale) || !d8_aligned(W2_NDH) || S2 == nullptr || !d8_aligned(y_sorted))
         return MOMOE_ERR_ARG;
     const int D = plan->D, H = plan->H;
     CUtensorMap tmW, tmX;
     if ((rc = encode_tmap_3d(&tmW, W2_NDH, plan->N, D, H / 2, 128, D8_K / 2)) != MOMOE_OK) return rc;
     if ((rc = encode_tmap_2d(&tmX, h_sorted, plan->rows_capacity, H / 2, 32, D8_K / 2)) != MOMOE_OK) return rc;
     Fp8DecArgs g;
-    d8_args(plan, g);
+    d8_args(plan, tile_rows, g);
     g.n_cblk = (D + 255) / 256;
     g.nkb = (H + D8_K - 1) / D8_K;
     g.out_cols = D;

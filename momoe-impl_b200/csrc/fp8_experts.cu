@@ -83,7 +83,7 @@ struct DispatchArgs {
     int* tile_expert;
     int* pair_info;
     int* sched;
-    int* row_token;
+    int* tile_rows;
     float* row_weight;
     int* pos;
     uint8_t* dst;
@@ -119,21 +119,24 @@ __device__ __forceinline__ uint4 fp8_convert16(const float (&v)[16], float inv) 
     return o;
 }
 
-// One warp a token: its row is read once, converted (ROWS8: copied) and stored to the K expert-major rows of its experts,
-// the scales in the blocks the GEMMs read.  A lane holds 16 columns, 8 lanes a block of 128, the warp the 512 columns
-// whose four scale bytes make one word.  Bound by HBM: M D (2 + K) bytes from 16-bit rows, M D (1 + K) from 8-bit ones.
-// Padding rows of dst are left as they are.
-template <bool ROWS8, bool SMALL>
+// A token's row is read once, converted (ROWS8: copied) and stored to the K expert-major rows of its experts, the scales in
+// the blocks the GEMMs read.  A lane holds 16 columns, 8 lanes a block of 128, a warp the 512 columns whose four scale
+// bytes make one word.  One warp a token, or (ONE, few tokens) one block a token, its warps on different columns.  Bound by
+// HBM: M D (2 + K) bytes from 16-bit rows, M D (1 + K) from 8-bit ones; by latency for few tokens (one token 7.9 us with one
+// warp a token, XXX with one block).  Padding rows of dst are left as they are.
+template <bool ROWS8, bool SMALL, bool ONE>
 __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a) {
+    constexpr int STEP = ONE ? 8 : 1;    // warps that share a token
     __shared__ int s_next[DISPATCH_MAX_EXPERTS];     // next row of each expert for this block
     __shared__ int s_total[DISPATCH_MAX_EXPERTS];
     __shared__ unsigned s_first[DISPATCH_MAX_EXPERTS];    // first tile | first pair << 16 of each expert
     __shared__ unsigned s_warp[8];
+    __shared__ int s_pos[DISPATCH_MAX_TOPK];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int m0 = blockIdx.x * a.chunk, m1 = min(a.M, m0 + a.chunk);
     const bool first = blockIdx.x == 0;
     grid_launch_dependents();
-    constexpr int U = 4;             // groups of 512 columns in flight
+    constexpr int U = ONE ? 1 : 4;       // groups of 512 columns in flight
     const int n_chunks = a.D >> 4;
     const int n_blocks = (a.D + FP8_BLOCK - 1) / FP8_BLOCK;
     const int n_groups = (n_blocks + FP8_GROUP - 1) / FP8_GROUP;
@@ -142,7 +145,7 @@ __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a)
     auto fetch = [&](int m, int g0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int c = (g0 + u) * 32 + lane;
+            const int c = (g0 + u) * 32 + lane;      // (g0 of a warp that shares its token: its own group)
             lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
             byte[u] = 127u;
             if (c < n_chunks) {
@@ -157,8 +160,9 @@ __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a)
             }
         }
     };
-    // the first token's row is on its way while the layout is worked out
-    if (m0 + warp < m1) fetch(m0 + warp, 0);
+    // the first columns are on their way while the layout is worked out
+    const int m_first = ONE ? m0 : m0 + warp, g_first = ONE ? warp : 0;
+    if (m_first < m1) fetch(m_first, g_first);
     if constexpr (SMALL) {
         for (int e = tid; e < a.N; e += 256) s_next[e] = s_total[e] = 0;
         __syncthreads();
@@ -209,33 +213,34 @@ __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a)
         a.sched[SCHED_PAD_ROWS] = static_cast<int>((all & 0xFFFFu) * TILE_M);
         a.sched[SCHED_N_PAIRS] = static_cast<int>(all >> 16);
     }
-    // the tables of the tiles, and token -1 on padding rows: the experts are shared out among the blocks
-    for (int e = blockIdx.x * 8 + warp; e < a.N; e += gridDim.x * 8) {
+    // the tables of the tiles: the experts are shared out among the blocks, a thread each
+    for (int e = blockIdx.x + gridDim.x * tid; e < a.N; e += gridDim.x * 256) {
         const int cnt = s_total[e], t0 = static_cast<int>(s_first[e] & 0xFFFFu), p0 = static_cast<int>(s_first[e] >> 16);
         const int nt = (cnt + TILE_M - 1) / TILE_M;
-        for (int t = lane; t < nt; t += 32) {
+        a.sizes[e] = cnt;
+        for (int t = 0; t < nt; ++t) {
             a.tile_expert[t0 + t] = e;
+            a.tile_rows[t0 + t] = min(cnt - t * TILE_M, TILE_M);
             if ((t & 1) == 0) a.pair_info[p0 + t / 2] = (t0 + t) * 2 + (t + 1 < nt ? 1 : 0);
         }
-        for (int r = cnt + lane; r < nt * TILE_M; r += 32) {
-            a.row_token[t0 * TILE_M + r] = -1;
-            a.row_weight[t0 * TILE_M + r] = 0.0f;
-        }
-        if (lane == 0) a.sizes[e] = cnt;
     }
 
-    for (int m = m0 + warp; m < m1; m += 8) {
+    for (int m = m_first; m < m1; m += ONE ? 1 : 8) {
         int p = 0;
-        if (lane < a.K) {
+        if (lane < a.K && (!ONE || warp == 0)) {
             const int i = m * a.K + lane;
             const int e = dispatch_expert(a, i, false);
             p = static_cast<int>(s_first[e] & 0xFFFFu) * TILE_M + atomicAdd(&s_next[e], 1);
             a.pos[i] = p;
-            a.row_token[p] = m;
             a.row_weight[p] = __ldg(a.topk_w + i);
+            if constexpr (ONE) s_pos[lane] = p;
         }
-        for (int g0 = 0; g0 < n_groups; g0 += U) {
-            if (g0 != 0 || m != m0 + warp) fetch(m, g0);
+        if constexpr (ONE) {
+            __syncthreads();             // a block has one token, so this runs once
+            if (lane < a.K) p = s_pos[lane];
+        }
+        for (int g0 = g_first; g0 < n_groups; g0 += U * STEP) {
+            if (g0 != g_first || m != m_first) fetch(m, g0);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (g0 + u >= n_groups) break;
@@ -269,15 +274,17 @@ __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a)
 }
 
 static bool dispatch_small(int M, int K) { return static_cast<long long>(M) * K <= DISPATCH_SMALL_PAIRS; }
-// Tokens of a block: one a warp, more where there are more than four blocks an SM (a block has a set-up of its own).
-static int dispatch_chunk(int M) {
+// Tokens of a block: one up to four blocks an SM, else one a warp, more where that makes more than four blocks an SM (a block
+// has a set-up of its own).
+static int dispatch_chunk(int M, int K) {
     const int want = (M + 4 * sm_count() - 1) / (4 * sm_count());
+    if (want <= 1 && dispatch_small(M, K)) return 1;
     return (want + 7) / 8 * 8;
 }
 
 // Parts of the workspace of a whole forward pass, each on a 256-byte boundary.
 struct Fp8Workspace {
-    size_t tile_expert, pair_info, sched, row_token, row_weight, pos, dispatch, dispatch_bytes, x_scale, h, h_scale, rows,
+    size_t tile_expert, pair_info, sched, tile_rows, row_weight, pos, dispatch, dispatch_bytes, x_scale, h, h_scale, rows,
         bytes;
     long long tiles;
 };
@@ -296,7 +303,7 @@ static Fp8Workspace fp8_workspace(int M, int N, int K, int D, int H) {
     w.tile_expert = take(tiles * 4);
     w.pair_info = take(tiles * 4);
     w.sched = take(SCHED_WORDS * 4);
-    w.row_token = take(rows * 4);
+    w.tile_rows = take(tiles * 4);
     w.row_weight = take(rows * 4);
     w.pos = take(msum * 4);
     w.dispatch_bytes = momoe_fp8_dispatch_workspace_bytes(M, N, K);
@@ -333,18 +340,18 @@ MOMOE_API int momoe_fp8_quantize_weights(const void* W, int32_t type, int32_t N,
 
 MOMOE_API size_t momoe_fp8_dispatch_workspace_bytes(int32_t M, int32_t N, int32_t K) {
     if (M <= 0 || N <= 0 || K <= 0 || dispatch_small(M, K)) return 0;
-    const int c = dispatch_chunk(M);
+    const int c = dispatch_chunk(M, K);
     return (1 + static_cast<size_t>((M + c - 1) / c)) * N * 4;
 }
 
 MOMOE_API int momoe_fp8_dispatch_rows(const void* x, const uint8_t* x_scale, const int32_t* topk_idx_MK,
                                       const float* topk_w_MK, int32_t M, int32_t N, int32_t K, int32_t D,
                                       int64_t* sizes_N, int32_t* tile_expert, int32_t* pair_info, int32_t* sched,
-                                      int32_t* row_token, float* row_weight, int32_t* pos_MK, int64_t rows_capacity,
+                                      int32_t* tile_rows, float* row_weight, int32_t* pos_MK, int64_t rows_capacity,
                                       void* workspace, size_t workspace_bytes, uint8_t* dst_sorted, uint8_t* dst_scale,
                                       int32_t* status, momoe_stream_t stream) {
     if (x == nullptr || topk_idx_MK == nullptr || topk_w_MK == nullptr || sizes_N == nullptr || tile_expert == nullptr ||
-        pair_info == nullptr || sched == nullptr || row_token == nullptr || row_weight == nullptr || pos_MK == nullptr ||
+        pair_info == nullptr || sched == nullptr || tile_rows == nullptr || row_weight == nullptr || pos_MK == nullptr ||
         dst_sorted == nullptr || dst_scale == nullptr || status == nullptr)
         return MOMOE_ERR_ARG;
     if (M <= 0 || N <= 0 || K <= 0 || K > N || D <= 0) return MOMOE_ERR_ARG;
@@ -362,23 +369,26 @@ MOMOE_API int momoe_fp8_dispatch_rows(const void* x, const uint8_t* x_scale, con
     DispatchArgs a;
     a.x = x; a.x_scale = x_scale; a.topk_idx = topk_idx_MK; a.topk_w = topk_w_MK;
     a.M = M; a.N = N; a.K = K; a.D = D;
-    a.chunk = dispatch_chunk(M);
+    a.chunk = dispatch_chunk(M, K);
     a.total = static_cast<int*>(workspace);
     a.chunk_base = need > 0 ? a.total + N : nullptr;
     a.sizes = reinterpret_cast<long long*>(sizes_N);
     a.tile_expert = tile_expert; a.pair_info = pair_info; a.sched = sched;
-    a.row_token = row_token; a.row_weight = row_weight; a.pos = pos_MK;
+    a.tile_rows = tile_rows; a.row_weight = row_weight; a.pos = pos_MK;
     a.dst = dst_sorted; a.dst_scale = dst_scale; a.status = status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int grid = (M + a.chunk - 1) / a.chunk;
-    if (need == 0) {
-        if (x_scale != nullptr) fp8_dispatch_kernel<true, true><<<grid, 256, 0, st>>>(a);
-        else fp8_dispatch_kernel<false, true><<<grid, 256, 0, st>>>(a);
+    if (a.chunk == 1) {
+        if (x_scale != nullptr) fp8_dispatch_kernel<true, true, true><<<grid, 256, 0, st>>>(a);
+        else fp8_dispatch_kernel<false, true, true><<<grid, 256, 0, st>>>(a);
+    } else if (need == 0) {
+        if (x_scale != nullptr) fp8_dispatch_kernel<true, true, false><<<grid, 256, 0, st>>>(a);
+        else fp8_dispatch_kernel<false, true, false><<<grid, 256, 0, st>>>(a);
     } else {
         if (cudaMemsetAsync(a.total, 0, static_cast<size_t>(N) * 4, st) != cudaSuccess) return MOMOE_ERR_CUDA;
         fp8_count_kernel<<<grid, 256, 0, st>>>(a);
-        if (x_scale != nullptr) fp8_dispatch_kernel<true, false><<<grid, 256, 0, st>>>(a);
-        else fp8_dispatch_kernel<false, false><<<grid, 256, 0, st>>>(a);
+        if (x_scale != nullptr) fp8_dispatch_kernel<true, false, false><<<grid, 256, 0, st>>>(a);
+        else fp8_dispatch_kernel<false, false, false><<<grid, 256, 0, st>>>(a);
     }
     return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
@@ -414,22 +424,22 @@ MOMOE_API int momoe_fp8_experts_forward(const void* x_MD, const uint8_t* x_scale
     plan.sched = i32(l.sched);
     plan.tile_expert = i32(l.tile_expert);
     plan.pad_off = nullptr;
-    plan.row_token = i32(l.row_token);
+    plan.row_token = nullptr;
     plan.row_weight = reinterpret_cast<float*>(ws + l.row_weight);
     plan.pos_MK = i32(l.pos);
     plan.status = status;
     plan.pair_info = i32(l.pair_info);
     int rc = momoe_fp8_dispatch_rows(x_MD, x_scale, topk_idx_MK, topk_w_MK, M, N, K, D, sizes_N, i32(l.tile_expert),
-                                     i32(l.pair_info), i32(l.sched), i32(l.row_token),
+                                     i32(l.pair_info), i32(l.sched), i32(l.tile_rows),
                                      reinterpret_cast<float*>(ws + l.row_weight), i32(l.pos), plan.rows_capacity,
                                      ws + l.dispatch, l.dispatch_bytes, u8(l.rows), u8(l.x_scale), status, stream);
     if (rc != MOMOE_OK) return rc;
     // with few rows an expert, the kernels that stream the weights
     const bool decode = static_cast<int64_t>(M) * K <= static_cast<int64_t>(stream_max_avg_rows) * N;
-    rc = decode ? momoe_fp8_up_swiglu_decode(&plan, u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream)
+    rc = decode ? momoe_fp8_up_swiglu_decode(&plan, i32(l.tile_rows), u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream)
                 : momoe_fp8_up_swiglu(&plan, u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream);
     if (rc != MOMOE_OK) return rc;
-    rc = decode ? momoe_fp8_down_scale_decode(&plan, u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, stream)
+    rc = decode ? momoe_fp8_down_scale_decode(&plan, i32(l.tile_rows), u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, stream)
                 : momoe_fp8_down_scale(&plan, u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, stream);
     if (rc != MOMOE_OK) return rc;
     // launched early beside the tile kernel its blocks wait there for long and slow it down (1124 against 1098 us at 16384

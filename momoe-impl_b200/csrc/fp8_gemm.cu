@@ -471,7 +471,7 @@ static int f8_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUten
 
 int fp8_check_plan(const momoe_plan_t* p) {
     if (p == nullptr || p->sched == nullptr || p->tile_expert == nullptr || p->pair_info == nullptr ||
-        p->row_weight == nullptr || p->row_token == nullptr || p->pos_MK == nullptr || p->status == nullptr)
+        p->row_weight == nullptr || p->status == nullptr)
         return MOMOE_ERR_ARG;
     if (p->M <= 0 || p->N <= 0 || p->K <= 0 || p->D <= 0 || p->H <= 0 || p->rows_capacity <= 0) return MOMOE_ERR_ARG;
     if (p->D % 16 != 0 || p->H % 16 != 0) return MOMOE_ERR_UNSUPPORTED;   // TMA row pitch of 8-bit rows: 16 bytes

@@ -149,7 +149,7 @@ class Stages:
         i32 = lambda n: torch.full((n,), 77, dtype=torch.int32, device="cuda")
         u8 = lambda n: torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda")
         self.sizes = torch.empty(N, dtype=torch.int64, device="cuda")
-        self.tile_expert, self.pair_info, self.sched, self.row_token, self.pos = i32(tiles), i32(tiles), i32(8), i32(rows), i32(M * K)
+        self.tile_expert, self.pair_info, self.sched, self.tile_rows, self.pos = i32(tiles), i32(tiles), i32(8), i32(tiles), i32(M * K)
         self.row_weight = torch.full((rows,), float("nan"), device="cuda")
         self.xs, self.xsc = u8(rows * D), u8(tiles * -(-D // 512) * 512)
         self.hs, self.hsc = u8(rows * H), u8(tiles * -(-H // 512) * 512)
@@ -157,7 +157,7 @@ class Stages:
         self.M, self.N, self.K, self.D, self.H, self.rows, self.tiles = M, N, K, D, H, rows, tiles
         p = lambda t: t.data_ptr()
         self.c = _lib.Plan(M=M, N=N, K=K, D=D, H=H, reserved=0, rows_capacity=rows, sched=p(self.sched),
-                           tile_expert=p(self.tile_expert), pad_off=0, row_token=p(self.row_token),
+                           tile_expert=p(self.tile_expert), pad_off=0, row_token=0,
                            row_weight=p(self.row_weight), pos_MK=p(self.pos), status=p(self.status), pair_info=p(self.pair_info))
 
     def dispatch(self, x, scale, idx, w):
@@ -166,14 +166,16 @@ class Stages:
         p = self.ptr
         self.check(self.lib.momoe_fp8_dispatch_rows(p(x), p(scale), p(idx), p(w), self.M, self.N, self.K, self.D,
                                                     p(self.sizes), p(self.tile_expert), p(self.pair_info), p(self.sched),
-                                                    p(self.row_token), p(self.row_weight), p(self.pos), self.rows, p(ws),
+                                                    p(self.tile_rows), p(self.row_weight), p(self.pos), self.rows, p(ws),
                                                     nbytes, p(self.xs), p(self.xsc), p(self.status), self.st), "dispatch")
 
     def gemms(self, e, stream):
         import ctypes
         ref, p, L = ctypes.byref(self.c), self.ptr, self.lib
-        up, down = ((L.momoe_fp8_up_swiglu_decode, L.momoe_fp8_down_scale_decode) if stream
-                    else (L.momoe_fp8_up_swiglu, L.momoe_fp8_down_scale))
+        up, down = L.momoe_fp8_up_swiglu, L.momoe_fp8_down_scale
+        if stream:
+            up = lambda plan, *rest: L.momoe_fp8_up_swiglu_decode(plan, p(self.tile_rows), *rest)
+            down = lambda plan, *rest: L.momoe_fp8_down_scale_decode(plan, p(self.tile_rows), *rest)
         self.check(up(ref, p(self.xs), p(self.xsc), p(e.W1_N2HD), p(e.S1), p(self.hs), p(self.hsc), self.st), "up")
         self.check(down(ref, p(self.hs), p(self.hsc), p(e.W2_NDH), p(e.S2), p(self.ys), self.st), "down")
 
@@ -197,14 +199,13 @@ def check_tables(s, idx, w):
         pairs += [(t0 + j) * 2 + (1 if j + 1 < n else 0) for j in range(0, n, 2)]
         t0 += n
     assert s.pair_info[:len(pairs)].tolist() == pairs
-    tok, wt, pos = s.row_token[:T * 128], s.row_weight[:T * 128], s.pos.long()
-    assert len(pos.unique()) == s.M * s.K and int((tok >= 0).sum()) == s.M * s.K
-    assert torch.equal(tok[pos], torch.arange(s.M, device="cuda").int().repeat_interleave(s.K))
-    assert torch.equal(wt[pos], w.flatten()) and not wt[tok < 0].any()
+    rows = torch.cat([torch.tensor([min(128, n - j) for j in range(0, n, 128)], dtype=torch.int32) for n in sizes.tolist()])
+    assert torch.equal(s.tile_rows[:T].cpu(), rows)
+    pos = s.pos.long()
+    assert len(pos.unique()) == s.M * s.K
     assert torch.equal(s.tile_expert[pos // 128], idx.flatten())
-    first = torch.repeat_interleave((nt.cumsum(0) - nt) * 128, nt * 128)
-    at = torch.arange(T * 128, device="cuda") - first           # place inside the expert: real rows first
-    assert torch.equal(tok >= 0, at < torch.repeat_interleave(sizes, nt * 128))
+    assert (pos % 128 < s.tile_rows[pos // 128]).all()           # real rows come first in a tile
+    assert torch.equal(s.row_weight[pos], w.flatten())
 
 
 @pytest.mark.parametrize("stream", [False, True])

@@ -80,11 +80,13 @@ def test_fp8_arguments(lib):
     assert dispatch(M=8 << 20, rows=1 << 40) == -4                               # more tiles than a table entry counts
     assert L.momoe_fp8_dispatch_workspace_bytes(4, 8, 2) == 0
     assert L.momoe_fp8_dispatch_workspace_bytes(20000, 8, 2) > 8 * 4
-    for f in (L.momoe_fp8_up_swiglu, L.momoe_fp8_up_swiglu_decode):
+    stream = lambda f: lambda plan, *rest: f(plan, ONE, *rest)
+    for f in (L.momoe_fp8_up_swiglu, stream(L.momoe_fp8_up_swiglu_decode)):
         assert f(p, ONE, ONE, ONE, None, ONE, ONE, None) == -1 and f(p, ODD, ONE, ONE, ONE, ONE, ONE, None) == -1
         assert f(None, ONE, ONE, ONE, ONE, ONE, ONE, None) == -1
-    for f in (L.momoe_fp8_down_scale, L.momoe_fp8_down_scale_decode):
+    for f in (L.momoe_fp8_down_scale, stream(L.momoe_fp8_down_scale_decode)):
         assert f(p, ONE, ONE, ONE, None, ONE, None) == -1 and f(p, ONE, ONE, ONE, ONE, None, None) == -1
+    assert L.momoe_fp8_up_swiglu_decode(p, None, ONE, ONE, ONE, ONE, ONE, ONE, None) == -1
     def whole(M=4, N=8, K=2, D=64, H=32, x=ONE, ws=ONE, n=None):
         n = L.momoe_fp8_experts_workspace_bytes(M, N, K, D, H) if n is None else n
         return L.momoe_fp8_experts_forward(x, None, ONE, ONE, M, N, K, D, H, ONE, ONE, ONE, ONE, 16, ONE, ONE, ws, n, ONE,
