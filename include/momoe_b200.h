@@ -303,12 +303,19 @@ int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const int32_t* tile_row
                                const uint8_t* x_scale, const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
                                momoe_stream_t stream);
 
-/* Down GEMM on 8-bit operands: y_sorted[r, :] = bf16(w[r] * (h[r, :] W2[e]^T)).  W2 [N, D, H],
- * S2 [N, ceil(D / 128), ceil(H / 128)]; y_sorted 32-byte aligned. */
+/* Down GEMM on 8-bit operands: w[r] * (h[r, :] W2[e]^T) as y_sorted fp16 [rows, D] and y_scale fp32
+ * [rows, ceil(D / 256)], a power of two for each (row, 256 columns); the value is their product.  W2 [N, D, H],
+ * S2 [N, ceil(D / 128), ceil(H / 128)]. */
 int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
-                         const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, momoe_stream_t stream);
+                         const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, float* y_scale,
+                         momoe_stream_t stream);
 int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* h_sorted,
-                                const uint8_t* h_scale, const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, momoe_stream_t stream);
+                                const uint8_t* h_scale, const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted,
+                                float* y_scale, momoe_stream_t stream);
+
+/* y_MD[m, :] = bf16(sum over k of the value of row pos_MK[m, k]): 32-bit sums in ascending k, one rounding. */
+int momoe_fp8_combine_rows(const void* y_sorted, const float* y_scale, const int32_t* pos_MK, int32_t M, int32_t K,
+                           int32_t D, void* y_MD, momoe_stream_t stream);
 
 /* The whole forward pass of 8-bit experts from a compact routing: dispatch, up, down, combine, out of one workspace
  * (256-byte aligned).  x as for momoe_fp8_dispatch_rows; y_MD bf16 [M, D]; sizes_N int64 [N].  Calls with at

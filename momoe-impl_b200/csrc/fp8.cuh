@@ -42,6 +42,35 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
 }
 __device__ __forceinline__ uint8_t fp8_one(float a) { return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3); }
 
+// Result rows of the down GEMM on their way to the weighted sum: fp16 with one power of two for each (row, 256 columns).
+// bf16 rows would add a second rounding as large as that of the result itself; fp16 rows have the same size and one 16 times
+// smaller, and the power of two keeps them in range whatever the values: it comes from a bound on the row's products, so it
+// is known before the accumulators are.  With 448 2^a the largest value of a block, |sum| <= 2^max(a_h + a_W) 448^2 H and
+// 448^2 * 128 < 2^25.  The bound is 2^10 to 2^13 above typical values; fp16 has 28 binades of full precision below it.
+constexpr int FP8_YBLOCK = 256;
+
+// Exponent e of one row (a lane each): stored value = value * 2^e, |value * 2^e| <= 2^15.  hs: the word of the row's first
+// scales, the next group 512 bytes on; ws: scale bytes of the first of the two 128-column blocks, the second nkb bytes on.
+__device__ __forceinline__ int fp8_row_exponent(const uint8_t* hs, const uint8_t* ws, bool two, int nkb, float w) {
+    const int lane = threadIdx.x & 31;
+    int top = 0;
+    for (int g = 0; g * FP8_GROUP < nkb; ++g) {
+        const uint32_t hw = __ldcg(reinterpret_cast<const uint32_t*>(hs + static_cast<size_t>(g) * FP8_ATOM));
+        const int kb = g * FP8_GROUP + (lane & 3);
+        const bool second = (lane & 4) != 0;
+        int b = kb < nkb && (two || !second) ? static_cast<int>(__ldg(ws + (second ? nkb : 0) + kb)) : 0;
+        b = max(b, __shfl_xor_sync(0xffffffffu, b, 4));
+#pragma unroll
+        for (int j = 0; j < FP8_GROUP; ++j) {
+            const int wb = __shfl_sync(0xffffffffu, b, j);
+            if (g * FP8_GROUP + j < nkb) top = max(top, static_cast<int>((hw >> (8 * j)) & 255u) + wb);
+        }
+    }
+    const int bound = top - 254 + 25 + (32 - __clz(nkb - 1)) + static_cast<int>((__float_as_uint(w) >> 23) & 255u) - 126;
+    return min(max(15 - bound, -126), 126);
+}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }   // |e| <= 126
+
 // Eight consecutive values of a row as they lie in memory, read past L1 (each is used once), and in 32 bits.
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
     uint4 q;

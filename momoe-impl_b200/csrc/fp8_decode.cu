@@ -58,7 +58,8 @@ struct Fp8DecArgs {
     const uint8_t* w_scale;
     uint8_t* h;
     uint8_t* h_scale;
-    __nv_bfloat16* y;
+    __half* y;
+    float* y_scale;          // down: [rows, n_cblk]
 };
 
 struct D8Item {
@@ -99,7 +100,16 @@ __device__ __forceinline__ bool d8_read_out(const Fp8DecArgs& g, D8Epi& c, const
                                             bool last) {
     const int lane = threadIdx.x & 31, q = (threadIdx.x >> 5) & 3;
     float wgt = 0.0f;
-    if constexpr (!UP) wgt = __ldcg(g.row_weight + row0 + lane);   // lane t holds the weight of token t
+    if constexpr (!UP) {
+        // lane t holds the weight and the power of two of token t
+        wgt = __ldcg(g.row_weight + row0 + lane);
+        const int w_blocks = (g.out_cols + 127) / 128, n0 = w.cb * 2;
+        const int e = fp8_row_exponent(g.x_scale + fp8_atom_offset(row0 + lane, 0, (g.nkb + 3) >> 2),
+                                       g.w_scale + (static_cast<size_t>(w.e) * w_blocks + n0) * g.nkb, n0 + 1 < w_blocks,
+                                       g.nkb, wgt);
+        if (q == 0 && lane < T && (SPLIT == 1 || c.rank == 0)) g.y_scale[(row0 + lane) * g.n_cblk + w.cb] = pow2f(-e);
+        wgt *= pow2f(e);
+    }
     uint32_t r[T], rb[T];
     d8_tmem_ld<T>(taddr, r);
     d8_tmem_ld<T>(taddr + D8_NT, rb);
@@ -172,12 +182,12 @@ __device__ __forceinline__ bool d8_read_out(const Fp8DecArgs& g, D8Epi& c, const
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int col = w.cb * 256 + i * 128 + q * 32 + lane;
-            __nv_bfloat16* dst = g.y + row0 * g.out_cols + col;
+            __half* dst = g.y + row0 * g.out_cols + col;
 #pragma unroll
             for (int t = 0; t < T; ++t) {
                 const float s = __shfl_sync(0xffffffffu, wgt, t);
                 if (col < g.out_cols)
-                    dst[static_cast<size_t>(t) * g.out_cols] = __float2bfloat16_rn(__uint_as_float(i == 0 ? r[t] : rb[t]) * s);
+                    dst[static_cast<size_t>(t) * g.out_cols] = __float2half_rn(__uint_as_float(i == 0 ? r[t] : rb[t]) * s);
             }
         }
     }
@@ -473,10 +483,11 @@ MOMOE_API int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const int32_t
 
 MOMOE_API int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* h_sorted,
                                           const uint8_t* h_scale, const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted,
-                                          momoe_stream_t stream) {
+                                          float* y_scale, momoe_stream_t stream) {
     int rc = fp8_check_plan(plan);
     if (rc != MOMOE_OK) return rc;
-    if (tile_rows == nullptr || !d8_aligned(h_sorted) || !d8_aligned(h_scale) || !d8_aligned(W2_NDH) || S2 == nullptr || !d8_aligned(y_sorted))
+    if (tile_rows == nullptr || !d8_aligned(h_sorted) || !d8_aligned(h_scale) || !d8_aligned(W2_NDH) || S2 == nullptr || !d8_aligned(y_sorted) ||
+        y_scale == nullptr)
         return MOMOE_ERR_ARG;
     const int D = plan->D, H = plan->H;
     CUtensorMap tmW, tmX;
@@ -489,7 +500,8 @@ MOMOE_API int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const int32_
     g.out_cols = D;
     g.x_scale = h_scale;
     g.w_scale = S2;
-    g.y = static_cast<__nv_bfloat16*>(y_sorted);
+    g.y = static_cast<__half*>(y_sorted);
+    g.y_scale = y_scale;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return d8_split(plan, g) ? d8_launch<false, 2>(tmW, tmX, g, st) : d8_launch<false, 1>(tmW, tmX, g, st);
 }

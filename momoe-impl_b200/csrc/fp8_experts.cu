@@ -273,6 +273,80 @@ __global__ void __launch_bounds__(256) fp8_dispatch_kernel(const DispatchArgs a)
     }
 }
 
+// y[m, :] = bf16(sum over k of rows[pos[m, k], :] * scale), 32-bit sums in the order of k, one rounding.  A thread has 8 columns;
+// bound by HBM: M (K + 1) D 2 bytes.
+template <int KT>
+__global__ void __launch_bounds__(256) fp8_combine_kernel(const uint4* __restrict__ rows, const float* __restrict__ scale,
+                                                          const int* __restrict__ pos, int M, int K, int vec_per_row,
+                                                          int n_scale, uint4* __restrict__ dst) {
+    grid_wait();
+    const long long total = static_cast<long long>(M) * vec_per_row;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const int m = static_cast<int>(i / vec_per_row);
+        const int c = static_cast<int>(i - static_cast<long long>(m) * vec_per_row);
+        const int* p = pos + static_cast<size_t>(m) * (KT > 0 ? KT : K);
+        float a[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        auto add = [&](const uint4& q, float s) {
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                a[2 * j] = fmaf(f.x, s, a[2 * j]);
+                a[2 * j + 1] = fmaf(f.y, s, a[2 * j + 1]);
+            }
+        };
+        if constexpr (KT > 0) {
+            uint4 q[KT];
+            float s[KT];
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                const size_t row = static_cast<size_t>(__ldcg(p + k));
+                q[k] = __ldcg(rows + row * vec_per_row + c);
+                s[k] = __ldcg(scale + row * n_scale + (c >> 5));
+            }
+#pragma unroll
+            for (int k = 0; k < KT; ++k) add(q[k], s[k]);
+        } else {
+            for (int k = 0; k < K; ++k) {
+                const size_t row = static_cast<size_t>(__ldcg(p + k));
+                add(__ldcg(rows + row * vec_per_row + c), __ldcg(scale + row * n_scale + (c >> 5)));
+            }
+        }
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a[2 * j], a[2 * j + 1]);
+            o[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        dst[i] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+static int fp8_combine(const void* rows, const float* scale, const int32_t* pos, int M, int K, int D, void* y,
+                       cudaStream_t st, bool dependent) {
+    const int vec = D / 8, n_scale = (D + FP8_YBLOCK - 1) / FP8_YBLOCK;
+    const long long want = (static_cast<long long>(M) * vec + 255) / 256, cap = sm_count() * 16;
+    const int grid = static_cast<int>(want < cap ? want : cap);
+    const uint4* r = static_cast<const uint4*>(rows);
+    uint4* d = static_cast<uint4*>(y);
+#define COMBINE(KT)                                                                                                    \
+    if (dependent)                                                                                                     \
+        return launch_dependent(fp8_combine_kernel<KT>, grid, 256, 0, st, 1, r, scale, pos, M, K, vec, n_scale, d) ==  \
+               cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;                                                                \
+    fp8_combine_kernel<KT><<<grid, 256, 0, st>>>(r, scale, pos, M, K, vec, n_scale, d);                                \
+    break
+    switch (K) {
+        case 1: COMBINE(1);
+        case 2: COMBINE(2);
+        case 4: COMBINE(4);
+        case 6: COMBINE(6);
+        case 8: COMBINE(8);
+        default: COMBINE(0);
+    }
+#undef COMBINE
+    return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
+}
+
 static bool dispatch_small(int M, int K) { return static_cast<long long>(M) * K <= DISPATCH_SMALL_PAIRS; }
 // Tokens of a block: one up to four blocks an SM, else one a warp, more where that makes more than four blocks an SM (a block
 // has a set-up of its own).
@@ -285,7 +359,7 @@ static int dispatch_chunk(int M, int K) {
 // Parts of the workspace of a whole forward pass, each on a 256-byte boundary.
 struct Fp8Workspace {
     size_t tile_expert, pair_info, sched, tile_rows, row_weight, pos, dispatch, dispatch_bytes, x_scale, h, h_scale, rows,
-        bytes;
+        y_scale, bytes;
     long long tiles;
 };
 static Fp8Workspace fp8_workspace(int M, int N, int K, int D, int H) {
@@ -312,6 +386,7 @@ static Fp8Workspace fp8_workspace(int M, int N, int K, int D, int H) {
     w.h = take(rows * H);
     w.h_scale = take(tiles * ((H + 511) / 512) * FP8_ATOM);
     w.rows = take(rows * D * 2);     // 8-bit input rows, later the 16-bit result rows
+    w.y_scale = take(rows * ((D + FP8_YBLOCK - 1) / FP8_YBLOCK) * 4);
     w.bytes = at;
     return w;
 }
@@ -393,6 +468,15 @@ MOMOE_API int momoe_fp8_dispatch_rows(const void* x, const uint8_t* x_scale, con
     return cudaGetLastError() == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
 
+MOMOE_API int momoe_fp8_combine_rows(const void* y_sorted, const float* y_scale, const int32_t* pos_MK, int32_t M, int32_t K,
+                                     int32_t D, void* y_MD, momoe_stream_t stream) {
+    if (y_sorted == nullptr || y_scale == nullptr || pos_MK == nullptr || y_MD == nullptr || M <= 0 || K <= 0 || D <= 0)
+        return MOMOE_ERR_ARG;
+    if (D % 8 != 0) return MOMOE_ERR_UNSUPPORTED;
+    if (((reinterpret_cast<uintptr_t>(y_sorted) | reinterpret_cast<uintptr_t>(y_MD)) & 15) != 0) return MOMOE_ERR_ARG;
+    return fp8_combine(y_sorted, y_scale, pos_MK, M, K, D, y_MD, static_cast<cudaStream_t>(stream), false);
+}
+
 MOMOE_API size_t momoe_fp8_experts_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t D, int32_t H) {
     if (M <= 0 || N <= 0 || K <= 0 || D <= 0 || H <= 0) return 0;
     return fp8_workspace(M, N, K, D, H).bytes;
@@ -439,10 +523,11 @@ MOMOE_API int momoe_fp8_experts_forward(const void* x_MD, const uint8_t* x_scale
     rc = decode ? momoe_fp8_up_swiglu_decode(&plan, i32(l.tile_rows), u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream)
                 : momoe_fp8_up_swiglu(&plan, u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream);
     if (rc != MOMOE_OK) return rc;
-    rc = decode ? momoe_fp8_down_scale_decode(&plan, i32(l.tile_rows), u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, stream)
-                : momoe_fp8_down_scale(&plan, u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, stream);
+    float* y_scale = reinterpret_cast<float*>(ws + l.y_scale);
+    rc = decode ? momoe_fp8_down_scale_decode(&plan, i32(l.tile_rows), u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, y_scale, stream)
+                : momoe_fp8_down_scale(&plan, u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, y_scale, stream);
     if (rc != MOMOE_OK) return rc;
     // launched early beside the tile kernel its blocks wait there for long and slow it down (1124 against 1098 us at 16384
     // tokens, D2048 H1024, top-8 of 128); behind the streaming kernel it saves a launch gap (30.7 against 32.5 us, 1 token)
-    return combine_rows(&plan, ws + l.rows, D, y_MD, stream, decode);
+    return fp8_combine(ws + l.rows, y_scale, plan.pos_MK, M, K, D, y_MD, static_cast<cudaStream_t>(stream), decode);
 }

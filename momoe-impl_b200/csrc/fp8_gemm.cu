@@ -1,7 +1,7 @@
 // The experts' two forward GEMMs on 8-bit rows and weights (e4m3, a power of two for each block of 128), sm_100a.
 //
 //   up    a = x W1[e][:H]^T, b = x W1[e][H:]^T, h = b sigmoid(b) a in 32 bits, h -> 8-bit rows (128 columns a scale)
-//   down  y[r, :] = bf16(row_weight[r] * (h W2[e]^T))
+//   down  y[r, :] = row_weight[r] * (h W2[e]^T), as fp16 with a power of two for each (row, 256 columns) (fp8.cuh)
 //
 // Weights are K-major ([N, 2H, D] and [N, D, H]) with one scale for each 128 x 128 block.  All scales are powers of two,
 // so the tensor core applies them (kind::mxf8f6f4, block-scaled): accumulation is fp32 over the whole k axis and there is
@@ -63,10 +63,11 @@ struct Fp8Args {
     int b_blocks;               // down: ceil(D / 128)
     uint8_t* h_scale;           // up: scales of h, blocks of 512 bytes
     const float* row_weight;    // down
+    float* y_scale;             // down: [rows, n_nblk]
 };
 
-__device__ __forceinline__ uint32_t f8_pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+__device__ __forceinline__ uint32_t f8_pack_f16(float lo, float hi) {
+    const __half2 p = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&p);
 }
 __device__ __forceinline__ float f8_swiglu(float a, float b) { return b * __fdividef(1.0f, 1.0f + __expf(-b)) * a; }
@@ -298,7 +299,17 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             };
             float wgt = 0.0f;
             const size_t grow = static_cast<size_t>(w.tile) * TILE_M + row;
-            if constexpr (!UP) wgt = w.valid ? __ldcg(g.row_weight + grow) : 0.0f;
+            if constexpr (!UP) {
+                if (w.valid) {
+                    wgt = __ldcg(g.row_weight + grow);
+                    const int n0 = w.nb * 2;
+                    const int e = fp8_row_exponent(g.a_scale + fp8_atom_offset(grow, 0, n_groups),
+                                                   g.b_scale + (static_cast<size_t>(w.e) * g.b_blocks + n0) * g.nkb,
+                                                   n0 + 1 < g.b_blocks, g.nkb, wgt);
+                    if (half == 0) g.y_scale[grow * g.n_nblk + w.nb] = pow2f(-e);
+                    wgt *= pow2f(e);
+                }
+            }
             ok = mbar_wait(smem_u32(&bar_acc_full[ab]), (it >> 1) & 1u, abortp, g.status, DEV_TIMEOUT_EPILOGUE) &&
                  *abortp == 0;
             ok = __all_sync(0xffffffffu, ok);
@@ -398,8 +409,8 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                             uint32_t v[4];
 #pragma unroll
                             for (int u = 0; u < 4; ++u)
-                                v[u] = f8_pack_bf16(__uint_as_float(r[j * 8 + 2 * u]) * wgt,
-                                                    __uint_as_float(r[j * 8 + 2 * u + 1]) * wgt);
+                                v[u] = f8_pack_f16(__uint_as_float(r[j * 8 + 2 * u]) * wgt,
+                                                   __uint_as_float(r[j * 8 + 2 * u + 1]) * wgt);
                             st_shared_v4(base + ((j ^ x) << 4), v[0], v[1], v[2], v[3]);
                         }
                         fence_proxy_async_smem();
@@ -518,11 +529,12 @@ MOMOE_API int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const uint8_t* x_sor
 }
 
 MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
-                                   const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, momoe_stream_t stream) {
+                                   const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, float* y_scale,
+                                   momoe_stream_t stream) {
     int rc = fp8_check_plan(plan);
     if (rc != MOMOE_OK) return rc;
     if (!f8_aligned(h_sorted, 16) || !f8_aligned(h_scale, 16) || !f8_aligned(W2_NDH, 16) || S2 == nullptr ||
-        !f8_aligned(y_sorted, 32))
+        !f8_aligned(y_sorted, 16) || y_scale == nullptr)
         return MOMOE_ERR_ARG;
     const int D = plan->D, H = plan->H;
     CUtensorMap tmA, tmB, tmO;
@@ -542,5 +554,6 @@ MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_so
     g.b_scale = S2;
     g.b_blocks = f8_cdiv(D, 128);
     g.row_weight = plan->row_weight;
+    g.y_scale = y_scale;
     return f8_launch<false>(tmA, tmB, tmO, g, static_cast<cudaStream_t>(stream));
 }

@@ -84,9 +84,3 @@ int encode_tmap(CUtensorMap* m, const void* base, int rank, const uint64_t* dims
                 const uint32_t* box, int swizzle);
 
 }  // namespace momoe
-
-struct momoe_plan;
-namespace momoe {
-// momoe_combine_rows; `dependent`: launched as a programmatic dependent of the kernel before it in the stream.
-int combine_rows(const momoe_plan* plan, const void* src_sorted, int32_t cols, void* dst, void* stream, bool dependent);
-}  // namespace momoe

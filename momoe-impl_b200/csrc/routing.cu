@@ -5,7 +5,6 @@
 #include <mutex>
 
 #include "internal.h"
-#include "ptx.cuh"
 #include "../../include/momoe_b200.h"
 
 namespace momoe {
@@ -489,7 +488,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 template <int KT>
 __global__ void combine_rows_kernel(const uint4* __restrict__ src, const int* __restrict__ pos, int M, int K,
                                     int vec_per_row, uint4* __restrict__ dst) {
-    grid_wait();
     const long long total = static_cast<long long>(M) * vec_per_row;
     for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
          i += static_cast<long long>(gridDim.x) * blockDim.x) {
@@ -743,8 +741,8 @@ extern "C" __attribute__((visibility("default"))) int momoe_gather_rows(const mo
     return LAUNCH_OK();
 }
 
-int momoe::combine_rows(const momoe_plan* plan, const void* src_sorted, int32_t cols, void* dst, void* stream,
-                        bool dependent) {
+extern "C" __attribute__((visibility("default"))) int momoe_combine_rows(const momoe_plan_t* plan, const void* src_sorted, int32_t cols, void* dst,
+                                  momoe_stream_t stream) {
     if (plan == nullptr || src_sorted == nullptr || dst == nullptr || plan->pos_MK == nullptr) return MOMOE_ERR_ARG;
     if (cols <= 0 || cols % 8 != 0) return MOMOE_ERR_UNSUPPORTED;
     if (((reinterpret_cast<uintptr_t>(src_sorted) | reinterpret_cast<uintptr_t>(dst)) & 15) != 0) return MOMOE_ERR_ARG;
@@ -756,26 +754,14 @@ int momoe::combine_rows(const momoe_plan* plan, const void* src_sorted, int32_t 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint4* s = static_cast<const uint4*>(src_sorted);
     uint4* d = static_cast<uint4*>(dst);
-#define COMBINE(KT)                                                                                                  \
-    if (dependent)                                                                                                   \
-        return launch_dependent(combine_rows_kernel<KT>, blocks, 256, 0, st, 1, s, plan->pos_MK, plan->M, plan->K, vec, \
-                                d) == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;                                       \
-    combine_rows_kernel<KT><<<blocks, 256, 0, st>>>(s, plan->pos_MK, plan->M, plan->K, vec, d);                      \
-    break
     switch (plan->K) {
-        case 2: COMBINE(2);
-        case 4: COMBINE(4);
-        case 6: COMBINE(6);
-        case 8: COMBINE(8);
-        default: COMBINE(0);
+        case 2: combine_rows_kernel<2><<<blocks, 256, 0, st>>>(s, plan->pos_MK, plan->M, plan->K, vec, d); break;
+        case 4: combine_rows_kernel<4><<<blocks, 256, 0, st>>>(s, plan->pos_MK, plan->M, plan->K, vec, d); break;
+        case 6: combine_rows_kernel<6><<<blocks, 256, 0, st>>>(s, plan->pos_MK, plan->M, plan->K, vec, d); break;
+        case 8: combine_rows_kernel<8><<<blocks, 256, 0, st>>>(s, plan->pos_MK, plan->M, plan->K, vec, d); break;
+        default: combine_rows_kernel<0><<<blocks, 256, 0, st>>>(s, plan->pos_MK, plan->M, plan->K, vec, d); break;
     }
-#undef COMBINE
     return LAUNCH_OK();
-}
-
-extern "C" __attribute__((visibility("default"))) int momoe_combine_rows(const momoe_plan_t* plan, const void* src_sorted, int32_t cols, void* dst,
-                                  momoe_stream_t stream) {
-    return combine_rows(plan, src_sorted, cols, dst, stream, false);
 }
 
 extern "C" __attribute__((visibility("default"))) int momoe_scatter_gs(const momoe_plan_t* plan, const float* gs_part, int32_t n_part, float* G_s_NM,

@@ -153,7 +153,8 @@ class Stages:
         self.row_weight = torch.full((rows,), float("nan"), device="cuda")
         self.xs, self.xsc = u8(rows * D), u8(tiles * -(-D // 512) * 512)
         self.hs, self.hsc = u8(rows * H), u8(tiles * -(-H // 512) * 512)
-        self.ys = torch.full((rows, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+        self.ys = torch.full((rows, D), float("nan"), dtype=torch.float16, device="cuda")
+        self.yscale = torch.full((rows, -(-D // 256)), float("nan"), device="cuda")
         self.M, self.N, self.K, self.D, self.H, self.rows, self.tiles = M, N, K, D, H, rows, tiles
         p = lambda t: t.data_ptr()
         self.c = _lib.Plan(M=M, N=N, K=K, D=D, H=H, reserved=0, rows_capacity=rows, sched=p(self.sched),
@@ -177,12 +178,13 @@ class Stages:
             up = lambda plan, *rest: L.momoe_fp8_up_swiglu_decode(plan, p(self.tile_rows), *rest)
             down = lambda plan, *rest: L.momoe_fp8_down_scale_decode(plan, p(self.tile_rows), *rest)
         self.check(up(ref, p(self.xs), p(self.xsc), p(e.W1_N2HD), p(e.S1), p(self.hs), p(self.hsc), self.st), "up")
-        self.check(down(ref, p(self.hs), p(self.hsc), p(e.W2_NDH), p(e.S2), p(self.ys), self.st), "down")
+        self.check(down(ref, p(self.hs), p(self.hsc), p(e.W2_NDH), p(e.S2), p(self.ys), p(self.yscale), self.st), "down")
 
     def combine(self):
-        import ctypes
         y = torch.empty(self.M, self.D, dtype=torch.bfloat16, device="cuda")
-        self.check(self.lib.momoe_combine_rows(ctypes.byref(self.c), self.ptr(self.ys), self.D, self.ptr(y), self.st), "combine")
+        p = self.ptr
+        self.check(self.lib.momoe_fp8_combine_rows(p(self.ys), p(self.yscale), p(self.pos), self.M, self.K, self.D, p(y),
+                                                   self.st), "combine")
         return y
 
 
@@ -255,10 +257,19 @@ def test_stages_against_64_bits(fp8, monkeypatch, M, N, K, D, H, skew, stream):
         wt = w.flatten()[at, None].double()
         y = hv[at] @ W2v[n].T * wt
         dy = ACC * (hv[at].abs() @ W2v[n].abs().T) * wt
-        off = (s.ys[real[at]].double() - y).abs()
-        assert (off <= 2.0 ** -8 * (y.abs() + dy) + dy).all(), "y of expert %d" % n
-    # the whole call is these stages and the combine, bit for bit, from 16-bit and from 8-bit rows
+        # fp16 at a power of two: 2^-11 relative, and half a step of its smallest numbers, 2^-25 of that power
+        yv = s.ys.double() * s.yscale.double().repeat_interleave(256, 1)[:, :D]
+        off = (yv[real[at]] - y).abs()
+        fine = 2.0 ** -25 * s.yscale.double().repeat_interleave(256, 1)[:, :D][real[at]]
+        assert (off <= 2.0 ** -11 * (y.abs() + dy) + dy + fine).all(), "y of expert %d" % n
+        # the power of two is a bound, and not so far above the values that their precision suffers
+        assert torch.isfinite(s.ys[real[at]]).all()
+        assert (s.ys[real[at]].abs().amax(1) > 2.0 ** -8).all()
+    # the combine: one rounding of the sum of K values, each up to 2^-24 (fma) off
     want = s.combine()
+    vals = yv[real].view(M, K, D)
+    assert ((want.double() - vals.sum(1)).abs() <= 2.0 ** -8 * vals.sum(1).abs() + 2.0 ** -19 * vals.abs().sum(1)).all()
+    # the whole call is these stages, bit for bit, from 16-bit and from 8-bit rows
     monkeypatch.setattr(fp8, "STREAM_MAX_AVG_ROWS", 2 ** 20 if stream else 0)
     for rows_in in (x, fp8.Fp8Rows(q, scale.to(torch.float8_e8m0fnu)), fp8.quantize_rows(x)):
         y, sizes = fp8.experts_forward(rows_in, idx, w, e)
@@ -284,6 +295,38 @@ def test_bad_rows_stay_alone_and_strides(fp8):
     assert torch.equal(fp8.experts_forward(x.float(), idx, w, e)[0], want)
     zero, none = fp8.experts_forward(x[:0], idx[:0], w[:0], e)
     assert zero.shape == (0, D) and none.tolist() == [0] * N
+
+
+@pytest.mark.parametrize("stream", [False, True])
+def test_result_rows_keep_their_range(fp8, monkeypatch, stream):
+    """Values far beyond fp16 and far below it, and rows of unlike size, come out with one bfloat16 rounding: the
+    intermediate rows carry a power of two each."""
+    monkeypatch.setattr(fp8, "STREAM_MAX_AVG_ROWS", 2 ** 20 if stream else 0)
+    M, N, K, D, H = 60, 4, 2, 384, 160
+    idx, w = routing(M, N, K, 2, 0.0)
+    W1, W2 = weights(fp8, N, D, H, 4)
+    x = torch.randn(M, D, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    for exponent, columns in ((0, 0), (40, 0), (-50, 0), (0, 20)):
+        W = W2.clone()
+        W[:, :, :256] *= 2.0 ** columns                     # one block of columns much larger than the other
+        e = fp8.quantize_experts(W1, (W.float() * 2.0 ** exponent))
+        y, _ = fp8.experts_forward(x, idx, w * 3, e)
+        base = fp8.quantize_experts(W1, W2)
+        want, _ = fp8.experts_forward(x, idx, w * 3, base)
+        # powers of two pass through every stage unchanged
+        want = want.double() * 2.0 ** exponent
+        want[:, :256] *= 2.0 ** columns
+        assert torch.equal(y.double(), want)
+    y, _ = fp8.experts_forward(x, idx, -w * 2.0 ** 30, base)
+    assert torch.equal(y.double(), fp8.experts_forward(x, idx, w, base)[0].double() * -2.0 ** 30)
+    y, _ = fp8.experts_forward(x, idx, torch.zeros_like(w), base)
+    assert not y.any()
+    big = x.clone()
+    big[7] *= 2.0 ** 60                                      # both halves of the activation grow: h is 2^120 and more
+    y, _ = fp8.experts_forward(big, idx, w, base)
+    plain, _ = fp8.experts_forward(x, idx, w, base)
+    others = [i for i in range(M) if i != 7]
+    assert torch.equal(y[others], plain[others]) and not torch.isnan(y[7]).any()
 
 
 def test_capture_other_stream_and_two_graphs(fp8):
@@ -330,8 +373,8 @@ def test_an_expert_named_twice_counts_twice_and_bad_ids_are_reported(fp8):
     y, sizes = fp8.experts_forward(x, t([[0, 1], [2, 3], [4, 4], [5, 6]]), w, e)
     assert sizes.tolist() == [1, 1, 1, 1, 2, 1, 1, 0]
     one, _ = fp8.experts_forward(x[2:3], t([[4]]), torch.ones(1, 1, device="cuda"), e)
-    # 0.75 o + 0.25 o: each product and their sum rounded to bfloat16, half a step each
-    assert ((y[2].double() - one[0].double()).abs() <= 3 * 2.0 ** -8 * one[0].double().abs()).all()
+    # 0.75 o + 0.25 o and o, each rounded to bfloat16 once
+    assert ((y[2].double() - one[0].double()).abs() <= 2 * 2.0 ** -8 * one[0].double().abs()).all()
     ops.check_status()
     for ids in ([[0, 1], [2, 8], [4, 5], [5, 6]], [[0, 1], [2, 3], [4, -1], [5, 6]]):
         fp8.experts_forward(x, t(ids), w, e)

@@ -85,7 +85,11 @@ def test_fp8_arguments(lib):
         assert f(p, ONE, ONE, ONE, None, ONE, ONE, None) == -1 and f(p, ODD, ONE, ONE, ONE, ONE, ONE, None) == -1
         assert f(None, ONE, ONE, ONE, ONE, ONE, ONE, None) == -1
     for f in (L.momoe_fp8_down_scale, stream(L.momoe_fp8_down_scale_decode)):
-        assert f(p, ONE, ONE, ONE, None, ONE, None) == -1 and f(p, ONE, ONE, ONE, ONE, None, None) == -1
+        assert f(p, ONE, ONE, ONE, None, ONE, ONE, None) == -1 and f(p, ONE, ONE, ONE, ONE, None, ONE, None) == -1
+        assert f(p, ONE, ONE, ONE, ONE, ONE, None, None) == -1 and f(p, ONE, ONE, ONE, ONE, ODD, ONE, None) == -1
+    assert L.momoe_fp8_combine_rows(ONE, ONE, ONE, 4, 2, 60, ONE, None) == -2
+    assert L.momoe_fp8_combine_rows(ONE, ONE, ONE, 4, 0, 64, ONE, None) == -1
+    assert L.momoe_fp8_combine_rows(ODD, ONE, ONE, 4, 2, 64, ONE, None) == -1
     assert L.momoe_fp8_up_swiglu_decode(p, None, ONE, ONE, ONE, ONE, ONE, ONE, None) == -1
     def whole(M=4, N=8, K=2, D=64, H=32, x=ONE, ws=ONE, n=None):
         n = L.momoe_fp8_experts_workspace_bytes(M, N, K, D, H) if n is None else n
