@@ -93,23 +93,24 @@ __device__ __forceinline__ void d8_tmem_ld(uint32_t taddr, uint32_t (&r)[T]) {
     else tmem_ld32(taddr, r);
 }
 
+// down: lane t gets the weight of token t times its power of two, whose inverse is stored.
+__device__ __forceinline__ float d8_factor(const Fp8DecArgs& g, const D8Item& w, size_t row0, bool store) {
+    const int lane = threadIdx.x & 31;
+    const float wgt = __ldcg(g.row_weight + row0 + lane);
+    const int w_blocks = (g.out_cols + 127) / 128, n0 = w.cb * 2;
+    const int e = fp8_row_exponent(g.x_scale + fp8_atom_offset(row0 + lane, 0, (g.nkb + 3) >> 2),
+                                   g.w_scale + (static_cast<size_t>(w.e) * w_blocks + n0) * g.nkb, n0 + 1 < w_blocks, g.nkb,
+                                   wgt);
+    if (store) g.y_scale[(row0 + lane) * g.n_cblk + w.cb] = pow2f(-e);
+    return wgt * pow2f(e);
+}
+
 // The first T tokens of a 32-row block out of the accumulators (columns taddr and taddr + D8_NT), by the four epilogue
 // warps; `last`: hand the accumulators back.  False when a wait was abandoned.
 template <bool UP, int SPLIT, int T>
 __device__ __forceinline__ bool d8_read_out(const Fp8DecArgs& g, D8Epi& c, const D8Item& w, size_t row0, uint32_t taddr,
-                                            bool last) {
+                                            bool last, float factor) {
     const int lane = threadIdx.x & 31, q = (threadIdx.x >> 5) & 3;
-    float wgt = 0.0f;
-    if constexpr (!UP) {
-        // lane t holds the weight and the power of two of token t
-        wgt = __ldcg(g.row_weight + row0 + lane);
-        const int w_blocks = (g.out_cols + 127) / 128, n0 = w.cb * 2;
-        const int e = fp8_row_exponent(g.x_scale + fp8_atom_offset(row0 + lane, 0, (g.nkb + 3) >> 2),
-                                       g.w_scale + (static_cast<size_t>(w.e) * w_blocks + n0) * g.nkb, n0 + 1 < w_blocks,
-                                       g.nkb, wgt);
-        if (q == 0 && lane < T && (SPLIT == 1 || c.rank == 0)) g.y_scale[(row0 + lane) * g.n_cblk + w.cb] = pow2f(-e);
-        wgt *= pow2f(e);
-    }
     uint32_t r[T], rb[T];
     d8_tmem_ld<T>(taddr, r);
     d8_tmem_ld<T>(taddr + D8_NT, rb);
@@ -185,7 +186,7 @@ __device__ __forceinline__ bool d8_read_out(const Fp8DecArgs& g, D8Epi& c, const
             __half* dst = g.y + row0 * g.out_cols + col;
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                const float s = __shfl_sync(0xffffffffu, wgt, t);
+                const float s = __shfl_sync(0xffffffffu, factor, t);
                 if (col < g.out_cols)
                     dst[static_cast<size_t>(t) * g.out_cols] = __float2half_rn(__uint_as_float(i == 0 ? r[t] : rb[t]) * s);
             }
@@ -388,6 +389,10 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         bool ok = true;
         for (int item = first_item; ok && item < total_items; item += step_item, ++it) {
             const D8Item w = item == first_item ? first : d8_item(g, item);
+            // down: what does not need the accumulators is worked out while they fill
+            const bool store = q == 0 && (SPLIT == 1 || rank == 0);
+            float factor = 0.0f;
+            if constexpr (!UP) factor = d8_factor(g, w, static_cast<size_t>(w.tile) * TILE_M, store && lane < w.rows);
             ok = mbar_wait(smem_u32(&bar_acc_full), it & 1u, abortp, g.status, DEV_TIMEOUT_EPILOGUE);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -396,8 +401,12 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
                 const size_t row0 = static_cast<size_t>(w.tile) * TILE_M + sub * 32;
                 const bool last = sub + 1 == w.n_sub;
                 // a token more costs a reduction and a store, so a few rows take the short form
-                ok = w.rows - sub * 32 <= 8 ? d8_read_out<UP, SPLIT, 8>(g, c, w, row0, taddr + sub * 32, last)
-                               : d8_read_out<UP, SPLIT, 32>(g, c, w, row0, taddr + sub * 32, last);
+                const int left = w.rows - sub * 32;
+                if constexpr (!UP) {
+                    if (sub > 0) factor = d8_factor(g, w, row0, store && lane < left);
+                }
+                ok = left <= 8 ? d8_read_out<UP, SPLIT, 8>(g, c, w, row0, taddr + sub * 32, last, factor)
+                               : d8_read_out<UP, SPLIT, 32>(g, c, w, row0, taddr + sub * 32, last, factor);
             }
         }
     }
