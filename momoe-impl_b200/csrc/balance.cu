@@ -130,6 +130,7 @@ struct BalArgs {
     float* slot_z;       // [n_blk + B]
     float* share;        // [column blocks * B]
     unsigned* ticket;
+    int* totals;         // [2]: sequences that are not empty, all their tokens
     float* loss;
     long long* counts;   // [B, N]
     float* g;            // [B, N]
@@ -145,7 +146,27 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_partial_kernel(const BalA
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, l = lane % L;
     const int c = blockIdx.x;
     const int row0 = c * a.R, row1 = min(a.M, row0 + a.R);
-    if (c == 0 && threadIdx.x == 0) *a.ticket = 0u;
+    if (c == 0) {
+        // once for the whole call, whatever the number of sequences
+        __shared__ int s_tot[2];
+        if (threadIdx.x == 0) {
+            *a.ticket = 0u;
+            s_tot[0] = s_tot[1] = 0;
+        }
+        __syncthreads();
+        int n = 0, tokens = 0;
+        for (int i = threadIdx.x; i < a.B; i += BAL_THREADS) {
+            const int len = a.seq.bound(i + 1) - a.seq.bound(i);
+            if (len > 0) {
+                ++n;
+                tokens += len;
+            }
+        }
+        atomicAdd(&s_tot[0], n);
+        atomicAdd(&s_tot[1], tokens);
+        __syncthreads();
+        if (threadIdx.x < 2) a.totals[threadIdx.x] = s_tot[threadIdx.x];
+    }
     const T* logits = static_cast<const T*>(a.logits);
     const int Ng = a.N - a.Ks;
     int b = a.seq.of(row0);
@@ -213,30 +234,12 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_partial_kernel(const BalA
 __global__ void __launch_bounds__(1024) balance_finish_kernel(const BalArgs a) {
     __shared__ float s_p[32][33];
     __shared__ int s_c[32][33];
-    __shared__ int s_seq[32];
     __shared__ float s_red[32];
     __shared__ bool s_last;
     const int tx = threadIdx.x, ty = threadIdx.y, tid = ty * 32 + tx;
     const int b = blockIdx.y;
     const int start = a.seq.bound(b), end = a.seq.bound(b + 1);
-    // sequences that are not empty, and all their tokens
-    int n = 0, tokens = 0;
-    for (int i = tid; i < a.B; i += 1024) {
-        const int len = a.seq.bound(i + 1) - a.seq.bound(i);
-        if (len > 0) {
-            ++n;
-            tokens += len;
-        }
-    }
-    n = __reduce_add_sync(0xffffffffu, n);
-    tokens = __reduce_add_sync(0xffffffffu, tokens);
-    if (tx == 0) {
-        s_seq[ty] = n;
-        s_red[ty] = __int_as_float(tokens);
-    }
-    __syncthreads();
-    n = __reduce_add_sync(0xffffffffu, s_seq[tx]);
-    tokens = __reduce_add_sync(0xffffffffu, __float_as_int(s_red[tx]));
+    const int n = a.totals[0], tokens = a.totals[1];
 
     const int e = blockIdx.x * 32 + tx;
     const int Ng = a.N - a.Ks;
@@ -382,7 +385,7 @@ static int bal_rows(int M) {
 }
 
 struct BalLayout {
-    size_t p, count, z, share, ticket, bytes;
+    size_t p, count, z, share, ticket, totals, bytes;
 };
 static BalLayout bal_layout(int M, int N, int B) {
     const size_t slots = static_cast<size_t>((M + bal_rows(M) - 1) / bal_rows(M)) + B;
@@ -392,7 +395,8 @@ static BalLayout bal_layout(int M, int N, int B) {
     l.z = l.count + slots * N * 4;
     l.share = l.z + slots * 4;
     l.ticket = l.share + static_cast<size_t>((N + 31) / 32) * B * 4;
-    l.bytes = l.ticket + 4;
+    l.totals = l.ticket + 4;
+    l.bytes = l.totals + 8;
     return l;
 }
 
@@ -467,6 +471,7 @@ MOMOE_API int momoe_balance_loss(const void* logits_MN, int32_t type, const int3
     a.slot_z = reinterpret_cast<float*>(ws + l.z);
     a.share = reinterpret_cast<float*>(ws + l.share);
     a.ticket = reinterpret_cast<unsigned*>(ws + l.ticket);
+    a.totals = reinterpret_cast<int*>(ws + l.totals);
     a.loss = loss;
     a.counts = reinterpret_cast<long long*>(counts_BN);
     a.g = grad_BN;

@@ -85,6 +85,10 @@ Tensor dense(const Tensor& t) {
     Tensor c = t.contiguous();
     return is_aligned(c) ? c : c.clone();
 }
+// Whole numbers as contiguous int32; wider ones are first brought into [lo, hi], which keeps the ones outside outside.
+Tensor whole32(const Tensor& t, int64_t lo, int64_t hi) {
+    return (t.scalar_type() == at::kInt ? t : t.clamp(lo, hi).to(at::kInt)).contiguous();
+}
 // t [..., D] as [M, D] with contiguous columns, a row pitch of a multiple of 8 elements and a 16-byte aligned start: a
 // view where the layout allows it.
 Tensor as_rows(const Tensor& t) {
@@ -310,7 +314,7 @@ std::vector<Tensor> balance_loss(const Tensor& logits, const Tensor& topk_idx, i
                 "0 <= shared experts < K <= N <= 1024 is needed, but got: Ks = ", Ks, ", K = ", K, ", N = ", N);
     TORCH_CHECK(!(cu_seqlens && seq_len), "give cu_seqlens or seq_len, not both");
     const c10::cuda::CUDAGuard guard(dev);
-    const Tensor idx = topk_idx.to(at::kInt).contiguous();
+    const Tensor idx = whole32(topk_idx, -1, N);
     OptTensor cu;
     int64_t S = 0, B = 0;
     if (cu_seqlens) {
@@ -319,7 +323,7 @@ std::vector<Tensor> balance_loss(const Tensor& logits, const Tensor& topk_idx, i
                         at::isIntegralType(cu_seqlens->scalar_type(), false),
                     "cu_seqlens must be whole numbers [B + 1], but got: ", cu_seqlens->sizes(), " in ",
                     cu_seqlens->dtype());
-        cu = cu_seqlens->to(at::kInt).contiguous();
+        cu = whole32(*cu_seqlens, 0, M);
         B = cu->size(0) - 1;
     } else {
         const int64_t most = M > 0 ? M : 1;
@@ -383,7 +387,7 @@ std::vector<Tensor> experts_forward(const Tensor& x, const OptTensor& scale, con
                     "rows of ", x.dtype(), " need their scales: pass Fp8Rows");
         rows = dense(x.to(at::kBFloat16));
     }
-    const Tensor idx = topk_idx.to(at::kInt).contiguous(), w = topk_w.to(at::kFloat).contiguous();
+    const Tensor idx = whole32(topk_idx, -1, N), w = topk_w.to(at::kFloat).contiguous();
     const auto opt = rows.options();
     Tensor y = at::empty({M, D}, opt.dtype(at::kBFloat16));
     if (M == 0) return {y, at::zeros({N}, opt.dtype(at::kLong))};

@@ -91,6 +91,12 @@ class FusedMoEFunction(torch.autograd.Function):
 
 
 class MoE(nn.Module):
+    balance_coef = 0.0     # weight of the balance loss (each of a batch's sequences on its own)
+    z_coef = 0.0           # weight of the z-loss
+    aux_loss = None        # their sum of the latest forward pass, float32 [], differentiable; None if both are 0
+    experts_fp8 = None     # 8-bit weights of forward-only calls, from quantize_experts()
+    _fp8_versions = None
+
     def __init__(self, embedding_dim, intermediate_dim, num_experts, num_chosen_experts, num_shared_experts,
                  save_percent=0, bias_update_rate=1e-4, Wg_DN: torch.Tensor | None = None,
                  Wl1_ND2H: torch.Tensor | None = None, Wl2_NHD: torch.Tensor | None = None):
@@ -113,11 +119,12 @@ class MoE(nn.Module):
                        torch.full((self.Ks,), float("-inf"), device=dev, dtype=torch.float32)], dim=-1),
             requires_grad=False)
         self.fused = True
-        self.balance_coef = 0.0     # weight of the balance loss (each of a batch's sequences on its own)
-        self.z_coef = 0.0           # weight of the z-loss
-        self.aux_loss = None        # their sum of the latest forward pass, float32 [], differentiable; None if both are 0
-        self.experts_fp8 = None     # 8-bit weights of forward-only calls, from quantize_experts()
-        self._fp8_versions = None
+
+    def __getstate__(self):
+        state = dict(self.__dict__)
+        state.pop("aux_loss", None)         # belongs to the graph of a forward pass, not to a copy of the layer
+        state.pop("_fp8_versions", None)    # a copy's parameters count their versions anew
+        return state
 
     def quantize_experts(self):
         """From now on forward passes use an 8-bit copy of the expert weights as they are now.  Such passes have no
@@ -129,7 +136,10 @@ class MoE(nn.Module):
     def _forward_fp8(self, x_BSD, rows):
         if torch.is_grad_enabled() and (x_BSD.requires_grad or any(p.requires_grad for p in self.parameters())):
             raise RuntimeError("8-bit experts have no backward pass: call the layer under torch.no_grad()")
-        if self._fp8_versions != (self.momoe.Wl1_ND2H._version, self.momoe.Wl2_NHD._version):
+        versions = (self.momoe.Wl1_ND2H._version, self.momoe.Wl2_NHD._version)
+        if self._fp8_versions is None:
+            self._fp8_versions = versions
+        if self._fp8_versions != versions:
             raise RuntimeError("the expert weights have changed since quantize_experts(): call it again")
         Wg = self.router.Wg_DN
         assert Wg.dtype == torch.bfloat16, "Wg_DN must be of type torch.bfloat16"

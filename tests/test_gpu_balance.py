@@ -111,6 +111,11 @@ def test_many_rows_many_sequences_twice_the_same(balance):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+def test_as_many_sequences_as_rows(balance):
+    logits, idx = make(9001, 24, 2, 0, 13, torch.bfloat16)
+    check(balance, logits, idx, 0, 0.4, 0.2, list(range(9002)), seq_len=1)
+
+
 def test_even_routing_gives_the_coefficient_and_ids_outside_are_not_counted(balance):
     logits = torch.zeros(64, 16, dtype=torch.bfloat16, device="cuda")
     idx = (torch.arange(64)[:, None] * 2 + torch.arange(2)).remainder(16).int().cuda()
@@ -118,6 +123,7 @@ def test_even_routing_gives_the_coefficient_and_ids_outside_are_not_counted(bala
     assert float(loss) == pytest.approx(0.25, rel=F32) and (counts == 8).all()
     idx[0], idx[1, 0] = -1, 16
     check(balance, logits, idx, 0, 0.25, 0.1, [0, 64])
+    check(balance, logits, idx.long() + 2 ** 32 * (idx < 0), 0, 0.25, 0.1, [0, 64])      # wide ids are not wrapped around
     idx[5] = 3                                               # the same expert twice counts twice
     check(balance, logits, idx, 0, 0.25, 0.1, [0, 64])
 

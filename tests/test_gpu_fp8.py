@@ -298,6 +298,24 @@ def test_bad_rows_stay_alone_and_strides(fp8):
 
 
 @pytest.mark.parametrize("stream", [False, True])
+def test_same_bits_every_time(fp8, monkeypatch, stream):
+    """Rows of an expert are placed in no fixed order, across several tiles; the results do not depend on it."""
+    monkeypatch.setattr(fp8, "STREAM_MAX_AVG_ROWS", 2 ** 20 if stream else 0)
+    for M, N, K in ((700, 5, 3), (9000, 6, 2)):
+        idx, w = routing(M, N, K, 1, 2.0)
+        e = fp8.quantize_experts(*weights(fp8, N, 256, 144, 6))
+        x = torch.randn(M, 256, generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+        want, sizes = fp8.experts_forward(x, idx, w, e)
+        assert int(sizes.max()) > 256
+        for _ in range(12):
+            y, n = fp8.experts_forward(x, idx, w, e)
+            assert torch.equal(y, want) and torch.equal(n, sizes)
+        order = torch.randperm(M, generator=torch.Generator().manual_seed(7)).cuda()
+        y, _ = fp8.experts_forward(x[order], idx[order], w[order], e)
+        assert torch.equal(y, want[order])
+
+
+@pytest.mark.parametrize("stream", [False, True])
 def test_result_rows_keep_their_range(fp8, monkeypatch, stream):
     """Values far beyond fp16 and far below it, and rows of unlike size, come out with one bfloat16 rounding: the
     intermediate rows carry a power of two each."""
@@ -376,8 +394,9 @@ def test_an_expert_named_twice_counts_twice_and_bad_ids_are_reported(fp8):
     # 0.75 o + 0.25 o and o, each rounded to bfloat16 once
     assert ((y[2].double() - one[0].double()).abs() <= 2 * 2.0 ** -8 * one[0].double().abs()).all()
     ops.check_status()
-    for ids in ([[0, 1], [2, 8], [4, 5], [5, 6]], [[0, 1], [2, 3], [4, -1], [5, 6]]):
-        fp8.experts_forward(x, t(ids), w, e)
+    for ids in (t([[0, 1], [2, 8], [4, 5], [5, 6]]), t([[0, 1], [2, 3], [4, -1], [5, 6]]),
+                t([[0, 1], [2, 3], [4, 5], [5, 6]]).long() + 2 ** 32):
+        fp8.experts_forward(x, ids, w, e)
         with pytest.raises(RuntimeError, match="202"):
             ops.check_status()
     many = t([[0, 1]]).expand(9000, 2).clone()               # the two-launch dispatch reports as well
@@ -447,6 +466,11 @@ def test_prenorm_layer_in_eight_bits_is_its_operators_in_a_row(fp8):
         assert float((y.float() - y16.float()).norm() / y16.float().norm()) < 0.12
         alone = block(x)
         assert torch.equal(alone[1], x)
+    import copy
+    twin = copy.deepcopy(moe)
+    with torch.no_grad():
+        twin.biases_N.copy_(moe.biases_N)
+        assert torch.equal(twin(x), moe(x))
     # refusals: gradients, stale weights, rows without 8-bit experts, training coefficients
     with pytest.raises(RuntimeError, match="no backward"):
         moe(x)
@@ -459,7 +483,9 @@ def test_prenorm_layer_in_eight_bits_is_its_operators_in_a_row(fp8):
         with pytest.raises(RuntimeError, match="changed"):
             moe(x)
         moe.quantize_experts()
-        moe(x)
+        twin = copy.deepcopy(moe)
+        twin.biases_N.copy_(moe.biases_N)
+        assert torch.equal(twin(x), moe(x))
         moe.experts_fp8 = None
         with pytest.raises(RuntimeError, match="8-bit experts"):
             moe(x, n.rows)
@@ -489,6 +515,9 @@ def test_layer_with_balance_loss_trains_on_the_sum_of_both(fp8, fused):
     assert plain.aux_loss is None
     moe, block, x, y = run((0.2, 0.05))
     assert torch.equal(y, py)
+    import copy
+    twin = copy.deepcopy(moe)                                # the loss belongs to the graph, not to a copy of the layer
+    assert twin.aux_loss is None and twin.balance_coef == 0.2 and moe.aux_loss is not None
     # the operator on the same logits
     with torch.no_grad():
         n, _ = norm.rms_norm(x, block.norm.weight, torch.ones_like(x))
