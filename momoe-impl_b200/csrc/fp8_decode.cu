@@ -15,11 +15,10 @@
 // One CTA (320 threads) an SM, persistent over items = (128-row tile, column block).  Warp 0 loads, warp 1 issues MMAs,
 // warps 2..5 are the epilogue (a thread has one weight column and 32 tokens at a time), warps 6..9 write scales to TMEM
 // (see the row-tile kernel).  There is one accumulator: the MMAs of an item wait for the read-out of the item before, while
-// the ring goes on filling; they need less than half of the time that the weights take.
+// the ring goes on filling.
 //
-// With so few items that half of the SMs would idle (one token), two CTAs of a cluster share an item's k axis: the second
-// stores its accumulators into the first one's shared memory, which adds them and goes on (XXX against YYY us for both GEMMs
-// of one token, D2048 H768 top-8).
+// With so few items that half of the SMs would idle (one token) and more than 12 k slices, two CTAs of a cluster share an
+// item's k axis: the second stores its accumulators into the first one's shared memory, which adds them and goes on.
 #include <cstring>
 
 #include "fp8.cuh"
@@ -440,11 +439,13 @@ static int d8_launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const Fp8De
                             SPLIT, tmW, tmX, g) == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
 
-// Whether the items leave half of the SMs idle: then two CTAs share an item's k axis.
+// Whether two CTAs share an item's k axis: when the items leave half of the SMs idle, and the k axis is long enough to pay for
+// the meeting.  Whole passes of one token, with the up GEMM shared and not: 18.5 / 18.3 us at 8 k slices, 20.5 / 20.4 at 12,
+// 20.6 / 22.4 at 16, 26.2 / 28.7 at 32 (H512, top-4 of 32), 39.0 / 47.0 at 56 (top-8 of 64).
 static bool d8_split(const momoe_plan_t* p, const Fp8DecArgs& g) {
     const long long msum = static_cast<long long>(p->M) * p->K;
     const long long tiles = msum / TILE_M + (msum < p->N ? msum : p->N);      // an upper bound
-    return tiles * g.n_cblk * 2 <= sm_count() && g.nkb > FP8_GROUP;
+    return tiles * g.n_cblk * 2 <= sm_count() && g.nkb > 3 * FP8_GROUP;
 }
 
 static void d8_args(const momoe_plan_t* p, const int32_t* tile_rows, Fp8DecArgs& g) {

@@ -15,7 +15,7 @@
 // TMEM: 4 columns for the CTA's 128 rows, 8 for the 256 weight columns (one word each, repeated).  The MMAs of the four
 // slices pick their byte of each word through the scale ids of the instruction descriptor.  Two TMEM copies alternate; a
 // copy is overwritten after the commit behind the MMAs that read it has arrived.  (Copies from shared memory by tcgen05.cp
-// sit between the MMAs in the tensor pipe: 536 against XXX us for the up GEMM of 16384 tokens, D2048 H1024, top-8 of 128.)
+// sit between the MMAs in the tensor pipe: 536 against 515 us for the up GEMM of 16384 tokens, D2048 H1024, top-8 of 128.)
 //
 // TMEM.  Two accumulators of 256 columns and 24 columns of scales do not fit 512 columns, so the accumulators overlap: the
 // first takes columns 0..255, the second 224..479, the scales 480..503.  The epilogue reads the 32 shared columns of a
@@ -386,7 +386,8 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 }
             } else {
                 // results leave through shared memory by TMA: with one row a thread, stores straight from registers touch
-                // 32 sectors an instruction and take longer than the tile's MMAs (XXX us against YYY)
+                // 32 sectors an instruction and take longer than the tile's MMAs (328 against 285 us, 16384 tokens, D2048
+                // H1024, top-8 of 128)
 #pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
                     // half 1 starts with the last chunk, which may be the shared one

@@ -25,6 +25,7 @@ SHAPES = [
     (640, 5, 3, 4096, 48, 0.0),
     (90, 40, 6, 256, 144, 3.0),       # few rows on average, some experts with several 32-row blocks
     (1400, 1000, 3, 64, 32, 1.0),     # many experts
+    (40, 4, 2, 2576, 1680, 0.5),      # so few items that two thread blocks share an item's k axis, in both GEMMs
     (6000, 40, 3, 96, 64, 1.0),       # more pairs than one launch dispatches
 ]
 
