@@ -34,18 +34,24 @@ namespace momoe {
 constexpr int F8_EPI_WARPS = 8;
 constexpr int F8_SF_WARPS = 4;
 constexpr int F8_THREADS = 32 * (2 + F8_EPI_WARPS + F8_SF_WARPS);
-constexpr int F8_PAIR_N = 256;
+constexpr int F8_TILE_N = 256;
 constexpr int F8_K = 128;                                 // values of a k slice (128 bytes)
 constexpr int F8_A_BYTES = TILE_M * F8_K;                 // 16 KiB
-constexpr int F8_B_BYTES = F8_PAIR_N / 2 * F8_K;          // 16 KiB
-constexpr int F8_SLICE_BYTES = F8_A_BYTES + F8_B_BYTES;
-constexpr int F8_STAGE_BYTES = 2 * F8_SLICE_BYTES;
-constexpr int F8_STAGES = 3;
+// of CG thread blocks that share a tile: bytes of a CTA's part of a k slice, slices of a stage, stages
+template <int CG>
+constexpr int F8_SLICE_BYTES = F8_A_BYTES + F8_TILE_N / CG * F8_K;
+template <int CG>
+constexpr int F8_SLICES = CG;
+template <int CG>
+constexpr int F8_STAGES = CG == 2 ? 3 : 4;
+template <int CG>
+constexpr int F8_STAGE_BYTES = F8_SLICES<CG> * F8_SLICE_BYTES<CG>;
 constexpr int F8_PIECE = 2048;                            // staging of results: 32 rows x 64 bytes
 template <bool UP>
 constexpr int F8_PIECES = UP ? 1 : 2;                     // pieces an epilogue warp has
-template <bool UP>
-constexpr int F8_SMEM_BYTES = F8_STAGES * F8_STAGE_BYTES + F8_EPI_WARPS * F8_PIECES<UP> * F8_PIECE + 1024;
+template <bool UP, int CG>
+constexpr int F8_SMEM_BYTES = F8_STAGES<CG> * F8_STAGE_BYTES<CG> + F8_EPI_WARPS * F8_PIECES<UP> * F8_PIECE + 1024;
+constexpr long long F8_SINGLE_ROWS = 128;
 constexpr int F8_ACC1 = 224;                              // first column of the second accumulator
 constexpr int F8_SF_COL = 480;
 constexpr int F8_SF_COLS = 12;                            // 4 for A, 8 for B
@@ -76,23 +82,43 @@ struct Fp8Work {
     int tile, nb, e;
     bool valid;
 };
+template <int CG>
 __device__ __forceinline__ Fp8Work f8_work(const Fp8Args& g, int item, uint32_t cta_rank) {
     Fp8Work w;
     w.nb = item % g.n_nblk;
-    const int info = __ldcg(g.pair_info + item / g.n_nblk);
-    w.tile = (info >> 1) + static_cast<int>(cta_rank);
-    w.valid = cta_rank == 0 || (info & 1) != 0;
-    w.e = __ldcg(g.tile_expert + (info >> 1));
+    if constexpr (CG == 2) {
+        const int info = __ldcg(g.pair_info + item / g.n_nblk);
+        w.tile = (info >> 1) + static_cast<int>(cta_rank);
+        w.valid = cta_rank == 0 || (info & 1) != 0;
+        w.e = __ldcg(g.tile_expert + (info >> 1));
+    } else {
+        w.tile = item / g.n_nblk;
+        w.valid = true;
+        w.e = __ldcg(g.tile_expert + w.tile);
+    }
     return w;
 }
+// The same variable in the CTA that issues the MMAs.
+template <int CG>
+__device__ __forceinline__ uint32_t f8_lead(uint32_t addr) {
+    return CG == 2 ? mapa_shared(addr, 0) : addr;
+}
+// All MMAs so far have completed: an arrival in every CTA of the tile.
+template <int CG>
+__device__ __forceinline__ void f8_commit(uint32_t bar) {
+    if constexpr (CG == 2) umma_commit_pair(bar, 3);
+    else umma_commit(bar);
+}
 
-template <bool UP>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8_THREADS, 1)
+template <bool UP, int CG>
+__global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(F8_THREADS, 1)
 fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmO, const Fp8Args g) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bar_full[F8_STAGES];
-    __shared__ uint64_t bar_empty[F8_STAGES];
+    constexpr int STAGES = F8_STAGES<CG>, SLICES = F8_SLICES<CG>;
+    constexpr int SLICE_BYTES = F8_SLICE_BYTES<CG>, STAGE_BYTES = F8_STAGE_BYTES<CG>;
+    __shared__ uint64_t bar_full[STAGES];
+    __shared__ uint64_t bar_empty[STAGES];
     __shared__ uint64_t bar_sf_full[2];              // leader: both CTAs' scale warps have written this copy
     __shared__ uint64_t bar_sf_empty[2];             // both: the MMAs that read this copy have completed
     __shared__ uint64_t bar_acc_full[2];
@@ -104,47 +130,52 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const uint32_t cta_rank = cluster_ctarank();
+    const uint32_t cta_rank = CG == 2 ? cluster_ctarank() : 0u;
     const bool leader = cta_rank == 0;
-    const int cluster_id = blockIdx.x >> 1;
-    const int n_clusters = gridDim.x >> 1;
+    const int cluster_id = blockIdx.x / CG;
+    const int n_clusters = gridDim.x / CG;
     const uint32_t stage_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t epi_base = stage_base + F8_STAGES * F8_STAGE_BYTES;
+    const uint32_t epi_base = stage_base + STAGES * STAGE_BYTES;
 
     const int n_groups = (g.nkb + FP8_GROUP - 1) / FP8_GROUP;
     grid_launch_dependents();
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int s = 0; s < F8_STAGES; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&bar_full[s]), 1);
             mbar_init(smem_u32(&bar_empty[s]), 1);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(smem_u32(&bar_sf_full[b]), 2 * F8_SF_WARPS);
+            mbar_init(smem_u32(&bar_sf_full[b]), CG * F8_SF_WARPS);
             mbar_init(smem_u32(&bar_sf_empty[b]), 1);
             mbar_init(smem_u32(&bar_acc_full[b]), 1);
-            mbar_init(smem_u32(&bar_acc_empty[b]), 2 * F8_EPI_WARPS);
+            mbar_init(smem_u32(&bar_acc_empty[b]), CG * F8_EPI_WARPS);
         }
-        mbar_init(smem_u32(&bar_ovl), F8_EPI_WARPS);   // four warps of each CTA read the shared columns
+        mbar_init(smem_u32(&bar_ovl), CG * F8_EPI_WARPS / 2);   // four warps of each CTA read the shared columns
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
         tma_prefetch_desc(&tmO);
     }
     if (warp == 1) {
-        tmem_alloc_pair(smem_u32(&tmem_slot), 512);
-        tmem_relinquish_pair();
+        if constexpr (CG == 2) {
+            tmem_alloc_pair(smem_u32(&tmem_slot), 512);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_u32(&tmem_slot), 512);
+            tmem_relinquish();
+        }
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync_all();
+    if constexpr (CG == 2) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
     volatile int* abortp = &abort_flag;
     // everything above ran beside the tail of the kernel before; from here on its results are read
     grid_wait();
-    const int total_items = __ldcg(g.sched + SCHED_N_PAIRS) * g.n_nblk;
+    const int total_items = __ldcg(g.sched + (CG == 2 ? SCHED_N_PAIRS : SCHED_N_TILES)) * g.n_nblk;
 
     if (warp == 0) {
         // ================================================================ loads
@@ -154,23 +185,34 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             bool ok = true;
             const int r = static_cast<int>(cta_rank);
             for (int item = cluster_id; ok && item < total_items; item += n_clusters) {
-                const Fp8Work w = f8_work(g, item, cta_rank);
-                for (int kb = 0; kb < g.nkb; kb += 2) {
+                const Fp8Work w = f8_work<CG>(g, item, cta_rank);
+                for (int kb = 0; kb < g.nkb; kb += SLICES) {
                     ok = mbar_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, abortp, g.status, DEV_TIMEOUT_PRODUCER);
                     if (!ok) break;
-                    if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[stage]), 2 * F8_STAGE_BYTES);
-                    const uint32_t full = mapa_shared(smem_u32(&bar_full[stage]), 0);
+                    if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[stage]), CG * STAGE_BYTES);
+                    const uint32_t full = f8_lead<CG>(smem_u32(&bar_full[stage]));
                     // tensor maps count in 16-bit units; a slice past the end of the k axis is zero-filled
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t sa = stage_base + stage * F8_STAGE_BYTES + h * F8_SLICE_BYTES;
+                    for (int h = 0; h < SLICES; ++h) {
+                        const uint32_t sa = stage_base + stage * STAGE_BYTES + h * SLICE_BYTES;
                         const int k0 = (kb + h) * (F8_K / 2);
-                        tma_load_2d_pair(sa, &tmA, full, k0, w.tile * TILE_M);
-                        // up: the leader loads 128 rows of the linear half of W1[e], its peer the matching gate rows
-                        if constexpr (UP) tma_load_3d_pair(sa + F8_A_BYTES, &tmB, full, k0, w.nb * 128, w.e * 2 + r);
-                        else tma_load_3d_pair(sa + F8_A_BYTES, &tmB, full, k0, w.nb * F8_PAIR_N + r * 128, w.e);
+                        // up: 128 rows of the linear half of W1[e] and the matching gate rows; of a pair, the leader
+                        // loads the former and its peer the latter
+                        if constexpr (CG == 2) {
+                            tma_load_2d_pair(sa, &tmA, full, k0, w.tile * TILE_M);
+                            if constexpr (UP) tma_load_3d_pair(sa + F8_A_BYTES, &tmB, full, k0, w.nb * 128, w.e * 2 + r);
+                            else tma_load_3d_pair(sa + F8_A_BYTES, &tmB, full, k0, w.nb * F8_TILE_N + r * 128, w.e);
+                        } else {
+                            tma_load_2d(sa, &tmA, full, k0, w.tile * TILE_M);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t sb = sa + F8_A_BYTES + i * 128 * F8_K;
+                                if constexpr (UP) tma_load_3d(sb, &tmB, full, k0, w.nb * 128, w.e * 2 + i);
+                                else tma_load_3d(sb, &tmB, full, k0, w.nb * F8_TILE_N + i * 128, w.e);
+                            }
+                        }
                     }
-                    if (++stage == F8_STAGES) { stage = 0; phase ^= 1u; }
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
         }
@@ -201,38 +243,44 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
 #pragma unroll
                     for (int j = 0; j < FP8_GROUP; ++j) {
                         if (kb0 + j < g.nkb) {
-                            if ((j & 1) == 0) {
+                            if (j % SLICES == 0) {
                                 ok = ok && mbar_wait(smem_u32(&bar_full[stage]), phase, abortp, g.status, DEV_TIMEOUT_MMA);
                                 tc_fence_after();
                             }
                             if (ok) {
-                                const uint32_t idesc = umma_idesc_fp8(2 * TILE_M, F8_PAIR_N, j);
-                                const uint32_t lo = a_lo + (j & 1) * (F8_SLICE_BYTES >> 4);
+                                const uint32_t idesc = umma_idesc_fp8(CG * TILE_M, F8_TILE_N, j);
+                                const uint32_t lo = a_lo + j % SLICES * (SLICE_BYTES >> 4);
 #pragma unroll
-                                for (uint32_t k = 0; k < 4; ++k)
-                                    umma_fp8_pair_lohi(tmem_d, lo + k * 2u, desc_hi, lo + b_off + k * 2u, desc_hi, idesc,
-                                                       sf, sf + 4, (kb0 + j + static_cast<int>(k)) != 0 ? 1u : 0u);
-                                if ((j & 1) == 1 || kb0 + j + 1 == g.nkb) {
-                                    umma_commit_pair(smem_u32(&bar_empty[stage]), 3);
-                                    a_lo += F8_STAGE_BYTES >> 4;
-                                    if (++stage == F8_STAGES) { stage = 0; phase ^= 1u; a_lo = a_lo0; }
+                                for (uint32_t k = 0; k < 4; ++k) {
+                                    const uint32_t more = (kb0 + j + static_cast<int>(k)) != 0 ? 1u : 0u;
+                                    if constexpr (CG == 2)
+                                        umma_fp8_pair_lohi(tmem_d, lo + k * 2u, desc_hi, lo + b_off + k * 2u, desc_hi,
+                                                           idesc, sf, sf + 4, more);
+                                    else
+                                        umma_fp8_lohi(tmem_d, lo + k * 2u, desc_hi, lo + b_off + k * 2u, desc_hi, idesc, sf,
+                                                      sf + 4, more);
+                                }
+                                if (j % SLICES == SLICES - 1 || kb0 + j + 1 == g.nkb) {
+                                    f8_commit<CG>(smem_u32(&bar_empty[stage]));
+                                    a_lo += STAGE_BYTES >> 4;
+                                    if (++stage == STAGES) { stage = 0; phase ^= 1u; a_lo = a_lo0; }
                                 }
                             }
                         }
                     }
-                    if (ok) umma_commit_pair(smem_u32(&bar_sf_empty[gi & 1]), 3);
+                    if (ok) f8_commit<CG>(smem_u32(&bar_sf_empty[gi & 1]));
                 }
-                if (ok) umma_commit_pair(smem_u32(&bar_acc_full[ab]), 3);
+                if (ok) f8_commit<CG>(smem_u32(&bar_acc_full[ab]));
             }
         }
     } else if (warp >= 2 + F8_EPI_WARPS) {
         // ================================================================ scales (both CTAs, four whole warps)
         int gi = 0;
         bool ok = true;
-        const uint32_t full0 = mapa_shared(smem_u32(&bar_sf_full[0]), 0);
+        const uint32_t full0 = f8_lead<CG>(smem_u32(&bar_sf_full[0]));
         const uint32_t sf0 = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + F8_SF_COL;
         for (int item = cluster_id; ok && item < total_items; item += n_clusters) {
-            const Fp8Work w = f8_work(g, item, cta_rank);
+            const Fp8Work w = f8_work<CG>(g, item, cta_rank);
             const int tile = w.valid ? w.tile : w.tile - 1;     // a missing half reads its partner's scales
             const uint4* src = reinterpret_cast<const uint4*>(g.a_scale + static_cast<size_t>(tile) * n_groups * FP8_ATOM);
             // the two blocks of 128 weight columns of this item
@@ -274,15 +322,15 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const int q = warp & 3;
         const int row = q * 32 + lane;
         const int half = (warp - 2) >> 2;
-        const uint32_t acc_empty_leader = mapa_shared(smem_u32(&bar_acc_empty[0]), 0);
-        const uint32_t ovl_leader = mapa_shared(smem_u32(&bar_ovl), 0);
+        const uint32_t acc_empty_leader = f8_lead<CG>(smem_u32(&bar_acc_empty[0]));
+        const uint32_t ovl_leader = f8_lead<CG>(smem_u32(&bar_ovl));
         constexpr int PIECES = F8_PIECES<UP>;
         const uint32_t stage_area = epi_base + (warp - 2) * PIECES * F8_PIECE;
         int it = 0;
         bool ok = true;
         int n_stored = 0;                  // pieces handed to TMA stores so far (lane 0 owns the bulk groups)
         for (int item = cluster_id; ok && item < total_items; item += n_clusters, ++it) {
-            const Fp8Work w = f8_work(g, item, cta_rank);
+            const Fp8Work w = f8_work<CG>(g, item, cta_rank);
             const int ab = it & 1;
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + ab * F8_ACC1;
             // the accumulator whose neighbour follows above shares its last 32 columns, the other one its first
@@ -397,7 +445,7 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     tmem_ld_wait();
                     if (i == 0 && shares) hand_back_shared();
                     if (i == 3) hand_back_all();
-                    const int col0 = w.nb * F8_PAIR_N + c * 32;
+                    const int col0 = w.nb * F8_TILE_N + c * 32;
                     if (w.valid && col0 < g.out_cols) {
                         const uint32_t slot = stage_area + n_stored % PIECES * F8_PIECE;
                         if (n_stored >= PIECES && lane == 0) bulk_wait_read<PIECES - 1>();
@@ -436,49 +484,53 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000LL) __nanosleep(1000);
     }
-    cluster_sync_all();
+    if constexpr (CG == 2) cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_pair(tmem_base, 512);
+        if constexpr (CG == 2) tmem_dealloc_pair(tmem_base, 512);
+        else tmem_dealloc(tmem_base, 512);
     }
 }
 
-template <bool UP>
+template <bool UP, int CG>
 static int f8_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmO, const Fp8Args& g,
                      cudaStream_t stream) {
-    static bool attr_set[64] = {false};
-    static int pairs[64] = {0};
+    static int blocks[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MOMOE_ERR_CUDA;
-    if (!attr_set[dev]) {
-        if (cudaFuncSetAttribute(fp8_grouped_gemm_kernel<UP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 F8_SMEM_BYTES<UP>) != cudaSuccess)
+    const auto kernel = fp8_grouped_gemm_kernel<UP, CG>;
+    constexpr int smem = F8_SMEM_BYTES<UP, CG>;
+    if (blocks[dev] == 0) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
             return MOMOE_ERR_CUDA;
-        attr_set[dev] = true;
-    }
-    if (pairs[dev] == 0) {
-        cudaLaunchConfig_t cfg;
-        memset(&cfg, 0, sizeof(cfg));
-        cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
-        cfg.blockDim = dim3(F8_THREADS);
-        cfg.dynamicSmemBytes = F8_SMEM_BYTES<UP>;
-        cudaLaunchAttribute attr;
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = 2;
-        attr.val.clusterDim.y = 1;
-        attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, fp8_grouped_gemm_kernel<UP>, &cfg) != cudaSuccess || n <= 0) {
-            (void)cudaGetLastError();
-            n = sm_count() / 2;
+        int n = sm_count() / CG;
+        if (CG == 2) {
+            cudaLaunchConfig_t cfg;
+            memset(&cfg, 0, sizeof(cfg));
+            cfg.gridDim = dim3(static_cast<unsigned>(n * CG));
+            cfg.blockDim = dim3(F8_THREADS);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = CG;
+            attr.val.clusterDim.y = 1;
+            attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            int most = 0;
+            if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess) (void)cudaGetLastError();
+            if (most > 0 && most < n) n = most;
         }
-        pairs[dev] = n < sm_count() / 2 ? n : sm_count() / 2;
+        blocks[dev] = n * CG;
     }
     // (the cluster shape is the kernel's own attribute)
-    return launch_dependent(fp8_grouped_gemm_kernel<UP>, 2 * pairs[dev], F8_THREADS, F8_SMEM_BYTES<UP>, stream, 1, tmA, tmB,
-                            tmO, g) == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
+    return launch_dependent(kernel, blocks[dev], F8_THREADS, smem, stream, 1, tmA, tmB, tmO, g) == cudaSuccess
+               ? MOMOE_OK : MOMOE_ERR_CUDA;
+}
+
+// Whether a CTA works on a tile of its own.
+static bool f8_single(const momoe_plan_t* p) {
+    return static_cast<long long>(p->M) * p->K <= F8_SINGLE_ROWS * static_cast<long long>(p->N);
 }
 
 int fp8_check_plan(const momoe_plan_t* p) {
@@ -526,7 +578,8 @@ MOMOE_API int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const uint8_t* x_sor
     g.a_scale = x_scale;
     g.b_scale = S1;
     g.h_scale = h_scale;
-    return f8_launch<true>(tmA, tmB, tmO, g, static_cast<cudaStream_t>(stream));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return f8_single(plan) ? f8_launch<true, 1>(tmA, tmB, tmO, g, st) : f8_launch<true, 2>(tmA, tmB, tmO, g, st);
 }
 
 MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
@@ -548,7 +601,7 @@ MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_so
     g.tile_expert = plan->tile_expert;
     g.pair_info = plan->pair_info;
     g.status = plan->status;
-    g.n_nblk = f8_cdiv(D, F8_PAIR_N);
+    g.n_nblk = f8_cdiv(D, F8_TILE_N);
     g.nkb = f8_cdiv(H, F8_K);
     g.out_cols = D;
     g.a_scale = h_scale;
@@ -556,5 +609,6 @@ MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_so
     g.b_blocks = f8_cdiv(D, 128);
     g.row_weight = plan->row_weight;
     g.y_scale = y_scale;
-    return f8_launch<false>(tmA, tmB, tmO, g, static_cast<cudaStream_t>(stream));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return f8_single(plan) ? f8_launch<false, 1>(tmA, tmB, tmO, g, st) : f8_launch<false, 2>(tmA, tmB, tmO, g, st);
 }
