@@ -294,21 +294,21 @@ int momoe_fp8_dispatch_rows(const void* x, const uint8_t* x_scale, const int32_t
 
 /* Up/gate GEMM + SwiGLU on 8-bit operands: a, b = x W1[e]^T (fp32), h = b sigmoid(b) a as 8-bit rows (rounded once, from
  * fp32).  W1 [N, 2H, D], S1 [N, 2, ceil(H / 128), ceil(D / 128)].  The second form streams the weights past a few rows an
- * expert.  Of the plan they read sched, tile_expert, pair_info (first form) and row_weight (down).  Padding rows of the
- * results are not defined.  D and H multiples of 16. */
-int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const uint8_t* x_sorted, const uint8_t* x_scale,
-                        const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
-                        momoe_stream_t stream);
+ * expert.  tile_rows: the real rows of each tile.  Of the plan they read sched, tile_expert, pair_info (first form) and
+ * row_weight (down).  Padding rows of the results are not defined.  D and H multiples of 16. */
+int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* x_sorted,
+                        const uint8_t* x_scale, const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted,
+                        uint8_t* h_scale, momoe_stream_t stream);
 int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* x_sorted,
-                               const uint8_t* x_scale, const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
-                               momoe_stream_t stream);
+                               const uint8_t* x_scale, const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted,
+                               uint8_t* h_scale, momoe_stream_t stream);
 
 /* Down GEMM on 8-bit operands: w[r] * (h[r, :] W2[e]^T) as y_sorted fp16 [rows, D] and y_scale fp32
  * [rows, ceil(D / 256)], a power of two for each (row, 256 columns); the value is their product.  W2 [N, D, H],
  * S2 [N, ceil(D / 128), ceil(H / 128)]. */
-int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
-                         const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, float* y_scale,
-                         momoe_stream_t stream);
+int momoe_fp8_down_scale(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* h_sorted,
+                         const uint8_t* h_scale, const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted,
+                         float* y_scale, momoe_stream_t stream);
 int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* h_sorted,
                                 const uint8_t* h_scale, const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted,
                                 float* y_scale, momoe_stream_t stream);

@@ -439,9 +439,9 @@ static int d8_launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const Fp8De
                             SPLIT, tmW, tmX, g) == cudaSuccess ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
 
-// Whether two CTAs share an item's k axis: when the items leave half of the SMs idle, and the k axis is long enough to pay for
-// the meeting.  Whole passes of one token, with the up GEMM shared and not: 18.5 / 18.3 us at 8 k slices, 20.5 / 20.4 at 12,
-// 20.6 / 22.4 at 16, 26.2 / 28.7 at 32 (H512, top-4 of 32), 39.0 / 47.0 at 56 (top-8 of 64).
+// Whether two CTAs share an item's k axis: when the items leave half of the SMs idle, and the k axis is long enough to pay
+// for the meeting.  Whole passes of one token, with the up GEMM shared and not: 18.5 / 18.3 us at 8 k slices, 20.5 / 20.4 at
+// 12, 20.6 / 22.4 at 16, 26.2 / 28.7 at 32 (H512, top-4 of 32), 39.0 / 47.0 at 56 (top-8 of 64).
 static bool d8_split(const momoe_plan_t* p, const Fp8DecArgs& g) {
     const long long msum = static_cast<long long>(p->M) * p->K;
     const long long tiles = msum / TILE_M + (msum < p->N ? msum : p->N);      // an upper bound
@@ -496,8 +496,8 @@ MOMOE_API int momoe_fp8_down_scale_decode(const momoe_plan_t* plan, const int32_
                                           float* y_scale, momoe_stream_t stream) {
     int rc = fp8_check_plan(plan);
     if (rc != MOMOE_OK) return rc;
-    if (tile_rows == nullptr || !d8_aligned(h_sorted) || !d8_aligned(h_scale) || !d8_aligned(W2_NDH) || S2 == nullptr || !d8_aligned(y_sorted) ||
-        y_scale == nullptr)
+    if (tile_rows == nullptr || !d8_aligned(h_sorted) || !d8_aligned(h_scale) || !d8_aligned(W2_NDH) || S2 == nullptr ||
+        !d8_aligned(y_sorted) || y_scale == nullptr)
         return MOMOE_ERR_ARG;
     const int D = plan->D, H = plan->H;
     CUtensorMap tmW, tmX;

@@ -520,12 +520,12 @@ MOMOE_API int momoe_fp8_experts_forward(const void* x_MD, const uint8_t* x_scale
     if (rc != MOMOE_OK) return rc;
     // with few rows an expert, the kernels that stream the weights
     const bool decode = static_cast<int64_t>(M) * K <= static_cast<int64_t>(stream_max_avg_rows) * N;
-    rc = decode ? momoe_fp8_up_swiglu_decode(&plan, i32(l.tile_rows), u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream)
-                : momoe_fp8_up_swiglu(&plan, u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream);
+    const auto up = decode ? momoe_fp8_up_swiglu_decode : momoe_fp8_up_swiglu;
+    const auto down = decode ? momoe_fp8_down_scale_decode : momoe_fp8_down_scale;
+    rc = up(&plan, i32(l.tile_rows), u8(l.rows), u8(l.x_scale), W1_N2HD, S1, u8(l.h), u8(l.h_scale), stream);
     if (rc != MOMOE_OK) return rc;
     float* y_scale = reinterpret_cast<float*>(ws + l.y_scale);
-    rc = decode ? momoe_fp8_down_scale_decode(&plan, i32(l.tile_rows), u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, y_scale, stream)
-                : momoe_fp8_down_scale(&plan, u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, y_scale, stream);
+    rc = down(&plan, i32(l.tile_rows), u8(l.h), u8(l.h_scale), W2_NDH, S2, ws + l.rows, y_scale, stream);
     if (rc != MOMOE_OK) return rc;
     // launched early beside the tile kernel its blocks wait there for long and slow it down (1124 against 1098 us at 16384
     // tokens, D2048 H1024, top-8 of 128); behind the streaming kernel it saves a launch gap (30.7 against 32.5 us, 1 token)

@@ -7,9 +7,16 @@
 // so the tensor core applies them (kind::mxf8f6f4, block-scaled): accumulation is fp32 over the whole k axis and there is
 // no per-block pass over the accumulators, which fp32 scales would need.
 //
-// Tensor-bound at large row counts.  The structure is that of the 16-bit grouped GEMM: a CTA pair computes 256 x 256, each
-// CTA loads its 128 rows of A and half of B, ring of 3 stages of two 128-byte k slices (a slice is 128 values here), warp
-// 0 loads, warp 1 of the leader issues the MMAs, warps 2..9 are the epilogue.  What differs:
+// Bound at large row counts by the tensor pipe at the clock that the power limit leaves and by the tiles' way out of L2, 10
+// TB/s at 16384 tokens (D2048 H1024, top-8 of 128: up 2.3, down 1.9 PFLOP/s).  The structure is that of the 16-bit grouped
+// GEMM: a CTA pair computes 256 x 256, each CTA loads its 128 rows of A and half of B, ring of 3 stages of two 128-byte k
+// slices (a slice is 128 values here), warp 0 loads, warp 1 of the leader issues the MMAs, warps 2..9 are the epilogue.
+//
+// With few rows an expert the second tile of a pair is mostly missing and half of its MMAs and A loads are for nothing.
+// Then (CG = 1) a CTA computes 128 x 256 by itself, in 4 stages of one slice, and loads the 32-row blocks of A that hold
+// real rows.  It takes half as many loads of B more, 48 KiB a slice for 128 rows against 64 KiB for 256.
+//
+// What differs from the 16-bit kernel:
 //
 // Scales.  Warps 10..13 of each CTA (one for each TMEM lane quarter) write the scales of four slices (512 k) straight into
 // TMEM: 4 columns for the CTA's 128 rows, 8 for the 256 weight columns (one word each, repeated).  The MMAs of the four
@@ -51,7 +58,6 @@ template <bool UP>
 constexpr int F8_PIECES = UP ? 1 : 2;                     // pieces an epilogue warp has
 template <bool UP, int CG>
 constexpr int F8_SMEM_BYTES = F8_STAGES<CG> * F8_STAGE_BYTES<CG> + F8_EPI_WARPS * F8_PIECES<UP> * F8_PIECE + 1024;
-constexpr long long F8_SINGLE_ROWS = 128;
 constexpr int F8_ACC1 = 224;                              // first column of the second accumulator
 constexpr int F8_SF_COL = 480;
 constexpr int F8_SF_COLS = 12;                            // 4 for A, 8 for B
@@ -60,6 +66,7 @@ struct Fp8Args {
     const int* sched;
     const int* tile_expert;
     const int* pair_info;
+    const int* tile_rows;
     int* status;
     int n_nblk;                 // column blocks of 128 (up, both halves) or 256 (down)
     int nkb;                    // k slices
@@ -80,7 +87,7 @@ __device__ __forceinline__ float f8_swiglu(float a, float b) { return b * __fdiv
 
 struct Fp8Work {
     int tile, nb, e;
-    bool valid;
+    int rows;          // the tile's real rows, which come first; pairs: TILE_M, or 0 for a missing second tile
 };
 template <int CG>
 __device__ __forceinline__ Fp8Work f8_work(const Fp8Args& g, int item, uint32_t cta_rank) {
@@ -89,11 +96,11 @@ __device__ __forceinline__ Fp8Work f8_work(const Fp8Args& g, int item, uint32_t 
     if constexpr (CG == 2) {
         const int info = __ldcg(g.pair_info + item / g.n_nblk);
         w.tile = (info >> 1) + static_cast<int>(cta_rank);
-        w.valid = cta_rank == 0 || (info & 1) != 0;
+        w.rows = cta_rank == 0 || (info & 1) != 0 ? TILE_M : 0;
         w.e = __ldcg(g.tile_expert + (info >> 1));
     } else {
         w.tile = item / g.n_nblk;
-        w.valid = true;
+        w.rows = __ldcg(g.tile_rows + w.tile);
         w.e = __ldcg(g.tile_expert + w.tile);
     }
     return w;
@@ -126,7 +133,7 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     __shared__ uint64_t bar_ovl;                     // leader: the shared columns of the latest tile have been read
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
-    __shared__ uint32_t s_top[UP ? 2 : 1][UP ? 2 : 1][UP ? TILE_M : 1];   // up: [accumulator][column half][row]
+    __shared__ uint32_t s_top[UP ? 2 : 1][UP ? 2 : 1][UP ? TILE_M : 1];   // up: [meeting][column half][row]
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -186,10 +193,14 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
             const int r = static_cast<int>(cta_rank);
             for (int item = cluster_id; ok && item < total_items; item += n_clusters) {
                 const Fp8Work w = f8_work<CG>(g, item, cta_rank);
+                // of a tile of its own a CTA loads the blocks of 32 rows that hold real ones: the rest of a stage holds
+                // what it held before, and so do the rows of the accumulator that nothing reads
+                const int blocks = CG == 2 ? 4 : (w.rows + 31) >> 5;
+                const uint32_t bytes = CG == 2 ? 2 * STAGE_BYTES : SLICE_BYTES - (4 - blocks) * (F8_A_BYTES / 4);
                 for (int kb = 0; kb < g.nkb; kb += SLICES) {
                     ok = mbar_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, abortp, g.status, DEV_TIMEOUT_PRODUCER);
                     if (!ok) break;
-                    if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[stage]), CG * STAGE_BYTES);
+                    if (leader) mbar_arrive_expect_tx(smem_u32(&bar_full[stage]), bytes);
                     const uint32_t full = f8_lead<CG>(smem_u32(&bar_full[stage]));
                     // tensor maps count in 16-bit units; a slice past the end of the k axis is zero-filled
 #pragma unroll
@@ -203,7 +214,8 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                             if constexpr (UP) tma_load_3d_pair(sa + F8_A_BYTES, &tmB, full, k0, w.nb * 128, w.e * 2 + r);
                             else tma_load_3d_pair(sa + F8_A_BYTES, &tmB, full, k0, w.nb * F8_TILE_N + r * 128, w.e);
                         } else {
-                            tma_load_2d(sa, &tmA, full, k0, w.tile * TILE_M);
+                            for (int i = 0; i < blocks; ++i)
+                                tma_load_2d(sa + i * (F8_A_BYTES / 4), &tmA, full, k0, w.tile * TILE_M + i * 32);
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 const uint32_t sb = sa + F8_A_BYTES + i * 128 * F8_K;
@@ -281,7 +293,7 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const uint32_t sf0 = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + F8_SF_COL;
         for (int item = cluster_id; ok && item < total_items; item += n_clusters) {
             const Fp8Work w = f8_work<CG>(g, item, cta_rank);
-            const int tile = w.valid ? w.tile : w.tile - 1;     // a missing half reads its partner's scales
+            const int tile = w.rows > 0 ? w.tile : w.tile - 1;     // a missing half reads its partner's scales
             const uint4* src = reinterpret_cast<const uint4*>(g.a_scale + static_cast<size_t>(tile) * n_groups * FP8_ATOM);
             // the two blocks of 128 weight columns of this item
             const int i = (lane >> 2) & 1;
@@ -328,6 +340,7 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const uint32_t stage_area = epi_base + (warp - 2) * PIECES * F8_PIECE;
         int it = 0;
         bool ok = true;
+        int meet = 0;                      // up: meetings with the warp of the other column half so far
         int n_stored = 0;                  // pieces handed to TMA stores so far (lane 0 owns the bulk groups)
         for (int item = cluster_id; ok && item < total_items; item += n_clusters, ++it) {
             const Fp8Work w = f8_work<CG>(g, item, cta_rank);
@@ -345,10 +358,11 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + ab * static_cast<uint32_t>(sizeof(uint64_t)));
             };
+            const bool live = q * 32 < w.rows;         // this warp has real rows
             float wgt = 0.0f;
             const size_t grow = static_cast<size_t>(w.tile) * TILE_M + row;
             if constexpr (!UP) {
-                if (w.valid) {
+                if (live) {
                     wgt = __ldcg(g.row_weight + grow);
                     const int n0 = w.nb * 2;
                     const int e = fp8_row_exponent(g.a_scale + fp8_atom_offset(grow, 0, n_groups),
@@ -367,6 +381,11 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 break;
             }
             tc_fence_after();
+            if (CG == 1 && !live) {
+                if (shares) hand_back_shared();
+                hand_back_all();
+                continue;
+            }
             if constexpr (UP) {
                 // columns 32c .. 32c + 31 of the block, first the chunk that touches the shared columns
                 const int s0 = half;                     // position of the first chunk inside this warp's 64 columns
@@ -392,15 +411,16 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 uint32_t top = 0u;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) top = max(top, max(abs_bits(h0[i]), abs_bits(h1[i])));
-                s_top[ab][half][row] = top;
-                // two warps share a row's 128 columns; s_top[ab] is written again two tiles later, after the partner has
-                // passed the next meeting, i.e. after it has read this one
+                s_top[meet & 1][half][row] = top;
+                // two warps share a row's 128 columns; this half of s_top is written again two meetings later, after the
+                // partner has been at the next one, i.e. after it has read this one
                 asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
-                top = max(top, s_top[ab][half ^ 1][row]);
+                top = max(top, s_top[meet & 1][half ^ 1][row]);
+                ++meet;
                 const uint32_t byte = fp8_scale_byte(top);
                 const float inv = fp8_inv_scale(byte);
                 const int col0 = w.nb * 128 + half * 64;
-                if (w.valid) {
+                if (CG == 1 || live) {
                     if (half == 0)
                         g.h_scale[fp8_atom_offset(grow, w.nb >> 2, (g.n_nblk + 3) >> 2) + (w.nb & 3)] =
                             static_cast<uint8_t>(byte);
@@ -446,7 +466,7 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     if (i == 0 && shares) hand_back_shared();
                     if (i == 3) hand_back_all();
                     const int col0 = w.nb * F8_TILE_N + c * 32;
-                    if (w.valid && col0 < g.out_cols) {
+                    if ((CG == 1 || live) && col0 < g.out_cols) {
                         const uint32_t slot = stage_area + n_stored % PIECES * F8_PIECE;
                         if (n_stored >= PIECES && lane == 0) bulk_wait_read<PIECES - 1>();
                         __syncwarp();
@@ -528,7 +548,12 @@ static int f8_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUten
                ? MOMOE_OK : MOMOE_ERR_CUDA;
 }
 
-// Whether a CTA works on a tile of its own.
+// Whether a CTA works on a tile of its own: up to F8_SINGLE_ROWS rows an expert on average.  Whole passes in us, on tiles of
+// their own and in pairs:  rows an expert       48          128          192          256          384
+//   D2176 H1152, top-6 of 64                113 / 130    142 / 156    190 / 199    233 / 219    325 / 277
+//   D2048 H1024, top-8 of 128               178 / 237    221 / 250    289 / 292    376 / 375    507 / 450
+//   D7168 H2048, top-4 of 32                265 / 319    365 / 418    480 / 458    578 / 600    810 / 683
+constexpr long long F8_SINGLE_ROWS = 192;
 static bool f8_single(const momoe_plan_t* p) {
     return static_cast<long long>(p->M) * p->K <= F8_SINGLE_ROWS * static_cast<long long>(p->N);
 }
@@ -544,7 +569,9 @@ int fp8_check_plan(const momoe_plan_t* p) {
 }
 
 static inline int f8_cdiv(int a, int b) { return (a + b - 1) / b; }
-static inline bool f8_aligned(const void* p, uintptr_t n) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+static inline bool f8_aligned(const void* p, uintptr_t n) {
+    return p != nullptr && (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
+}
 
 }  // namespace momoe
 
@@ -552,17 +579,19 @@ using namespace momoe;
 
 #define MOMOE_API extern "C" __attribute__((visibility("default")))
 
-MOMOE_API int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const uint8_t* x_sorted, const uint8_t* x_scale,
-                                  const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted, uint8_t* h_scale,
-                                  momoe_stream_t stream) {
+MOMOE_API int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* x_sorted,
+                                  const uint8_t* x_scale, const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted,
+                                  uint8_t* h_scale, momoe_stream_t stream) {
     int rc = fp8_check_plan(plan);
     if (rc != MOMOE_OK) return rc;
-    if (!f8_aligned(x_sorted, 16) || !f8_aligned(x_scale, 16) || !f8_aligned(W1_N2HD, 16) || S1 == nullptr ||
-        !f8_aligned(h_sorted, 16) || !f8_aligned(h_scale, 16))
+    if (tile_rows == nullptr || !f8_aligned(x_sorted, 16) || !f8_aligned(x_scale, 16) || !f8_aligned(W1_N2HD, 16) ||
+        S1 == nullptr || !f8_aligned(h_sorted, 16) || !f8_aligned(h_scale, 16))
         return MOMOE_ERR_ARG;
     const int D = plan->D, H = plan->H;
     CUtensorMap tmA, tmB, tmO;
-    if ((rc = encode_tmap_2d(&tmA, x_sorted, plan->rows_capacity, D / 2, TILE_M, F8_K / 2)) != MOMOE_OK) return rc;
+    const bool single = f8_single(plan);
+    if ((rc = encode_tmap_2d(&tmA, x_sorted, plan->rows_capacity, D / 2, single ? 32 : TILE_M, F8_K / 2)) != MOMOE_OK)
+        return rc;
     if ((rc = encode_tmap_3d(&tmB, W1_N2HD, static_cast<uint64_t>(plan->N) * 2, H, D / 2, 128, F8_K / 2)) != MOMOE_OK)
         return rc;
     if ((rc = encode_tmap_2d(&tmO, h_sorted, plan->rows_capacity, H / 2, 32, 32, TMAP_SWIZZLE_64B)) != MOMOE_OK) return rc;
@@ -571,6 +600,7 @@ MOMOE_API int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const uint8_t* x_sor
     g.sched = plan->sched;
     g.tile_expert = plan->tile_expert;
     g.pair_info = plan->pair_info;
+    g.tile_rows = tile_rows;
     g.status = plan->status;
     g.n_nblk = f8_cdiv(H, 128);
     g.nkb = f8_cdiv(D, F8_K);
@@ -579,20 +609,22 @@ MOMOE_API int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const uint8_t* x_sor
     g.b_scale = S1;
     g.h_scale = h_scale;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return f8_single(plan) ? f8_launch<true, 1>(tmA, tmB, tmO, g, st) : f8_launch<true, 2>(tmA, tmB, tmO, g, st);
+    return single ? f8_launch<true, 1>(tmA, tmB, tmO, g, st) : f8_launch<true, 2>(tmA, tmB, tmO, g, st);
 }
 
-MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_sorted, const uint8_t* h_scale,
-                                   const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted, float* y_scale,
-                                   momoe_stream_t stream) {
+MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* h_sorted,
+                                   const uint8_t* h_scale, const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted,
+                                   float* y_scale, momoe_stream_t stream) {
     int rc = fp8_check_plan(plan);
     if (rc != MOMOE_OK) return rc;
-    if (!f8_aligned(h_sorted, 16) || !f8_aligned(h_scale, 16) || !f8_aligned(W2_NDH, 16) || S2 == nullptr ||
-        !f8_aligned(y_sorted, 16) || y_scale == nullptr)
+    if (tile_rows == nullptr || !f8_aligned(h_sorted, 16) || !f8_aligned(h_scale, 16) || !f8_aligned(W2_NDH, 16) ||
+        S2 == nullptr || !f8_aligned(y_sorted, 16) || y_scale == nullptr)
         return MOMOE_ERR_ARG;
     const int D = plan->D, H = plan->H;
     CUtensorMap tmA, tmB, tmO;
-    if ((rc = encode_tmap_2d(&tmA, h_sorted, plan->rows_capacity, H / 2, TILE_M, F8_K / 2)) != MOMOE_OK) return rc;
+    const bool single = f8_single(plan);
+    if ((rc = encode_tmap_2d(&tmA, h_sorted, plan->rows_capacity, H / 2, single ? 32 : TILE_M, F8_K / 2)) != MOMOE_OK)
+        return rc;
     if ((rc = encode_tmap_3d(&tmB, W2_NDH, plan->N, D, H / 2, 128, F8_K / 2)) != MOMOE_OK) return rc;
     if ((rc = encode_tmap_2d(&tmO, y_sorted, plan->rows_capacity, D, 32, 32, TMAP_SWIZZLE_64B)) != MOMOE_OK) return rc;
     Fp8Args g;
@@ -600,6 +632,7 @@ MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_so
     g.sched = plan->sched;
     g.tile_expert = plan->tile_expert;
     g.pair_info = plan->pair_info;
+    g.tile_rows = tile_rows;
     g.status = plan->status;
     g.n_nblk = f8_cdiv(D, F8_TILE_N);
     g.nkb = f8_cdiv(H, F8_K);
@@ -610,5 +643,5 @@ MOMOE_API int momoe_fp8_down_scale(const momoe_plan_t* plan, const uint8_t* h_so
     g.row_weight = plan->row_weight;
     g.y_scale = y_scale;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return f8_single(plan) ? f8_launch<false, 1>(tmA, tmB, tmO, g, st) : f8_launch<false, 2>(tmA, tmB, tmO, g, st);
+    return single ? f8_launch<false, 1>(tmA, tmB, tmO, g, st) : f8_launch<false, 2>(tmA, tmB, tmO, g, st);
 }

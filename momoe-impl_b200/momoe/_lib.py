@@ -83,9 +83,9 @@ _PROTOS = {
     "momoe_fp8_dispatch_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
     "momoe_fp8_dispatch_rows": (C.c_int, [c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
                                           c_vp, c_vp, c_i64, c_vp, c_sz, c_vp, c_vp, c_vp, c_vp]),
-    "momoe_fp8_up_swiglu": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "momoe_fp8_up_swiglu": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "momoe_fp8_up_swiglu_decode": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
-    "momoe_fp8_down_scale": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "momoe_fp8_down_scale": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "momoe_fp8_down_scale_decode": (C.c_int, [PlanP, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "momoe_fp8_combine_rows": (C.c_int, [c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_vp, c_vp]),
     "momoe_fp8_experts_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32]),

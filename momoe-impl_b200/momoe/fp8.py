@@ -14,9 +14,9 @@ from ._lib import as_rows, lib, native, on_device, pitch, ptr, raw_stream
 
 BLOCK = 128                      # values that share a scale
 # Calls with at most this many rows per expert on average stream the weights past the rows; more take the row-tile kernels.
-# Whole passes, streaming against tiles: 175 / 203 us at 32 rows, 224 / 214 at 48 (D2048 H1024, top-8 of 128); 120 / 131 and
-# 145 / 134 us (D2176 H1152, top-6 of 64).
-STREAM_MAX_AVG_ROWS = 40
+# Whole passes, streaming against tiles: one token 24.7 / 26.7 us, 1 row an expert 86 / 90, 4 rows 125 / 127, 8 rows 131.5 /
+# 131.9, 12 rows 151 / 145, 24 rows 166 / 154 (D2048 H1024, top-8 of 128).
+STREAM_MAX_AVG_ROWS = 8
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 

@@ -19,6 +19,7 @@ SHAPES = [
     (37, 6, 3, 144, 272, 0.0),        # ragged in both widths
     (70, 2, 1, 512, 640, 0.0),        # more than one 32-row block
     (300, 4, 2, 528, 400, 1.0),
+    (900, 4, 1, 656, 400, 0.5),       # enough rows an expert for pairs of tiles
     (1000, 16, 4, 640, 1152, 2.0),    # skewed: empty experts, experts of many tiles
     (257, 3, 1, 2176, 128, 0.0),
     (129, 1, 1, 128, 4096, 0.0),
@@ -174,12 +175,12 @@ class Stages:
     def gemms(self, e, stream):
         import ctypes
         ref, p, L = ctypes.byref(self.c), self.ptr, self.lib
-        up, down = L.momoe_fp8_up_swiglu, L.momoe_fp8_down_scale
-        if stream:
-            up = lambda plan, *rest: L.momoe_fp8_up_swiglu_decode(plan, p(self.tile_rows), *rest)
-            down = lambda plan, *rest: L.momoe_fp8_down_scale_decode(plan, p(self.tile_rows), *rest)
-        self.check(up(ref, p(self.xs), p(self.xsc), p(e.W1_N2HD), p(e.S1), p(self.hs), p(self.hsc), self.st), "up")
-        self.check(down(ref, p(self.hs), p(self.hsc), p(e.W2_NDH), p(e.S2), p(self.ys), p(self.yscale), self.st), "down")
+        up = L.momoe_fp8_up_swiglu_decode if stream else L.momoe_fp8_up_swiglu
+        down = L.momoe_fp8_down_scale_decode if stream else L.momoe_fp8_down_scale
+        rows = p(self.tile_rows)
+        self.check(up(ref, rows, p(self.xs), p(self.xsc), p(e.W1_N2HD), p(e.S1), p(self.hs), p(self.hsc), self.st), "up")
+        self.check(down(ref, rows, p(self.hs), p(self.hsc), p(e.W2_NDH), p(e.S2), p(self.ys), p(self.yscale), self.st),
+                   "down")
 
     def combine(self):
         y = torch.empty(self.M, self.D, dtype=torch.bfloat16, device="cuda")

@@ -68,7 +68,7 @@ def test_fp8_arguments(lib):
     plan = lib.Plan(M=4, N=8, K=2, D=72, H=32, reserved=0, rows_capacity=128 * 9, sched=16, tile_expert=16,
                     pad_off=16, row_token=16, row_weight=16, pos_MK=16, status=16, pair_info=16)
     p = C.byref(plan)
-    assert L.momoe_fp8_up_swiglu(p, ONE, ONE, ONE, ONE, ONE, ONE, None) == -2    # D not a multiple of 16
+    assert L.momoe_fp8_up_swiglu(p, ONE, ONE, ONE, ONE, ONE, ONE, ONE, None) == -2    # D not a multiple of 16
     plan.D = 64
     def dispatch(x=ONE, M=4, N=8, K=2, D=64, rows=128 * 9, ws=ONE, n=None, dst=ONE):
         n = L.momoe_fp8_dispatch_workspace_bytes(M, N, K) if n is None else n
@@ -80,17 +80,17 @@ def test_fp8_arguments(lib):
     assert dispatch(M=8 << 20, rows=1 << 40) == -4                               # more tiles than a table entry counts
     assert L.momoe_fp8_dispatch_workspace_bytes(4, 8, 2) == 0
     assert L.momoe_fp8_dispatch_workspace_bytes(20000, 8, 2) > 8 * 4
-    stream = lambda f: lambda plan, *rest: f(plan, ONE, *rest)
-    for f in (L.momoe_fp8_up_swiglu, stream(L.momoe_fp8_up_swiglu_decode)):
-        assert f(p, ONE, ONE, ONE, None, ONE, ONE, None) == -1 and f(p, ODD, ONE, ONE, ONE, ONE, ONE, None) == -1
-        assert f(None, ONE, ONE, ONE, ONE, ONE, ONE, None) == -1
-    for f in (L.momoe_fp8_down_scale, stream(L.momoe_fp8_down_scale_decode)):
-        assert f(p, ONE, ONE, ONE, None, ONE, ONE, None) == -1 and f(p, ONE, ONE, ONE, ONE, None, ONE, None) == -1
-        assert f(p, ONE, ONE, ONE, ONE, ONE, None, None) == -1 and f(p, ONE, ONE, ONE, ONE, ODD, ONE, None) == -1
+    for f in (L.momoe_fp8_up_swiglu, L.momoe_fp8_up_swiglu_decode):
+        assert f(p, ONE, ONE, ONE, ONE, None, ONE, ONE, None) == -1 and f(p, ONE, ODD, ONE, ONE, ONE, ONE, ONE, None) == -1
+        assert f(None, ONE, ONE, ONE, ONE, ONE, ONE, ONE, None) == -1
+    for f in (L.momoe_fp8_down_scale, L.momoe_fp8_down_scale_decode):
+        assert f(p, ONE, ONE, ONE, ONE, None, ONE, ONE, None) == -1 and f(p, ONE, ONE, ONE, ONE, ONE, None, ONE, None) == -1
+        assert f(p, ONE, ONE, ONE, ONE, ONE, ONE, None, None) == -1 and f(p, ONE, ONE, ONE, ONE, ONE, ODD, ONE, None) == -1
     assert L.momoe_fp8_combine_rows(ONE, ONE, ONE, 4, 2, 60, ONE, None) == -2
     assert L.momoe_fp8_combine_rows(ONE, ONE, ONE, 4, 0, 64, ONE, None) == -1
     assert L.momoe_fp8_combine_rows(ODD, ONE, ONE, 4, 2, 64, ONE, None) == -1
-    assert L.momoe_fp8_up_swiglu_decode(p, None, ONE, ONE, ONE, ONE, ONE, ONE, None) == -1
+    for f in (L.momoe_fp8_up_swiglu, L.momoe_fp8_up_swiglu_decode, L.momoe_fp8_down_scale, L.momoe_fp8_down_scale_decode):
+        assert f(p, None, ONE, ONE, ONE, ONE, ONE, ONE, None) == -1
     def whole(M=4, N=8, K=2, D=64, H=32, x=ONE, ws=ONE, n=None):
         n = L.momoe_fp8_experts_workspace_bytes(M, N, K, D, H) if n is None else n
         return L.momoe_fp8_experts_forward(x, None, ONE, ONE, M, N, K, D, H, ONE, ONE, ONE, ONE, 16, ONE, ONE, ws, n, ONE,
