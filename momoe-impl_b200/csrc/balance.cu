@@ -13,7 +13,9 @@
 // Bound by HBM for large batches (the logits are read once in each direction and the gradient written once) and by the
 // launches for small ones.  Forward, two launches: blocks of rows leave partial sums, one slot for each (row block,
 // sequence) that meet; then the slots of a sequence are added in a fixed order, 32 experts a block, and the last block
-// to finish adds the blocks' shares of the loss, also in a fixed order: no result depends on timing.
+// to finish adds the blocks' shares of the loss, also in a fixed order: no result depends on timing.  At 65521 rows of 256
+// logits in 37 sequences the partial sums take 21 us, their sum 7 and the gradient 26, against 16 us for the bytes alone:
+// a row costs an exponential a logit and two reductions across its lanes in each direction.  At 1024 x 32: 3.7, 5.7, 2.9.
 #include <cmath>
 
 #include "internal.h"
