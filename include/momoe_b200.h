@@ -234,7 +234,8 @@ int momoe_bias_update(float* biases_N, const int64_t* sizes_N, int32_t N, int32_
  *   residual and r: both NULL (then r is x) or both non-NULL; r [M, D] contiguous, rounded to `type`
  *   y [M, D] contiguous in `type`, or NULL;  q [M, D], scale [M, ceil(D / 128)]: y before its rounding as 8-bit rows, or
  *   both NULL (one of y and q is needed);  rstd fp32 [M] or NULL: 1 / sqrt(mean(r^2) + eps)
- *   weight [D] in `type` or fp32 (weight_type).  D a multiple of 8, at most 16384.  M = 0 does nothing. */
+ *   weight [D] in `type` or fp32 (weight_type).  D a multiple of 8, at most 16384; M at most 2^30 (0 does
+ *   nothing). */
 int momoe_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
                    int32_t type, int32_t weight_type, int32_t M, int32_t D, float eps, void* r, void* y, float* rstd,
                    uint8_t* q, uint8_t* scale, momoe_stream_t stream);
@@ -258,8 +259,8 @@ int momoe_quantize_rows(const void* x, int64_t x_stride, int32_t type, int32_t M
  * the Ng = N - Ks gating logits, T_b a sequence's tokens, T all tokens and B' the sequences that are not empty:
  *   loss = balance_coef / B' * sum_b sum_e [Ng / ((K - Ks) T_b) count[b, e]] [mean over b of p[., e]]
  *        + z_coef / T * sum_t (log sum_e exp logit[t, e])^2
- * loss fp32 [1]; counts_BN int64 [B, N]; grad_BN fp32 [B, N]: for the backward pass.  N <= 1024, B <= 65535.
- * Deterministic.  Replaces nothing: the reference balances by bias only (momoe/sample_moe.py:64-66). */
+ * loss fp32 [1]; counts_BN int64 [B, N]; grad_BN fp32 [B, N]: for the backward pass.  N <= 1024, B <= 65535,
+ * M <= 2^30.  Deterministic.  Replaces nothing: the reference balances by bias only (momoe/sample_moe.py:64-66). */
 size_t momoe_balance_loss_workspace_bytes(int32_t M, int32_t N, int32_t B);
 int momoe_balance_loss(const void* logits_MN, int32_t type, const int32_t* topk_idx_MK, const int32_t* cu_seqlens,
                        int32_t seq_len, int32_t M, int32_t N, int32_t K, int32_t Ks, int32_t B, float balance_coef,

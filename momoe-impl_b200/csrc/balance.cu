@@ -405,7 +405,8 @@ static BalLayout bal_layout(int M, int N, int B) {
 static int bal_check(int32_t M, int32_t N, int32_t Ks, int32_t B, int32_t type) {
     if (M < 0 || N <= 0 || Ks < 0 || Ks >= N || B <= 0) return MOMOE_ERR_ARG;
     if (type != 0 && type != 2) return MOMOE_ERR_UNSUPPORTED;
-    if (N > BAL_MAX_EXPERTS || B > 65535) return MOMOE_ERR_TOO_LARGE;
+    // row numbers stay inside 32 bits, with room for a step past the last row
+    if (N > BAL_MAX_EXPERTS || B > 65535 || M > 1 << 30) return MOMOE_ERR_TOO_LARGE;
     return MOMOE_OK;
 }
 
@@ -444,8 +445,9 @@ MOMOE_API size_t momoe_balance_loss_workspace_bytes(int32_t M, int32_t N, int32_
 
 MOMOE_API int momoe_balance_loss(const void* logits_MN, int32_t type, const int32_t* topk_idx_MK,
                                  const int32_t* cu_seqlens, int32_t seq_len, int32_t M, int32_t N, int32_t K,
-                                 int32_t Ks, int32_t B, float balance_coef, float z_coef, float* loss, int64_t* counts_BN, float* grad_BN,
-                                 void* workspace, size_t workspace_bytes, momoe_stream_t stream) {
+                                 int32_t Ks, int32_t B, float balance_coef, float z_coef, float* loss,
+                                 int64_t* counts_BN, float* grad_BN, void* workspace, size_t workspace_bytes,
+                                 momoe_stream_t stream) {
     int rc = bal_check(M, N, Ks, B, type);
     if (rc != MOMOE_OK) return rc;
     if (M == 0 || K <= Ks || K > N || !bal_uniform(cu_seqlens, seq_len, M, B)) return MOMOE_ERR_ARG;

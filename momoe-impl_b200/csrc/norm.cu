@@ -23,6 +23,7 @@ namespace momoe {
 
 constexpr int NORM_MAX_THREADS = 512;
 constexpr int NORM_MAX_D = NORM_MAX_THREADS * 4 * 8;
+constexpr int NORM_MAX_M = 1 << 30;          // row numbers stay inside 32 bits, with room for a step past the last row
 
 // How a row of n chunks is shared out: chunks a thread holds, threads of a row, rows of a block.
 struct NormShape {
@@ -365,7 +366,7 @@ static int norm_check(int32_t M, int32_t D, int32_t type, int32_t weight_type) {
     if (M < 0 || D <= 0) return MOMOE_ERR_ARG;
     if (type < 0 || type > 2 || (weight_type != type && weight_type != 2)) return MOMOE_ERR_UNSUPPORTED;
     if (D % 8 != 0) return MOMOE_ERR_UNSUPPORTED;
-    if (D > NORM_MAX_D) return MOMOE_ERR_TOO_LARGE;
+    if (D > NORM_MAX_D || M > NORM_MAX_M) return MOMOE_ERR_TOO_LARGE;
     return MOMOE_OK;
 }
 

@@ -109,3 +109,12 @@ def test_there_is_no_cpu_path(lib):
                  lambda: norm.RMSNorm(64, device="cpu")(x.bfloat16())):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def test_row_numbers_stay_inside_32_bits(lib):
+    """Kernels step past the last row before they compare, so the largest row counts are refused."""
+    L, M = lib.lib, 2 ** 30 + 1
+    assert L.momoe_rms_norm(ONE, 8, None, 0, ONE, 0, 0, M, 8, 1e-6, None, ONE, None, None, None, None) == -4
+    assert L.momoe_rms_norm_backward(ONE, None, ONE, 8, ONE, ONE, 0, 0, M, 8, ONE, None, None, 0, None) == -4
+    assert L.momoe_balance_loss(ONE, 0, ONE, None, M, M, 8, 2, 0, 1, 1.0, 0.0, ONE, ONE, ONE, ONE, 1 << 40, None) == -4
+    assert L.momoe_balance_loss_backward(ONE, 0, None, M, ONE, M, 8, 0, 1, 0.0, ONE, None, ONE, None) == -4
