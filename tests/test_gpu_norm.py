@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 F32 = 2.0 ** -17
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 SHAPES = [(1, 8), (3, 136), (257, 1024), (5, 1032), (130, 2176), (1, 4096), (33, 4104), (7, 8192), (4, 8200), (2, 16384),
-          (5000, 64)]
+          (5000, 64), (1000, 2048), (400, 7176)]        # the last three: several rows for each group of the backward pass
 
 
 @pytest.fixture(scope="module")
