@@ -12,7 +12,7 @@
 // to a warp up to 512 columns and to a thread block above; a thread holds 2 chunks of 8 columns (4 above 8192 columns), so
 // that a block has few idle threads at widths between powers of two and enough blocks fit an SM to keep 60 KiB and more
 // in flight.  Sums are 32-bit.  Of the measured copy rate: 8-bit output 0.94 (8192 x 7168 bf16, 86 us), forward 0.98 and
-// backward 0.84 without its 4.5 us of partial sums (16384 x 2048 bf16, 42 and 49 us).
+// backward 0.84 without its 4.5 us of partial sums (16384 x 2048 bf16, 42 and 48 us).
 #include <cmath>
 
 #include "fp8.cuh"
