@@ -9,6 +9,8 @@ the dense router backward are never materialised.  `MoE.fused = False` restores 
 Two things the reference does not have are switched on by attributes: `balance_coef` / `z_coef` add the router's balance
 loss and z-loss (`momoe.balance`; the value is `MoE.aux_loss`, to be added to the training loss), and `quantize_experts()`
 makes forward-only calls run the experts in 8 bits (`momoe.fp8`)."""
+import weakref
+
 import torch
 import torch.nn as nn
 
@@ -95,7 +97,7 @@ class MoE(nn.Module):
     z_coef = 0.0           # weight of the z-loss
     aux_loss = None        # their sum of the latest forward pass, float32 [], differentiable; None if both are 0
     experts_fp8 = None     # 8-bit weights of forward-only calls, from quantize_experts()
-    _fp8_versions = None
+    _fp8_weights = None    # the weights that experts_fp8 stands for, with their versions; (): none of this layer's
 
     def __init__(self, embedding_dim, intermediate_dim, num_experts, num_chosen_experts, num_shared_experts,
                  save_percent=0, bias_update_rate=1e-4, Wg_DN: torch.Tensor | None = None,
@@ -123,23 +125,37 @@ class MoE(nn.Module):
     def __getstate__(self):
         state = dict(self.__dict__)
         state.pop("aux_loss", None)         # belongs to the graph of a forward pass, not to a copy of the layer
-        state.pop("_fp8_versions", None)    # a copy's parameters count their versions anew
+        # a copy has weights of its own, for which its 8-bit ones stand if they stand for this layer's
+        state["_fp8_weights"] = None if self.experts_fp8 is None or self._fp8_fresh() else ()
         return state
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if self.experts_fp8 is not None:
+            self._fp8_fresh()
+
+    def _fp8_fresh(self):
+        """Whether the 8-bit weights stand for the layer's weights as they are; ones that were set by hand do from the first
+        look on."""
+        weights = self.momoe.Wl1_ND2H, self.momoe.Wl2_NHD
+        if self._fp8_weights is None:
+            self._fp8_weights = tuple((weakref.ref(w), w._version) for w in weights)
+        return len(self._fp8_weights) == 2 and all(ref() is w and version == w._version
+                                                   for (ref, version), w in zip(self._fp8_weights, weights))
 
     def quantize_experts(self):
         """From now on forward passes use an 8-bit copy of the expert weights as they are now.  Such passes have no
         backward: they run under torch.no_grad() (or with nothing that requires a gradient).  When the weights have
-        changed since, forward raises; call this again, or set `experts_fp8 = None` to go back to 16 bits."""
+        changed since (in place or by other ones; changes through `.data` are not seen), forward raises; call this
+        again, or set `experts_fp8 = None` to go back to 16 bits."""
         self.experts_fp8 = fp8.quantize_experts(self.momoe.Wl1_ND2H, self.momoe.Wl2_NHD)
-        self._fp8_versions = (self.momoe.Wl1_ND2H._version, self.momoe.Wl2_NHD._version)
+        self._fp8_weights = None
+        self._fp8_fresh()
 
     def _forward_fp8(self, x_BSD, rows):
         if torch.is_grad_enabled() and (x_BSD.requires_grad or any(p.requires_grad for p in self.parameters())):
             raise RuntimeError("8-bit experts have no backward pass: call the layer under torch.no_grad()")
-        versions = (self.momoe.Wl1_ND2H._version, self.momoe.Wl2_NHD._version)
-        if self._fp8_versions is None:
-            self._fp8_versions = versions
-        if self._fp8_versions != versions:
+        if not self._fp8_fresh():
             raise RuntimeError("the expert weights have changed since quantize_experts(): call it again")
         Wg = self.router.Wg_DN
         assert Wg.dtype == torch.bfloat16, "Wg_DN must be of type torch.bfloat16"

@@ -495,6 +495,39 @@ def test_prenorm_layer_in_eight_bits_is_its_operators_in_a_row(fp8):
     ops.check_status()
 
 
+def test_eight_bit_weights_that_stand_for_other_weights_are_refused(fp8):
+    """Swapped parameters, a copy of a layer whose weights have moved on, and a copy that is changed before its first pass."""
+    import copy
+    import io
+    moe = layer(128, 64, 8, 2, 0, 0)
+    x = torch.randn(1, 5, 128, device="cuda").bfloat16()
+    with torch.no_grad():
+        moe.quantize_experts()
+        want = moe(x)
+        twin = copy.deepcopy(moe)
+        twin.momoe.Wl1_ND2H.mul_(0.5)
+        with pytest.raises(RuntimeError, match="changed"):
+            twin(x)
+        with pytest.raises(RuntimeError, match="changed"):
+            copy.deepcopy(twin)(x)
+        twin.quantize_experts()
+        twin(x)
+        file = io.BytesIO()
+        torch.save(moe, file)
+        file.seek(0)
+        again = torch.load(file, weights_only=False)
+        again.biases_N.copy_(moe.biases_N)
+        assert torch.equal(again(x), moe(x)) and want.shape == x.shape
+        moe.momoe.Wl2_NHD = torch.nn.Parameter(moe.momoe.Wl2_NHD.detach().clone())
+        with pytest.raises(RuntimeError, match="changed"):
+            moe(x)
+        moe.quantize_experts()
+        moe(x)
+        plain = copy.deepcopy(layer(128, 64, 8, 2, 0, 0))       # one without 8-bit weights, which get set by hand
+        plain.experts_fp8 = moe.experts_fp8
+        plain(x)
+
+
 @pytest.mark.parametrize("fused", [True, False])
 def test_layer_with_balance_loss_trains_on_the_sum_of_both(fp8, fused):
     """The auxiliary loss and its share of the gradients are those of the operator on the layer's own logits."""
