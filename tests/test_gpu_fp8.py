@@ -26,6 +26,8 @@ SHAPES = [
     (640, 5, 3, 4096, 48, 0.0),
     (90, 40, 6, 256, 144, 3.0),       # few rows on average, some experts with several 32-row blocks
     (1400, 1000, 3, 64, 32, 1.0),     # many experts
+    (50, 24, 13, 144, 64, 0.5),       # more experts a token than the weighted sum reads at once
+    (33, 9, 7, 272, 48, 0.0),
     (40, 4, 2, 2576, 1680, 0.5),      # so few items that two thread blocks share an item's k axis, in both GEMMs
     (6000, 40, 3, 96, 64, 1.0),       # more pairs than one launch dispatches
 ]
