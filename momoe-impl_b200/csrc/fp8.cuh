@@ -51,20 +51,32 @@ constexpr int FP8_YBLOCK = 256;
 
 // Exponent e of one row (a lane each): stored value = value * 2^e, |value * 2^e| <= 2^15.  hs: the word of the row's first
 // scales, the next group 512 bytes on; ws: scale bytes of the first of the two 128-column blocks, the second nkb bytes on.
-__device__ __forceinline__ int fp8_row_exponent(const uint8_t* hs, const uint8_t* ws, bool two, int nkb, float w) {
+// What a group of four k blocks needs of both is read first, so that a caller can ask for the first group early.
+struct Fp8RowScales {
+    uint32_t hw;     // the row's scale bytes
+    int wb;          // lanes 0..3 (4..7): scale byte of block (lane & 3) of the first (second) 128 columns
+};
+__device__ __forceinline__ Fp8RowScales fp8_row_scales(const uint8_t* hs, const uint8_t* ws, bool two, int nkb, int grp) {
     const int lane = threadIdx.x & 31;
+    const int kb = grp * FP8_GROUP + (lane & 3);
+    const bool second = (lane & 4) != 0;
+    Fp8RowScales r;
+    r.hw = __ldcg(reinterpret_cast<const uint32_t*>(hs + static_cast<size_t>(grp) * FP8_ATOM));
+    r.wb = kb < nkb && (two || !second) ? static_cast<int>(__ldg(ws + (second ? nkb : 0) + kb)) : 0;
+    return r;
+}
+__device__ __forceinline__ int fp8_row_exponent(Fp8RowScales r, const uint8_t* hs, const uint8_t* ws, bool two, int nkb,
+                                                float w) {
     int top = 0;
-    for (int g = 0; g * FP8_GROUP < nkb; ++g) {
-        const uint32_t hw = __ldcg(reinterpret_cast<const uint32_t*>(hs + static_cast<size_t>(g) * FP8_ATOM));
-        const int kb = g * FP8_GROUP + (lane & 3);
-        const bool second = (lane & 4) != 0;
-        int b = kb < nkb && (two || !second) ? static_cast<int>(__ldg(ws + (second ? nkb : 0) + kb)) : 0;
-        b = max(b, __shfl_xor_sync(0xffffffffu, b, 4));
+    for (int g = 0;;) {
+        const int b = max(r.wb, __shfl_xor_sync(0xffffffffu, r.wb, 4));
 #pragma unroll
         for (int j = 0; j < FP8_GROUP; ++j) {
             const int wb = __shfl_sync(0xffffffffu, b, j);
-            if (g * FP8_GROUP + j < nkb) top = max(top, static_cast<int>((hw >> (8 * j)) & 255u) + wb);
+            if (g * FP8_GROUP + j < nkb) top = max(top, static_cast<int>((r.hw >> (8 * j)) & 255u) + wb);
         }
+        if (++g * FP8_GROUP >= nkb) break;
+        r = fp8_row_scales(hs, ws, two, nkb, g);
     }
     const int bound = top - 254 + 25 + (32 - __clz(nkb - 1)) + static_cast<int>((__float_as_uint(w) >> 23) & 255u) - 126;
     return min(max(15 - bound, -126), 126);

@@ -97,9 +97,10 @@ __device__ __forceinline__ float d8_factor(const Fp8DecArgs& g, const D8Item& w,
     const int lane = threadIdx.x & 31;
     const float wgt = __ldcg(g.row_weight + row0 + lane);
     const int w_blocks = (g.out_cols + 127) / 128, n0 = w.cb * 2;
-    const int e = fp8_row_exponent(g.x_scale + fp8_atom_offset(row0 + lane, 0, (g.nkb + 3) >> 2),
-                                   g.w_scale + (static_cast<size_t>(w.e) * w_blocks + n0) * g.nkb, n0 + 1 < w_blocks, g.nkb,
-                                   wgt);
+    const uint8_t* hs = g.x_scale + fp8_atom_offset(row0 + lane, 0, (g.nkb + 3) >> 2);
+    const uint8_t* ws = g.w_scale + (static_cast<size_t>(w.e) * w_blocks + n0) * g.nkb;
+    const bool two = n0 + 1 < w_blocks;
+    const int e = fp8_row_exponent(fp8_row_scales(hs, ws, two, g.nkb, 0), hs, ws, two, g.nkb, wgt);
     if (store) g.y_scale[(row0 + lane) * g.n_cblk + w.cb] = pow2f(-e);
     return wgt * pow2f(e);
 }
