@@ -305,8 +305,9 @@ int momoe_fp8_up_swiglu_decode(const momoe_plan_t* plan, const int32_t* tile_row
                                uint8_t* h_scale, momoe_stream_t stream);
 
 /* Down GEMM on 8-bit operands: w[r] * (h[r, :] W2[e]^T) as y_sorted fp16 [rows, D] and y_scale fp32
- * [rows, ceil(D / 256)], a power of two for each (row, 256 columns); the value is their product.  W2 [N, D, H],
- * S2 [N, ceil(D / 128), ceil(H / 128)]. */
+ * [rows, ceil(D / 256)], a power of two for each (row, 256 columns); the value is their product.  The power is that which
+ * stores the largest finite value of the 256 as 2^13 to 2^15: values down to 2^-27 of it have 11 bits, smaller ones are off by
+ * up to 2^-38 of it.  W2 [N, D, H], S2 [N, ceil(D / 128), ceil(H / 128)]. */
 int momoe_fp8_down_scale(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* h_sorted,
                          const uint8_t* h_scale, const uint8_t* W2_NDH, const uint8_t* S2, void* y_sorted,
                          float* y_scale, momoe_stream_t stream);

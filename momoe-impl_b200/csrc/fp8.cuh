@@ -44,42 +44,19 @@ __device__ __forceinline__ uint8_t fp8_one(float a) { return __nv_cvt_float_to_f
 
 // Result rows of the down GEMM on their way to the weighted sum: fp16 with one power of two for each (row, 256 columns).
 // bf16 rows would add a second rounding as large as that of the result itself; fp16 rows have the same size and one 16 times
-// smaller, and the power of two keeps them in range whatever the values: it comes from a bound on the row's products, so it
-// is known before the accumulators are.  With 448 2^a the largest value of a block, |sum| <= 2^max(a_h + a_W) 448^2 H and
-// 448^2 * 128 < 2^25.  The bound is 2^10 to 2^13 above typical values; fp16 has 28 binades of full precision below it.
+// smaller, and the power of two keeps them in range.  It comes from the largest finite sum of the row's 256 columns, which is
+// stored as 2^13 to 2^15.  Values down to 2^-27 of the largest keep their 11 bits; smaller ones are off by up to 2^-38 of it.
+// (A bound from the blocks' scales is known before the sums are and 0.5 to 1.5 us a call cheaper, but a block of zeros has a
+// scale of 1, which says nothing about it: beside it real results fell below fp16's normal numbers.)
 constexpr int FP8_YBLOCK = 256;
 
-// Exponent e of one row (a lane each): stored value = value * 2^e, |value * 2^e| <= 2^15.  hs: the word of the row's first
-// scales, the next group 512 bytes on; ws: scale bytes of the first of the two 128-column blocks, the second nkb bytes on.
-// What a group of four k blocks needs of both is read first, so that a caller can ask for the first group early.
-struct Fp8RowScales {
-    uint32_t hw;     // the row's scale bytes
-    int wb;          // lanes 0..3 (4..7): scale byte of block (lane & 3) of the first (second) 128 columns
-};
-__device__ __forceinline__ Fp8RowScales fp8_row_scales(const uint8_t* hs, const uint8_t* ws, bool two, int nkb, int grp) {
-    const int lane = threadIdx.x & 31;
-    const int kb = grp * FP8_GROUP + (lane & 3);
-    const bool second = (lane & 4) != 0;
-    Fp8RowScales r;
-    r.hw = __ldcg(reinterpret_cast<const uint32_t*>(hs + static_cast<size_t>(grp) * FP8_ATOM));
-    r.wb = kb < nkb && (two || !second) ? static_cast<int>(__ldg(ws + (second ? nkb : 0) + kb)) : 0;
-    return r;
-}
-__device__ __forceinline__ int fp8_row_exponent(Fp8RowScales r, const uint8_t* hs, const uint8_t* ws, bool two, int nkb,
-                                                float w) {
-    int top = 0;
-    for (int g = 0;;) {
-        const int b = max(r.wb, __shfl_xor_sync(0xffffffffu, r.wb, 4));
-#pragma unroll
-        for (int j = 0; j < FP8_GROUP; ++j) {
-            const int wb = __shfl_sync(0xffffffffu, b, j);
-            if (g * FP8_GROUP + j < nkb) top = max(top, static_cast<int>((r.hw >> (8 * j)) & 255u) + wb);
-        }
-        if (++g * FP8_GROUP >= nkb) break;
-        r = fp8_row_scales(hs, ws, two, nkb, g);
-    }
-    const int bound = top - 254 + 25 + (32 - __clz(nkb - 1)) + static_cast<int>((__float_as_uint(w) >> 23) & 255u) - 126;
-    return min(max(15 - bound, -126), 126);
+// Magnitude of a sum that sets the power: infinities and NaN stay what they are whatever the power is, and do not set it.
+__device__ __forceinline__ float finite_or_zero(float v) { return abs_bits(v) < 0x7F800000u ? fabsf(v) : 0.0f; }
+// Exponent e of a row: stored value = sum * w * 2^e.  et: biased exponent of the largest finite sum; w: the row's weight.
+__device__ __forceinline__ int fp8_row_exponent(int et, float w) {
+    const int ew = static_cast<int>((__float_as_uint(w) >> 23) & 255u);
+    // |sum| < 2^(et - 126) and |w| < 2^(ew - 126); the second limit keeps w * 2^e finite
+    return min(max(267 - et - ew, -126), min(126, 253 - ew));
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }   // |e| <= 126
 

@@ -10,7 +10,7 @@
 //   up    an item is 128 columns of h: two MMAs a k slice, the linear rows and the gate rows of W1[e], into two accumulators
 //         whose lane j holds a[j] and b[j] of the same column, so the epilogue thread has both; h needs the maximum over
 //         the item's 128 columns (the scale of 8-bit rows): a warp reduction for each token and one meeting of four warps
-//   down  an item is 256 columns of y in two MMAs
+//   down  an item is 256 columns of y in two MMAs; a result row needs its largest sum (its power of two): the same
 //
 // One CTA (320 threads) an SM, persistent over items = (128-row tile, column block).  Warp 0 loads, warp 1 issues MMAs,
 // warps 2..5 are the epilogue (a thread has one weight column and 32 tokens at a time), warps 6..9 write scales to TMEM
@@ -80,7 +80,7 @@ __device__ __forceinline__ D8Item d8_item(const Fp8DecArgs& g, int item) {
 struct D8Epi {
     uint32_t bar_acc_empty, bar_meet, bar_part_full, bar_part_free;
     uint32_t part;           // split: this lane's place in the buffer of the first CTA
-    uint32_t* s_top;         // up: [2][4 quarters][32 tokens]
+    uint32_t* s_top;         // [2][4 quarters][32 tokens]
     volatile int* abortp;
     int rank;
     int meet, parts;
@@ -92,24 +92,12 @@ __device__ __forceinline__ void d8_tmem_ld(uint32_t taddr, uint32_t (&r)[T]) {
     else tmem_ld32(taddr, r);
 }
 
-// down: lane t gets the weight of token t times its power of two, whose inverse is stored.
-__device__ __forceinline__ float d8_factor(const Fp8DecArgs& g, const D8Item& w, size_t row0, bool store) {
-    const int lane = threadIdx.x & 31;
-    const float wgt = __ldcg(g.row_weight + row0 + lane);
-    const int w_blocks = (g.out_cols + 127) / 128, n0 = w.cb * 2;
-    const uint8_t* hs = g.x_scale + fp8_atom_offset(row0 + lane, 0, (g.nkb + 3) >> 2);
-    const uint8_t* ws = g.w_scale + (static_cast<size_t>(w.e) * w_blocks + n0) * g.nkb;
-    const bool two = n0 + 1 < w_blocks;
-    const int e = fp8_row_exponent(fp8_row_scales(hs, ws, two, g.nkb, 0), hs, ws, two, g.nkb, wgt);
-    if (store) g.y_scale[(row0 + lane) * g.n_cblk + w.cb] = pow2f(-e);
-    return wgt * pow2f(e);
-}
-
 // The first T tokens of a 32-row block out of the accumulators (columns taddr and taddr + D8_NT), by the four epilogue
-// warps; `last`: hand the accumulators back.  False when a wait was abandoned.
+// warps; `last`: hand the accumulators back; left: real rows from row0 on; wgt: down, the weight of row0 + lane.  False when a
+// wait was abandoned.
 template <bool UP, int SPLIT, int T>
 __device__ __forceinline__ bool d8_read_out(const Fp8DecArgs& g, D8Epi& c, const D8Item& w, size_t row0, uint32_t taddr,
-                                            bool last, float factor) {
+                                            bool last, int left, float wgt) {
     const int lane = threadIdx.x & 31, q = (threadIdx.x >> 5) & 3;
     uint32_t r[T], rb[T];
     d8_tmem_ld<T>(taddr, r);
@@ -147,28 +135,43 @@ __device__ __forceinline__ bool d8_read_out(const Fp8DecArgs& g, D8Epi& c, const
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(c.bar_part_free, 1));
     }
-    if constexpr (UP) {
-        const int col = w.cb * 128 + q * 32 + lane;
-        float v[T];
-        uint32_t mine = 0u;
+    // lane t gets the largest of token t's columns (up: 128, the rest has zero weights; down: the finite ones of 256)
+    float v[T];
+    uint32_t mine = 0u;
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
+    for (int t = 0; t < T; ++t) {
+        uint32_t top;
+        if constexpr (UP) {
             const float b = __uint_as_float(rb[t]);
             v[t] = b * __fdividef(1.0f, 1.0f + __expf(-b)) * __uint_as_float(r[t]);
-            // columns past H have zero weights, so v is zero there
-            const uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(v[t]));
-            if (lane == t) mine = top;
+            top = __reduce_max_sync(0xffffffffu, abs_bits(v[t]));
+        } else {
+            top = __reduce_max_sync(0xffffffffu, abs_bits(fmaxf(fabsf(__uint_as_float(r[t])), fabsf(__uint_as_float(rb[t])))));
         }
-        const int mb = c.meet & 1;
-        uint32_t* s_top = c.s_top + mb * 128;
-        s_top[q * 32 + lane] = mine;
-        // this half of s_top is written again two meetings later, after every warp has been at the next one
-        __syncwarp();
-        if (lane == 0) mbar_arrive(c.bar_meet);
-        bool ok = mbar_wait(c.bar_meet, static_cast<uint32_t>(mb), c.abortp, g.status, DEV_TIMEOUT_EPILOGUE);
-        if (!__all_sync(0xffffffffu, ok)) return false;
-        ++c.meet;
-        mine = max(max(s_top[lane], s_top[32 + lane]), max(s_top[64 + lane], s_top[96 + lane]));
+        if (lane == t) mine = top;
+    }
+    if constexpr (!UP) {
+        if (__any_sync(0xffffffffu, mine >= 0x7F800000u)) {
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                const uint32_t top = __reduce_max_sync(
+                    0xffffffffu, __float_as_uint(fmaxf(finite_or_zero(__uint_as_float(r[t])), finite_or_zero(__uint_as_float(rb[t])))));
+                if (lane == t) mine = top;
+            }
+        }
+    }
+    const int mb = c.meet & 1;
+    uint32_t* s_top = c.s_top + mb * 128;
+    s_top[q * 32 + lane] = mine;
+    // this half of s_top is written again two meetings later, after every warp has been at the next one
+    __syncwarp();
+    if (lane == 0) mbar_arrive(c.bar_meet);
+    bool ok = mbar_wait(c.bar_meet, static_cast<uint32_t>(mb), c.abortp, g.status, DEV_TIMEOUT_EPILOGUE);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    ++c.meet;
+    mine = max(max(s_top[lane], s_top[32 + lane]), max(s_top[64 + lane], s_top[96 + lane]));
+    if constexpr (UP) {
+        const int col = w.cb * 128 + q * 32 + lane;
         const uint32_t byte = fp8_scale_byte(mine);
         const float inv = fp8_inv_scale(byte);
         if (q == 0 && lane < T)
@@ -180,16 +183,17 @@ __device__ __forceinline__ bool d8_read_out(const Fp8DecArgs& g, D8Epi& c, const
             if (col < g.out_cols) dst[static_cast<size_t>(t) * g.out_cols] = fp8_one(v[t] * s);
         }
     } else {
+        const int e = fp8_row_exponent(static_cast<int>(mine >> 23), wgt);
+        if (q == 0 && lane < left && lane < T) g.y_scale[(row0 + lane) * g.n_cblk + w.cb] = pow2f(-e);
+        const float factor = wgt * pow2f(e);
+        const int col = w.cb * 256 + q * 32 + lane;
+        __half* dst = g.y + row0 * g.out_cols + col;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int col = w.cb * 256 + i * 128 + q * 32 + lane;
-            __half* dst = g.y + row0 * g.out_cols + col;
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
-                const float s = __shfl_sync(0xffffffffu, factor, t);
-                if (col < g.out_cols)
-                    dst[static_cast<size_t>(t) * g.out_cols] = __float2half_rn(__uint_as_float(i == 0 ? r[t] : rb[t]) * s);
-            }
+        for (int t = 0; t < T; ++t) {
+            const float s = __shfl_sync(0xffffffffu, factor, t);
+            if (col < g.out_cols) dst[0] = __float2half_rn(__uint_as_float(r[t]) * s);
+            if (col + 128 < g.out_cols) dst[128] = __float2half_rn(__uint_as_float(rb[t]) * s);
+            dst += g.out_cols;
         }
     }
     return true;
@@ -205,8 +209,8 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     __shared__ uint64_t bar_sf_empty[2];
     __shared__ uint64_t bar_acc_full;
     __shared__ uint64_t bar_acc_empty;
-    __shared__ uint64_t bar_meet;                    // up: the four epilogue warps have written their part of s_top
-    __shared__ uint32_t s_top[UP ? 2 : 1][UP ? 4 : 1][UP ? 32 : 1];
+    __shared__ uint64_t bar_meet;                    // the four epilogue warps have written their part of s_top
+    __shared__ uint32_t s_top[2][4][32];
     __shared__ uint64_t bar_part_full[4];            // split: the other CTA's part of a quarter's accumulators has arrived
     __shared__ uint64_t bar_part_free[4];            // split, other CTA: its buffer has been read
     __shared__ uint32_t tmem_slot;
@@ -389,24 +393,21 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
         bool ok = true;
         for (int item = first_item; ok && item < total_items; item += step_item, ++it) {
             const D8Item w = item == first_item ? first : d8_item(g, item);
-            // down: what does not need the accumulators is worked out while they fill
-            const bool store = q == 0 && (SPLIT == 1 || rank == 0);
-            float factor = 0.0f;
-            if constexpr (!UP) factor = d8_factor(g, w, static_cast<size_t>(w.tile) * TILE_M, store && lane < w.rows);
+            // down: the first rows' weights are asked for while the accumulators fill
+            const size_t tile0 = static_cast<size_t>(w.tile) * TILE_M;
+            float wgt = UP ? 0.0f : __ldcg(g.row_weight + tile0 + lane);
             ok = mbar_wait(smem_u32(&bar_acc_full), it & 1u, abortp, g.status, DEV_TIMEOUT_EPILOGUE);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             for (int sub = 0; ok && sub < w.n_sub; ++sub) {
-                const size_t row0 = static_cast<size_t>(w.tile) * TILE_M + sub * 32;
+                const size_t row0 = tile0 + sub * 32;
                 const bool last = sub + 1 == w.n_sub;
                 // a token more costs a reduction and a store, so a few rows take the short form
                 const int left = w.rows - sub * 32;
-                if constexpr (!UP) {
-                    if (sub > 0) factor = d8_factor(g, w, row0, store && lane < left);
-                }
-                ok = left <= 8 ? d8_read_out<UP, SPLIT, 8>(g, c, w, row0, taddr + sub * 32, last, factor)
-                               : d8_read_out<UP, SPLIT, 32>(g, c, w, row0, taddr + sub * 32, last, factor);
+                if (!UP && sub > 0) wgt = __ldcg(g.row_weight + row0 + lane);
+                ok = left <= 8 ? d8_read_out<UP, SPLIT, 8>(g, c, w, row0, taddr + sub * 32, last, left, wgt)
+                               : d8_read_out<UP, SPLIT, 32>(g, c, w, row0, taddr + sub * 32, last, left, wgt);
             }
         }
     }

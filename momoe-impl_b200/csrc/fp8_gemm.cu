@@ -30,6 +30,7 @@
 //
 // Padding rows hold anything: no row of a forward pass depends on another, and no consumer reads their results.
 #include <cstring>
+#include <type_traits>
 
 #include "fp8.cuh"
 #include "internal.h"
@@ -133,7 +134,8 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
     __shared__ uint64_t bar_ovl;                     // leader: the shared columns of the latest tile have been read
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
-    __shared__ uint32_t s_top[UP ? 2 : 1][UP ? 2 : 1][UP ? TILE_M : 1];   // up: [meeting][column half][row]
+    // [meeting][column half][row]: up, the bits of the largest magnitude; down, its exponent alone, since memory is short
+    __shared__ std::conditional_t<UP, uint32_t, uint8_t> s_top[2][2][TILE_M];
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -340,26 +342,15 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
         const uint32_t stage_area = epi_base + (warp - 2) * PIECES * F8_PIECE;
         int it = 0;
         bool ok = true;
-        int meet = 0;                      // up: meetings with the warp of the other column half so far
+        int meet = 0;                      // meetings with the warp of the other column half so far
         int n_stored = 0;                  // pieces handed to TMA stores so far (lane 0 owns the bulk groups)
-        // down: what a row's power of two depends on is asked for an item ahead, since a short k axis leaves no time for it
-        // (H256, 8192 tokens: 101 -> 93 us at D4096 top-4, 51 -> 46 us at D1024 top-8; nothing at H1024)
+        // an item's table entries, and down the rows' weights, are asked for an item ahead
         Fp8Work next = {};
-        const uint8_t *hs = nullptr, *ws = nullptr;
-        bool two = false;
         float w_next = 0.0f;
-        Fp8RowScales s_next = {};
         auto ask = [&](int item) {
             next = f8_work<CG>(g, item, cta_rank);
             if constexpr (!UP) {
-                if (q * 32 < next.rows) {
-                    const size_t r = static_cast<size_t>(next.tile) * TILE_M + row;
-                    hs = g.a_scale + fp8_atom_offset(r, 0, n_groups);
-                    ws = g.b_scale + (static_cast<size_t>(next.e) * g.b_blocks + next.nb * 2) * g.nkb;
-                    two = next.nb * 2 + 1 < g.b_blocks;
-                    w_next = __ldcg(g.row_weight + r);
-                    s_next = fp8_row_scales(hs, ws, two, g.nkb, 0);
-                }
+                if (q * 32 < next.rows) w_next = __ldcg(g.row_weight + static_cast<size_t>(next.tile) * TILE_M + row);
             }
         };
         if (cluster_id < total_items) ask(cluster_id);
@@ -380,26 +371,19 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                 if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty_leader + ab * static_cast<uint32_t>(sizeof(uint64_t)));
             };
             const bool live = q * 32 < w.rows;         // this warp has real rows
-            float wgt = 0.0f;
+            const float wgt = w_next;
             const size_t grow = static_cast<size_t>(w.tile) * TILE_M + row;
-            if constexpr (!UP) {
-                if (live) {
-                    const int e = fp8_row_exponent(s_next, hs, ws, two, g.nkb, w_next);
-                    if (half == 0) g.y_scale[grow * g.n_nblk + w.nb] = pow2f(-e);
-                    wgt = w_next * pow2f(e);
-                }
-            }
             if (item + n_clusters < total_items) ask(item + n_clusters);
             ok = mbar_wait(smem_u32(&bar_acc_full[ab]), (it >> 1) & 1u, abortp, g.status, DEV_TIMEOUT_EPILOGUE) &&
                  *abortp == 0;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) {
                 // the partner warp may be on its way into the meeting below: it must not wait for this one
-                if constexpr (UP) asm volatile("bar.arrive %0, 64;" ::"r"(1 + q) : "memory");
+                asm volatile("bar.arrive %0, 64;" ::"r"(1 + q) : "memory");
                 break;
             }
             tc_fence_after();
-            if (CG == 1 && !live) {
+            if ((CG == 1 || !UP) && !live) {           // so is its partner's
                 if (shares) hand_back_shared();
                 hand_back_all();
                 continue;
@@ -471,44 +455,77 @@ fp8_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_co
                     }
                 }
             } else {
+                // The largest sum of a row decides its power of two, so all are read before the first is stored.  Three chunks of
+                // 32 columns stay in registers, among them the one that may hold shared columns; the other is read again.
+                auto chunk = [&](int i) { return half == 0 ? i : 4 + ((i + 3) & 3); };   // half 1 starts with its last chunk
+                auto top_of = [](const uint32_t (&r)[32]) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) top = fmaxf(top, fabsf(__uint_as_float(r[j])));   // passes NaN over
+                    if (top == INFINITY) {
+                        top = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) top = fmaxf(top, finite_or_zero(__uint_as_float(r[j])));
+                    }
+                    return top;
+                };
+                uint32_t r0[32], r1[32], r[32];
+                tmem_ld32(taddr + chunk(0) * 32, r0);
+                tmem_ld32(taddr + chunk(1) * 32, r1);
+                tmem_ld_wait();
+                if (shares) hand_back_shared();
+                float top = fmaxf(top_of(r0), top_of(r1));
+#pragma unroll 1
+                for (int i = 2; i < 4; ++i) {
+                    tmem_ld32(taddr + chunk(i) * 32, r);
+                    tmem_ld_wait();
+                    top = fmaxf(top, top_of(r));
+                }
+                // as in the up GEMM, two warps share a row's columns
+                int et = static_cast<int>(__float_as_uint(top) >> 23);
+                s_top[meet & 1][half][row] = static_cast<uint8_t>(et);
+                asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+                et = max(et, static_cast<int>(s_top[meet & 1][half ^ 1][row]));
+                ++meet;
+                const int e = fp8_row_exponent(et, wgt);
+                if (half == 0) g.y_scale[grow * g.n_nblk + w.nb] = pow2f(-e);
+                const float factor = wgt * pow2f(e);
                 // results leave through shared memory by TMA: with one row a thread, stores straight from registers touch
                 // 32 sectors an instruction and take longer than the tile's MMAs (328 against 285 us, 16384 tokens, D2048
                 // H1024, top-8 of 128)
-#pragma unroll 1
-                for (int i = 0; i < 4; ++i) {
-                    // half 1 starts with the last chunk, which may be the shared one
-                    const int c = half == 0 ? i : 4 + ((i + 3) & 3);
-                    uint32_t r[32];
-                    tmem_ld32(taddr + c * 32, r);
-                    tmem_ld_wait();
-                    if (i == 0 && shares) hand_back_shared();
-                    if (i == 3) hand_back_all();
+                auto store = [&](int c, const uint32_t (&v)[32]) {
                     const int col0 = w.nb * F8_TILE_N + c * 32;
-                    if ((CG == 1 || live) && col0 < g.out_cols) {
-                        const uint32_t slot = stage_area + n_stored % PIECES * F8_PIECE;
-                        if (n_stored >= PIECES && lane == 0) bulk_wait_read<PIECES - 1>();
-                        __syncwarp();
-                        // [32 rows x 64 bytes], 64-byte swizzle: 16-byte chunk j of row r at chunk j ^ ((r >> 1) & 3)
-                        const uint32_t base = slot + lane * 64;
-                        const uint32_t x = (lane >> 1) & 3;
+                    if (col0 >= g.out_cols) return;
+                    const uint32_t slot = stage_area + n_stored % PIECES * F8_PIECE;
+                    if (n_stored >= PIECES && lane == 0) bulk_wait_read<PIECES - 1>();
+                    __syncwarp();
+                    // [32 rows x 64 bytes], 64-byte swizzle: 16-byte chunk j of row r at chunk j ^ ((r >> 1) & 3)
+                    const uint32_t base = slot + lane * 64;
+                    const uint32_t x = (lane >> 1) & 3;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t v[4];
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t p[4];
 #pragma unroll
-                            for (int u = 0; u < 4; ++u)
-                                v[u] = f8_pack_f16(__uint_as_float(r[j * 8 + 2 * u]) * wgt,
-                                                   __uint_as_float(r[j * 8 + 2 * u + 1]) * wgt);
-                            st_shared_v4(base + ((j ^ x) << 4), v[0], v[1], v[2], v[3]);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tma_store_2d(&tmO, slot, col0, w.tile * TILE_M + q * 32);   // columns past D are not written
-                            bulk_commit();
-                        }
-                        ++n_stored;
+                        for (int u = 0; u < 4; ++u)
+                            p[u] = f8_pack_f16(__uint_as_float(v[j * 8 + 2 * u]) * factor,
+                                               __uint_as_float(v[j * 8 + 2 * u + 1]) * factor);
+                        st_shared_v4(base + ((j ^ x) << 4), p[0], p[1], p[2], p[3]);
                     }
-                }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmO, slot, col0, w.tile * TILE_M + q * 32);   // columns past D are not written
+                        bulk_commit();
+                    }
+                    ++n_stored;
+                };
+                store(chunk(0), r0);
+                tmem_ld32(taddr + chunk(2) * 32, r0);
+                store(chunk(1), r1);
+                store(chunk(3), r);
+                tmem_ld_wait();
+                hand_back_all();
+                store(chunk(2), r0);
             }
         }
         if (lane == 0) bulk_wait_all<0>();   // the staging area must outlive every store issued from it
