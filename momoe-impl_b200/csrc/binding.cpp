@@ -85,9 +85,19 @@ Tensor dense(const Tensor& t) {
     Tensor c = t.contiguous();
     return is_aligned(c) ? c : c.clone();
 }
-// Whole numbers as contiguous int32; wider ones are first brought into [lo, hi], which keeps the ones outside outside.
+// Whole numbers as contiguous int32; ones that int32 does not hold are first brought into [lo, hi], which keeps the ones
+// outside outside.  In 64 bits, since a narrow type does not hold the limits either (-1 wraps around in an unsigned one).
 Tensor whole32(const Tensor& t, int64_t lo, int64_t hi) {
-    return (t.scalar_type() == at::kInt ? t : t.clamp(lo, hi).to(at::kInt)).contiguous();
+    switch (t.scalar_type()) {
+        case at::kInt:
+            return t.contiguous();
+        case at::kLong:
+        case at::kUInt32:
+        case at::kUInt64:
+            return t.to(at::kLong).clamp(lo, hi).to(at::kInt).contiguous();
+        default:
+            return t.to(at::kInt).contiguous();
+    }
 }
 // t [..., D] as [M, D] with contiguous columns, a row pitch of a multiple of 8 elements and a 16-byte aligned start: a
 // view where the layout allows it.

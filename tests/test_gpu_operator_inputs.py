@@ -1,0 +1,60 @@
+"""What callers hand to the operators around the expert layer besides the usual tensors."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+WHOLE = [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.uint32, torch.int64]
+
+
+@pytest.fixture(scope="module")
+def momoe():
+    import __graft_entry__
+    __graft_entry__.build()
+    import momoe
+    import momoe.balance
+    import momoe.fp8
+    import momoe.norm
+    return momoe
+
+
+def top(dtype):
+    return min(torch.iinfo(dtype).max, 2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("dtype", WHOLE)
+@pytest.mark.parametrize("N", [8, 130, 300])
+def test_ids_and_bounds_of_every_whole_type(momoe, dtype, N):
+    """Narrow types hold neither -1 nor N nor M: the limits must not be formed in them."""
+    g = torch.Generator().manual_seed(N)
+    M = 600
+    ids = torch.stack([torch.randperm(min(N, top(dtype) + 1), generator=g)[:3] for _ in range(M)]).int().cuda()
+    logits = torch.randn(M, N, generator=g).cuda()
+    cu = torch.tensor([0, 5, 90, 127], dtype=torch.int32, device="cuda")
+
+    def both(ids, cu):
+        leaf = logits.clone().requires_grad_(True)
+        loss, counts = momoe.balance.balance_loss(leaf, ids, 0, 0.5, 0.1, cu_seqlens=cu)
+        return loss.detach(), counts, torch.autograd.grad(loss, leaf)[0]
+    want = both(ids, cu)
+    assert int(want[1].sum()) == 127 * 3
+    assert all(torch.equal(a, b) for a, b in zip(both(ids.to(dtype), cu), want))
+    assert all(torch.equal(a, b) for a, b in zip(both(ids, cu.to(dtype)), want))
+    if torch.iinfo(dtype).min < 0:
+        out = ids.clone()
+        out[3] = -1
+        assert all(torch.equal(a, b) for a, b in zip(both(out.to(dtype), cu), both(out, cu)))
+
+
+@pytest.mark.parametrize("dtype", WHOLE)
+def test_expert_ids_of_every_whole_type(momoe, dtype):
+    from momoe import ops
+    g = torch.Generator().manual_seed(0)
+    for N in (8, 300):
+        e = momoe.fp8.quantize_experts(torch.randn(N, 64, 64, generator=g).cuda() * 0.1, torch.randn(N, 32, 64, generator=g).cuda() * 0.1)
+        ids = torch.stack([torch.randperm(min(N, top(dtype) + 1), generator=g)[:2] for _ in range(40)]).int().cuda()
+        x, w = torch.randn(40, 64, generator=g).bfloat16().cuda(), torch.rand(40, 2, generator=g).cuda()
+        want = momoe.fp8.experts_forward(x, ids, w, e)
+        got = momoe.fp8.experts_forward(x, ids.to(dtype), w, e)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        ops.check_status()
