@@ -513,7 +513,15 @@ class ExpertParallelMoE(nn.Module):
     needs them, or needs larger ones, must be reached by every rank (same token count per rank, or `reserve()` with
     the largest count up front).  Device-side problems (status 301: a peer did not reach a hand-shake in time,
     302: the routing does not fit the buffers, raise `capacity_factor`) are reported as a RuntimeError by the NEXT
-    forward pass without synchronising the host; `MOMOE_B200_CHECK=1` reports them at the end of the same pass."""
+    forward pass without synchronising the host; `MOMOE_B200_CHECK=1` reports them at the end of the same pass.
+
+    The single-GPU layer's auxiliary losses and 8-bit experts are not part of this layer: a forward pass with
+    `balance_coef`, `z_coef` or `experts_fp8` set raises (`momoe.balance.balance_loss` works on the logits of
+    `router.Wg_DN` by itself)."""
+
+    balance_coef = 0.0
+    z_coef = 0.0
+    experts_fp8 = None
 
     def __init__(self, embedding_dim, intermediate_dim, num_experts, num_chosen_experts, num_shared_experts,
                  save_percent=0, bias_update_rate=1e-4, Wg_DN=None, Wl1_ND2H=None, Wl2_NHD=None, *, group=None,
@@ -564,6 +572,11 @@ class ExpertParallelMoE(nn.Module):
         return self.momoe.Wl2_NHD
 
     def forward(self, x_BSD):
+        if self.balance_coef != 0 or self.z_coef != 0:
+            raise RuntimeError("balance_coef and z_coef have no effect in ExpertParallelMoE: add momoe.balance.balance_loss "
+                               "of the router's logits to the loss instead")
+        if self.experts_fp8 is not None:
+            raise RuntimeError("ExpertParallelMoE has no 8-bit experts")
         B, S, _ = x_BSD.shape
         ops.status_poll(self.momoe.Wl1_ND2H.device)    # raises if an earlier pass left a device-side error code
         if self.transport == "peer":
