@@ -10,6 +10,7 @@
 #include <optional>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/extension.h>
@@ -77,6 +78,14 @@ void no_second_derivative(const char* what) {
     TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative (create_graph=True)");
 }
 
+// There are no forward-mode derivatives: a tangent would be lost, so it is refused.
+template <typename... T>
+void no_tangent(const char* what, const T&... inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    const auto dual = [](const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); };
+    TORCH_CHECK(!(dual(inputs) || ...), what, " has no forward-mode derivative");
+}
+
 int type_code(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat ? 2 : -1; }
 
 bool is_aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
@@ -135,6 +144,7 @@ void norm_check(const Tensor& x, const Tensor& weight, const OptTensor& residual
                     "the residual must be like x, ", x.sizes(), " in ", x.dtype(), ", but got: ", residual->sizes(), " in ",
                     residual->dtype());
     }
+    no_tangent("rms_norm", x, weight, residual ? *residual : Tensor());
 }
 
 struct Norm {
@@ -323,6 +333,7 @@ std::vector<Tensor> balance_loss(const Tensor& logits, const Tensor& topk_idx, i
     TORCH_CHECK(0 <= Ks && Ks < K && K <= N && N <= 1024,
                 "0 <= shared experts < K <= N <= 1024 is needed, but got: Ks = ", Ks, ", K = ", K, ", N = ", N);
     TORCH_CHECK(!(cu_seqlens && seq_len), "give cu_seqlens or seq_len, not both");
+    no_tangent("balance_loss", logits);
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor idx = whole32(topk_idx, -1, N);
     OptTensor cu;
@@ -363,6 +374,7 @@ std::vector<Tensor> experts_forward(const Tensor& x, const OptTensor& scale, con
     require_device(topk_w, dev);
     TORCH_CHECK(!(at::GradMode::is_enabled() && (x.requires_grad() || topk_w.requires_grad())),
                 "8-bit experts have no backward pass: call them under torch.no_grad()");
+    no_tangent("the forward pass of 8-bit experts", x, topk_w);
     TORCH_CHECK(W2.dim() == 3 && x.dim() == 2 && topk_idx.dim() == 2 && topk_idx.size(0) == x.size(0),
                 "x must be [M, D], topk_idx_MK [M, K] and the weights [N, 2H, D] and [N, D, H], but got: ", x.sizes(), ", ",
                 topk_idx.sizes(), ", ", W1.sizes(), " and ", W2.sizes());

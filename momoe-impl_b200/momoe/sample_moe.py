@@ -13,6 +13,7 @@ import weakref
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import balance, fp8, ops
 from ._lib import native, require_cuda
@@ -155,6 +156,8 @@ class MoE(nn.Module):
     def _forward_fp8(self, x_BSD, rows):
         if torch.is_grad_enabled() and (x_BSD.requires_grad or any(p.requires_grad for p in self.parameters())):
             raise RuntimeError("8-bit experts have no backward pass: call the layer under torch.no_grad()")
+        if forward_ad.unpack_dual(x_BSD).tangent is not None:
+            raise RuntimeError("8-bit experts have no forward-mode derivative")
         if not self._fp8_fresh():
             raise RuntimeError("the expert weights have changed since quantize_experts(): call it again")
         Wg = self.router.Wg_DN

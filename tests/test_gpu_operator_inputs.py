@@ -58,3 +58,31 @@ def test_expert_ids_of_every_whole_type(momoe, dtype):
         got = momoe.fp8.experts_forward(x, ids.to(dtype), w, e)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         ops.check_status()
+
+
+def test_tangents_are_refused(momoe):
+    """Forward-mode gradients: none of the operators has them, and none drops them."""
+    from torch.autograd import forward_ad
+    x, w = torch.randn(6, 64, device="cuda"), torch.ones(64, device="cuda")
+    e = momoe.fp8.quantize_experts(torch.randn(4, 64, 64, device="cuda"), torch.randn(4, 32, 64, device="cuda"))
+    ids, top = torch.zeros(6, 2, dtype=torch.int32, device="cuda"), torch.rand(6, 2, device="cuda")
+    ids[:, 1] = 1
+    moe = momoe.MoE(64, 32, 4, 2, 0)
+    moe.quantize_experts()
+    calls = [lambda: momoe.norm.rms_norm(x, w), lambda: momoe.norm.rms_norm(x, w, x), lambda: momoe.norm.rms_norm_fp8(x, w),
+             lambda: momoe.fp8.experts_forward(x.bfloat16(), ids, top, e), lambda: momoe.balance.balance_loss(x, ids)]
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for f in (lambda: momoe.norm.rms_norm(dual(x), w), lambda: momoe.norm.rms_norm(x, dual(w)),
+                          lambda: momoe.norm.rms_norm(x, w, dual(x)), lambda: momoe.norm.rms_norm_fp8(dual(x), w),
+                          lambda: momoe.fp8.experts_forward(dual(x.bfloat16()), ids, top, e),
+                          lambda: momoe.fp8.experts_forward(x.bfloat16(), ids, dual(top), e),
+                          lambda: momoe.balance.balance_loss(dual(x), ids)):
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        f()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            moe(dual(x.bfloat16()[None]))
+        for f in calls:                                     # nothing to lose: inside a level, without tangents
+            f()
