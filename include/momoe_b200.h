@@ -254,7 +254,8 @@ int momoe_quantize_rows(const void* x, int64_t x_stride, int32_t type, int32_t M
 
 /* Balance loss and z-loss of a router, with per-expert counts.  logits [M, N] contiguous in bf16 or fp32; topk_idx_MK
  * int32 [M, K], ids outside [0, N) are not counted.  The M rows are B sequences: sequence b is rows cu_seqlens[b] ..
- * cu_seqlens[b + 1] - 1 (int32 [B + 1], ascending; rows outside are neither read nor counted), or, with cu_seqlens
+ * cu_seqlens[b + 1] - 1 (int32 [B + 1], ascending; bounds outside [0, M] count as 0 and M; rows outside are neither read nor
+ * counted; a table that does not ascend gives a loss and grad_BN of NaN and counts of 0), or, with cu_seqlens
  * NULL, consecutive sequences of seq_len rows (the last may be shorter; B = ceil(M / seq_len)).  With p the softmax over
  * the Ng = N - Ks gating logits, T_b a sequence's tokens, T all tokens and B' the sequences that are not empty:
  *   loss = balance_coef / B' * sum_b sum_e [Ng / ((K - Ks) T_b) count[b, e]] [mean over b of p[., e]]

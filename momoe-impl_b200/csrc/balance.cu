@@ -8,7 +8,7 @@
 // The counts carry no gradient, so with g[b,e] = balance_coef f[b,e] / (B' T_b)
 //   dloss/dlogit[t,e] = p[t,e] (g[b,e] - sum_j g[b,j] p[t,j] + 2 z_coef / T * lse_t)
 // Rows outside every sequence are neither read nor counted and get a zero gradient; a row whose gating logits are all
-// -inf has p = 0 and lse = 0.
+// -inf has p = 0 and lse = 0.  A table of sequences that does not ascend gives a loss and coefficients of NaN, and no counts.
 //
 // Bound by HBM for large batches (the logits are read once in each direction and the gradient written once) and by the
 // launches for small ones.  Forward, two launches: blocks of rows leave partial sums, one slot for each (row block,
@@ -132,7 +132,7 @@ struct BalArgs {
     float* slot_z;       // [n_blk + B]
     float* share;        // [column blocks * B]
     unsigned* ticket;
-    int* totals;         // [2]: sequences that are not empty, all their tokens
+    int* totals;         // [3]: sequences that are not empty, all their tokens, whether a bound is below the one before
     float* loss;
     long long* counts;   // [B, N]
     float* g;            // [B, N]
@@ -150,24 +150,24 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_partial_kernel(const BalA
     const int row0 = c * a.R, row1 = min(a.M, row0 + a.R);
     if (c == 0) {
         // once for the whole call, whatever the number of sequences
-        __shared__ int s_tot[2];
-        if (threadIdx.x == 0) {
-            *a.ticket = 0u;
-            s_tot[0] = s_tot[1] = 0;
-        }
+        __shared__ unsigned s_tot[3];
+        if (threadIdx.x < 3) s_tot[threadIdx.x] = 0u;
+        if (threadIdx.x == 0) *a.ticket = 0u;
         __syncthreads();
-        int n = 0, tokens = 0;
+        unsigned n = 0u, tokens = 0u, bad = 0u;
         for (int i = threadIdx.x; i < a.B; i += BAL_THREADS) {
             const int len = a.seq.bound(i + 1) - a.seq.bound(i);
             if (len > 0) {
                 ++n;
-                tokens += len;
+                tokens += static_cast<unsigned>(len);
             }
+            if (len < 0) bad = 1u;
         }
         atomicAdd(&s_tot[0], n);
         atomicAdd(&s_tot[1], tokens);
+        atomicOr(&s_tot[2], bad);
         __syncthreads();
-        if (threadIdx.x < 2) a.totals[threadIdx.x] = s_tot[threadIdx.x];
+        if (threadIdx.x < 3) a.totals[threadIdx.x] = static_cast<int>(s_tot[threadIdx.x]);
     }
     const T* logits = static_cast<const T*>(a.logits);
     const int Ng = a.N - a.Ks;
@@ -175,8 +175,9 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_partial_kernel(const BalA
     if (b < 0) b = 0;
     for (; b < a.seq.B; ++b) {
         const int start = a.seq.bound(b);
-        if (start >= row1) break;
-        const int lo = max(start, row0), hi = min(a.seq.bound(b + 1), row1);
+        const int end = a.seq.bound(b + 1);
+        if (start >= row1 || end < start) break;
+        const int lo = max(start, row0), hi = min(end, row1);
         if (hi <= lo) continue;
         for (int e = threadIdx.x; e < a.N; e += BAL_THREADS) s_cnt[e] = 0;
         __syncthreads();
@@ -242,10 +243,11 @@ __global__ void __launch_bounds__(1024) balance_finish_kernel(const BalArgs a) {
     const int b = blockIdx.y;
     const int start = a.seq.bound(b), end = a.seq.bound(b + 1);
     const int n = a.totals[0], tokens = a.totals[1];
+    const bool bad = a.totals[2] != 0;          // then nothing is read of the slots, which need not have been written
 
     const int e = blockIdx.x * 32 + tx;
     const int Ng = a.N - a.Ks;
-    const int T_b = end - start;
+    const int T_b = bad ? 0 : end - start;
     float p = 0.0f;
     int cnt = 0;
     if (T_b > 0 && e < a.N) {
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(1024) balance_finish_kernel(const BalArgs a) {
         term = gf * p;
         if (tx == 0) {
             a.counts[static_cast<size_t>(b) * a.N + eo] = cnt;
-            a.g[static_cast<size_t>(b) * a.N + eo] = gf;
+            a.g[static_cast<size_t>(b) * a.N + eo] = bad ? NAN : gf;
         }
     }
     // z-loss of the sequence, added by its first block
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(1024) balance_finish_kernel(const BalArgs a) {
     __syncthreads();
     if (ty == 0) {
         total = bal_sum(s_red[tx]);
-        if (tx == 0) *a.loss = total;
+        if (tx == 0) *a.loss = bad ? NAN : total;
     }
 }
 
@@ -398,7 +400,7 @@ static BalLayout bal_layout(int M, int N, int B) {
     l.share = l.z + slots * 4;
     l.ticket = l.share + static_cast<size_t>((N + 31) / 32) * B * 4;
     l.totals = l.ticket + 4;
-    l.bytes = l.totals + 8;
+    l.bytes = l.totals + 12;
     return l;
 }
 

@@ -17,7 +17,9 @@ def balance_loss(logits_MN, topk_idx_MK, num_shared_experts=0, balance_coef=1.0,
 
     The rows are packed sequences: cu_seqlens [B + 1] on the device, ascending, sequence b is rows cu_seqlens[b] up
     to cu_seqlens[b + 1] (empty ones count for nothing; rows outside, such as padding, are not read and get a zero
-    gradient); or seq_len, consecutive sequences of that many rows (B = ceil(M / seq_len)); or neither, one sequence.
+    gradient; bounds outside [0, M] count as 0 and M; a table that does not ascend, which only the device can see, gives a
+    loss and gradients of NaN and counts of 0); or seq_len, consecutive sequences of that many rows (B =
+    ceil(M / seq_len)); or neither, one sequence.
     Returns (loss float32 [], tokens_per_expert_BN int64 [B, N]); shared experts are counted but not balanced."""
     loss, counts = native.balance_loss(logits_MN, topk_idx_MK, num_shared_experts, balance_coef, z_coef, cu_seqlens,
                                        seq_len)

@@ -86,3 +86,25 @@ def test_tangents_are_refused(momoe):
             moe(dual(x.bfloat16()[None]))
         for f in calls:                                     # nothing to lose: inside a level, without tangents
             f()
+
+
+@pytest.mark.parametrize("bounds", [[0, 30, 20, 50], [10, 5], [60, 0], [0, 60, 59], [0, 60, 0, 60, 0, 60], [7] + list(range(600, 0, -1))])
+def test_bounds_that_do_not_ascend_give_nan(momoe, bounds):
+    """Not numbers from whatever the workspace held."""
+    g = torch.Generator().manual_seed(1)
+    M = 700
+    logits, ids = torch.randn(M, 40, generator=g).cuda(), torch.randint(0, 40, (M, 2), generator=g).int().cuda()
+
+    def run(bounds):
+        leaf = logits.clone().requires_grad_(True)
+        cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+        loss, counts = momoe.balance.balance_loss(leaf, ids, 0, 0.5, 0.1, cu_seqlens=cu)
+        return loss.detach(), counts, torch.autograd.grad(loss, leaf)[0]
+    want = run([0, 20, 700])
+    loss, counts, grad = run(bounds)
+    assert torch.isnan(loss) and not counts.any()
+    inside = torch.zeros(M, dtype=torch.bool, device="cuda")
+    inside[bounds[0]:bounds[-1]] = True
+    assert torch.isnan(grad[inside]).all() and not grad[~inside].any()
+    assert all(torch.equal(a, b) for a, b in zip(run([-3, 20, 701]), want))    # outside [0, M]: as 0 and M
+    assert all(torch.equal(a, b) for a, b in zip(run([0, 20, 700]), want))
