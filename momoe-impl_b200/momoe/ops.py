@@ -47,7 +47,8 @@ def status_word(device):
     """Per-device int32 word the kernels report device-side problems into (0 = fine)."""
     key = torch.device(device).index if torch.device(device).index is not None else torch.cuda.current_device()
     if key not in _status_words:
-        _status_words[key] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
+        with torch.inference_mode(False):      # it outlives the first caller's mode and is cleared outside of it
+            _status_words[key] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
     return _status_words[key]
 
 
@@ -88,8 +89,9 @@ def status_post(device):
     key = w.device.index
     rep = _status_reports.get(key)
     if rep is None:
-        rep = _status_reports[key] = dict(host=torch.zeros(1, dtype=torch.int32).pin_memory(),
-                                          event=torch.cuda.Event(), posted=False)
+        with torch.inference_mode(False):
+            rep = _status_reports[key] = dict(host=torch.zeros(1, dtype=torch.int32).pin_memory(),
+                                              event=torch.cuda.Event(), posted=False)
     elif rep["posted"] and not rep["event"].query():
         return          # the previous report is still on its way; it will carry any code that is set by then or later
     rep["host"].copy_(w, non_blocking=True)

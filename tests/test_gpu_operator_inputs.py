@@ -108,3 +108,23 @@ def test_bounds_that_do_not_ascend_give_nan(momoe, bounds):
     assert torch.isnan(grad[inside]).all() and not grad[~inside].any()
     assert all(torch.equal(a, b) for a, b in zip(run([-3, 20, 701]), want))    # outside [0, M]: as 0 and M
     assert all(torch.equal(a, b) for a, b in zip(run([0, 20, 700]), want))
+
+
+def test_status_is_cleared_outside_of_the_mode_it_was_first_used_in(momoe, monkeypatch):
+    from momoe import ops
+    monkeypatch.setattr(ops, "_status_words", {})
+    monkeypatch.setattr(ops, "_status_reports", {})
+    with torch.inference_mode():
+        e = momoe.fp8.quantize_experts(torch.randn(4, 64, 64, device="cuda"), torch.randn(4, 32, 64, device="cuda"))
+        x, w = torch.randn(3, 64, device="cuda").bfloat16(), torch.ones(3, 1, device="cuda")
+        momoe.fp8.experts_forward(x, torch.full((3, 1), 4, device="cuda"), w, e)
+        ops.status_post("cuda")
+    with pytest.raises(RuntimeError, match="202"):
+        ops.check_status()
+    ops.check_status()
+    momoe.fp8.experts_forward(x, torch.full((3, 1), 4, device="cuda"), w, e)
+    ops.status_post("cuda")
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="202"):
+        ops.status_poll("cuda")
+    ops.check_status()
