@@ -93,6 +93,11 @@ class FusedMoEFunction(torch.autograd.Function):
         return G_x.reshape(B, S, D).to(ctx.x_device), G_Wg, G_W1, G_W2, None, None, None, None, None, None
 
 
+def _version(w):
+    """Counts the in-place changes of a tensor; tensors made in inference mode have no count."""
+    return None if w.is_inference() else w._version
+
+
 class MoE(nn.Module):
     balance_coef = 0.0     # weight of the balance loss (each of a batch's sequences on its own)
     z_coef = 0.0           # weight of the z-loss
@@ -140,15 +145,15 @@ class MoE(nn.Module):
         look on."""
         weights = self.momoe.Wl1_ND2H, self.momoe.Wl2_NHD
         if self._fp8_weights is None:
-            self._fp8_weights = tuple((weakref.ref(w), w._version) for w in weights)
-        return len(self._fp8_weights) == 2 and all(ref() is w and version == w._version
+            self._fp8_weights = tuple((weakref.ref(w), _version(w)) for w in weights)
+        return len(self._fp8_weights) == 2 and all(ref() is w and version == _version(w)
                                                    for (ref, version), w in zip(self._fp8_weights, weights))
 
     def quantize_experts(self):
         """From now on forward passes use an 8-bit copy of the expert weights as they are now.  Such passes have no
         backward: they run under torch.no_grad() (or with nothing that requires a gradient).  When the weights have
-        changed since (in place or by other ones; changes through `.data` are not seen), forward raises; call this
-        again, or set `experts_fp8 = None` to go back to 16 bits."""
+        changed since (in place or by other ones; changes through `.data`, and in-place changes of tensors made in inference
+        mode, are not seen), forward raises; call this again, or set `experts_fp8 = None` to go back to 16 bits."""
         self.experts_fp8 = fp8.quantize_experts(self.momoe.Wl1_ND2H, self.momoe.Wl2_NHD)
         self._fp8_weights = None
         self._fp8_fresh()

@@ -128,3 +128,21 @@ def test_status_is_cleared_outside_of_the_mode_it_was_first_used_in(momoe, monke
     with pytest.raises(RuntimeError, match="202"):
         ops.status_poll("cuda")
     ops.check_status()
+
+
+def test_layer_made_in_inference_mode(momoe):
+    """Its parameters have no version counter; swapped ones are noticed all the same."""
+    x = torch.randn(1, 5, 64, device="cuda").bfloat16()
+    with torch.inference_mode():
+        moe = momoe.MoE(64, 32, 4, 2, 0)
+        moe.quantize_experts()
+        bias = moe.biases_N.clone()
+        want = moe(x)
+        moe.biases_N.copy_(bias)
+        assert torch.equal(moe(x), want)
+        moe.momoe.Wl2_NHD = torch.nn.Parameter(moe.momoe.Wl2_NHD.clone(), requires_grad=False)
+        with pytest.raises(RuntimeError, match="changed"):
+            moe(x)
+        moe.quantize_experts()
+        moe.biases_N.copy_(bias)
+        assert torch.equal(moe(x), want)
