@@ -103,7 +103,7 @@ class MoE(nn.Module):
     z_coef = 0.0           # weight of the z-loss
     aux_loss = None        # their sum of the latest forward pass, float32 [], differentiable; None if both are 0
     experts_fp8 = None     # 8-bit weights of forward-only calls, from quantize_experts()
-    _fp8_weights = None    # the weights that experts_fp8 stands for, with their versions; (): none of this layer's
+    _fp8_weights = None    # (experts_fp8, the weights that it stands for with their versions); no weights: none of this layer's
 
     def __init__(self, embedding_dim, intermediate_dim, num_experts, num_chosen_experts, num_shared_experts,
                  save_percent=0, bias_update_rate=1e-4, Wg_DN: torch.Tensor | None = None,
@@ -132,7 +132,7 @@ class MoE(nn.Module):
         state = dict(self.__dict__)
         state.pop("aux_loss", None)         # belongs to the graph of a forward pass, not to a copy of the layer
         # a copy has weights of its own, for which its 8-bit ones stand if they stand for this layer's
-        state["_fp8_weights"] = None if self.experts_fp8 is None or self._fp8_fresh() else ()
+        state["_fp8_weights"] = None if self.experts_fp8 is None or self._fp8_fresh() else (self.experts_fp8, ())
         return state
 
     def __setstate__(self, state):
@@ -144,10 +144,10 @@ class MoE(nn.Module):
         """Whether the 8-bit weights stand for the layer's weights as they are; ones that were set by hand do from the first
         look on."""
         weights = self.momoe.Wl1_ND2H, self.momoe.Wl2_NHD
-        if self._fp8_weights is None:
-            self._fp8_weights = tuple((weakref.ref(w), _version(w)) for w in weights)
-        return len(self._fp8_weights) == 2 and all(ref() is w and version == _version(w)
-                                                   for (ref, version), w in zip(self._fp8_weights, weights))
+        if self._fp8_weights is None or self._fp8_weights[0] is not self.experts_fp8:
+            self._fp8_weights = self.experts_fp8, tuple((weakref.ref(w), _version(w)) for w in weights)
+        seen = self._fp8_weights[1]
+        return len(seen) == 2 and all(ref() is w and version == _version(w) for (ref, version), w in zip(seen, weights))
 
     def quantize_experts(self):
         """From now on forward passes use an 8-bit copy of the expert weights as they are now.  Such passes have no

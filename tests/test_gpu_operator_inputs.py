@@ -146,3 +146,40 @@ def test_layer_made_in_inference_mode(momoe):
         moe.quantize_experts()
         moe.biases_N.copy_(bias)
         assert torch.equal(moe(x), want)
+
+
+def test_eight_bit_weights_set_by_hand_after_others(momoe):
+    """Ones that replace stale ones are the caller's; the stale ones stay refused, in copies as well."""
+    import copy
+    import io
+
+    def saved(layer):
+        file = io.BytesIO()
+        torch.save(layer, file)
+        file.seek(0)
+        return torch.load(file, weights_only=False)
+    x = torch.randn(1, 5, 64, device="cuda").bfloat16()
+    with torch.no_grad():
+        moe = momoe.MoE(64, 32, 4, 2, 0)
+        moe.quantize_experts()
+        old = moe.experts_fp8
+        moe.momoe.Wl1_ND2H.mul_(0.5)
+        with pytest.raises(RuntimeError, match="changed"):
+            moe(x)
+        for twin in (copy.deepcopy(moe), saved(moe)):
+            with pytest.raises(RuntimeError, match="changed"):
+                twin(x)
+        moe.experts_fp8 = momoe.fp8.quantize_experts(moe.momoe.Wl1_ND2H, moe.momoe.Wl2_NHD)
+        bias = moe.biases_N.clone()
+        want = moe(x)
+        for twin in (copy.deepcopy(moe), saved(moe)):
+            twin.biases_N.copy_(bias)
+            assert torch.equal(twin(x), want)
+        moe.experts_fp8 = None
+        moe(x)
+        moe.momoe.Wl1_ND2H.mul_(2)
+        moe.experts_fp8 = old
+        moe(x)
+        moe.momoe.Wl1_ND2H.mul_(2)
+        with pytest.raises(RuntimeError, match="changed"):
+            moe(x)
