@@ -62,14 +62,28 @@ def _run(head, tail, out, verbose):
         sys.stderr.write(res.stdout + res.stderr)
 
 
+def _built_for():
+    """What a compiled binding fits; part of the binary, and compared again when the package loads it."""
+    import torch
+    return "torch %s, Python %d.%d" % (torch.__version__, *sys.version_info[:2])
+
+
+def binding_stale(out=BINDING_PATH):
+    if _stale(out, [BINDING, HEADER]):
+        return True
+    with open(out, "rb") as f:
+        return _built_for().encode() + b"\0" not in f.read()
+
+
 def build_binding(out=BINDING_PATH, force=False, verbose=False):
     """The torch binding; it takes the entry points from the loaded library at run time, so neither links the other."""
-    if not force and not _stale(out, [BINDING, HEADER]):
+    if not force and not binding_stale(out):
         return out
     import torch
     home = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")))
     flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_native",
+             '-DMOMOE_BUILT_FOR="%s"' % _built_for(),
              "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
     includes = ["-isystem" + p for p in (os.path.join(home, "include"), os.path.join(cuda, "include"),
                                          os.path.join(home, "include", "torch", "csrc", "api", "include"),

@@ -430,6 +430,7 @@ std::vector<Tensor> experts_forward(const Tensor& x, const OptTensor& scale, con
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     using Release = pybind11::call_guard<pybind11::gil_scoped_release>;
+    m.attr("built_for") = MOMOE_BUILT_FOR;
     m.def("bind", &bind);
     m.def("launches", [] { return n_launches.load(); });
     m.def("rms_norm", &rms_norm, Release());

@@ -6,6 +6,7 @@ There is no fallback: if the library is missing, importing this module raises wi
 import contextlib
 import ctypes as C
 import os
+import sys
 
 import torch
 
@@ -21,8 +22,22 @@ lib = C.CDLL(LIB_PATH)
 
 if not os.path.exists(os.path.join(_HERE, "_native.so")):
     raise ImportError("_native.so is not built; run `python momoe-impl_b200/build.py` (needs g++ and torch's headers)")
-from . import _native as native      # noqa: E402  (torch tensors in, the same library underneath)
+_BUILT_FOR = "torch %s, Python %d.%d" % (torch.__version__, *sys.version_info[:2])
+_REBUILD = "_native.so does not fit %s: run `python momoe-impl_b200/build.py`" % _BUILT_FOR
+try:
+    from . import _native as native      # torch tensors in, the same library underneath
+except ImportError as e:
+    raise ImportError(_REBUILD) from e
 
+
+def require_fitting(binding):
+    """A binding of another torch or Python may load and misread its tensors."""
+    built_for = getattr(binding, "built_for", "unknown versions")
+    if built_for != _BUILT_FOR:
+        raise ImportError("%s (it was built for %s)" % (_REBUILD, built_for))
+
+
+require_fitting(native)
 native.bind(LIB_PATH)
 
 c_i32, c_i64, c_vp, c_sz, c_u32 = C.c_int32, C.c_int64, C.c_void_p, C.c_size_t, C.c_uint32
