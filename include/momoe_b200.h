@@ -248,7 +248,7 @@ int momoe_rms_norm_backward(const void* gy, const void* gr, const void* r, int64
                             const float* rstd, int32_t type, int32_t weight_type, int32_t M, int32_t D, void* gx,
                             void* gw, void* workspace, size_t workspace_bytes, momoe_stream_t stream);
 
-/* x [M, D] -> token-major 8-bit rows. */
+/* x [M, D] -> token-major 8-bit rows.  D at most 2^30. */
 int momoe_quantize_rows(const void* x, int64_t x_stride, int32_t type, int32_t M, int32_t D, uint8_t* q, uint8_t* scale,
                         momoe_stream_t stream);
 
@@ -297,7 +297,8 @@ int momoe_fp8_dispatch_rows(const void* x, const uint8_t* x_scale, const int32_t
 /* Up/gate GEMM + SwiGLU on 8-bit operands: a, b = x W1[e]^T (fp32), h = b sigmoid(b) a as 8-bit rows (rounded once, from
  * fp32).  W1 [N, 2H, D], S1 [N, 2, ceil(H / 128), ceil(D / 128)].  The second form streams the weights past a few rows an
  * expert.  tile_rows: the real rows of each tile.  Of the plan they read sched, tile_expert, pair_info (first form) and
- * row_weight (down).  Padding rows of the results are not defined.  D and H multiples of 16. */
+ * row_weight (down).  Padding rows of the results are not defined.  D and H multiples of 16, at most 2^22 (as everywhere in
+ * the 8-bit experts). */
 int momoe_fp8_up_swiglu(const momoe_plan_t* plan, const int32_t* tile_rows, const uint8_t* x_sorted,
                         const uint8_t* x_scale, const uint8_t* W1_N2HD, const uint8_t* S1, uint8_t* h_sorted,
                         uint8_t* h_scale, momoe_stream_t stream);

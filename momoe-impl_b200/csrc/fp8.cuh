@@ -10,6 +10,7 @@ namespace momoe {
 
 constexpr int FP8_BLOCK = 128;          // values that share a scale
 constexpr int FP8_GROUP = 4;            // blocks whose scale bytes share a 32-bit word
+constexpr int FP8_MAX_WIDTH = 1 << 22;  // of expert rows: up to 65535 tiles times column blocks are counted in 32 bits
 constexpr int FP8_ATOM = 512;           // bytes of the scales of 128 rows x 4 blocks
 
 // Scales of expert-major rows lie as the tensor core reads them: 512 bytes for each (128-row tile, 4 blocks of 128

@@ -407,8 +407,8 @@ MOMOE_API int momoe_fp8_quantize_weights(const void* W, int32_t type, int32_t N,
                                          uint8_t* q, uint8_t* S, momoe_stream_t stream) {
     if (W == nullptr || q == nullptr || S == nullptr || N <= 0 || Kd <= 0 || groups <= 0 || C <= 0) return MOMOE_ERR_ARG;
     if ((type != 0 && type != 2) || Kd % 16 != 0) return MOMOE_ERR_UNSUPPORTED;
-    const long long by = static_cast<long long>(groups) * ((C + 127) / 128);
-    if (N > 65535 || by > 65535) return MOMOE_ERR_TOO_LARGE;
+    const long long by = static_cast<long long>(groups) * ((C + 127LL) / 128);
+    if (N > 65535 || by > 65535 || Kd > FP8_MAX_WIDTH) return MOMOE_ERR_TOO_LARGE;
     if ((reinterpret_cast<uintptr_t>(q) & 15) != 0) return MOMOE_ERR_ARG;
     const dim3 grid((Kd + 127) / 128, static_cast<unsigned>(by), N);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -437,7 +437,7 @@ MOMOE_API int momoe_fp8_dispatch_rows(const void* x, const uint8_t* x_scale, con
         return MOMOE_ERR_ARG;
     if (M <= 0 || N <= 0 || K <= 0 || K > N || D <= 0) return MOMOE_ERR_ARG;
     if (D % 16 != 0) return MOMOE_ERR_UNSUPPORTED;
-    if (N > DISPATCH_MAX_EXPERTS || K > DISPATCH_MAX_TOPK) return MOMOE_ERR_TOO_LARGE;
+    if (N > DISPATCH_MAX_EXPERTS || K > DISPATCH_MAX_TOPK || D > FP8_MAX_WIDTH) return MOMOE_ERR_TOO_LARGE;
     // tiles and pairs share a word in the scan
     const int64_t msum = static_cast<int64_t>(M) * K, tiles = (msum + TILE_M - 1) / TILE_M + (msum < N ? msum : N);
     if (tiles > 0xFFFF) return MOMOE_ERR_TOO_LARGE;
@@ -501,6 +501,7 @@ MOMOE_API int momoe_fp8_experts_forward(const void* x_MD, const uint8_t* x_scale
                                         momoe_stream_t stream) {
     if (M <= 0 || N <= 0 || K <= 0 || D <= 0 || H <= 0) return MOMOE_ERR_ARG;
     if (D % 16 != 0 || H % 16 != 0) return MOMOE_ERR_UNSUPPORTED;
+    if (D > FP8_MAX_WIDTH || H > FP8_MAX_WIDTH) return MOMOE_ERR_TOO_LARGE;
     if (x_MD == nullptr || y_MD == nullptr || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
         return MOMOE_ERR_ARG;
     const Fp8Workspace l = fp8_workspace(M, N, K, D, H);

@@ -599,6 +599,7 @@ int fp8_check_plan(const momoe_plan_t* p) {
         return MOMOE_ERR_ARG;
     if (p->M <= 0 || p->N <= 0 || p->K <= 0 || p->D <= 0 || p->H <= 0 || p->rows_capacity <= 0) return MOMOE_ERR_ARG;
     if (p->D % 16 != 0 || p->H % 16 != 0) return MOMOE_ERR_UNSUPPORTED;   // TMA row pitch of 8-bit rows: 16 bytes
+    if (p->D > FP8_MAX_WIDTH || p->H > FP8_MAX_WIDTH) return MOMOE_ERR_TOO_LARGE;
     if (p->rows_capacity % TILE_M != 0) return MOMOE_ERR_ARG;
     return MOMOE_OK;
 }

@@ -23,6 +23,7 @@ namespace momoe {
 
 constexpr int NORM_MAX_THREADS = 512;
 constexpr int NORM_MAX_D = NORM_MAX_THREADS * 4 * 8;
+constexpr int QUANT_MAX_D = 1 << 30;         // column numbers too, with room for the rest of a block
 constexpr int NORM_MAX_M = 1 << 30;          // row numbers stay inside 32 bits, with room for a step past the last row
 
 // How a row of n chunks is shared out: chunks a thread holds, threads of a row, rows of a block.
@@ -457,6 +458,7 @@ MOMOE_API int momoe_quantize_rows(const void* x, int64_t x_stride, int32_t type,
                                   uint8_t* scale, momoe_stream_t stream) {
     if (M < 0 || D <= 0) return MOMOE_ERR_ARG;
     if (type < 0 || type > 2 || D % 8 != 0) return MOMOE_ERR_UNSUPPORTED;
+    if (D > QUANT_MAX_D) return MOMOE_ERR_TOO_LARGE;
     if (M == 0) return MOMOE_OK;
     if (x == nullptr || q == nullptr || scale == nullptr) return MOMOE_ERR_ARG;
     if (x_stride < 0 || x_stride % 8 != 0 || !aligned16(x) || (reinterpret_cast<uintptr_t>(q) & 7) != 0)

@@ -98,7 +98,7 @@ def experts_forward(x, topk_idx_MK, topk_w_MK, experts):
 
     x: bfloat16 [M, D] (converted on the way; other float types are cast to bfloat16 first), or Fp8Rows;
     topk_idx_MK int32 [M, K]: expert ids (one named twice counts with both weights); topk_w_MK float32 [M, K]; experts:
-    Fp8Experts.  D, H multiples of 16, N <= 1024, K <= 32, M K up to 8.2 million.  Returns (y bfloat16 [M, D], tokens_per_expert_N int64 [N]).  The hidden values are converted to
+    Fp8Experts.  D, H multiples of 16 up to 2^22, N <= 1024, K <= 32, M K up to 8.2 million.  Returns (y bfloat16 [M, D], tokens_per_expert_N int64 [N]).  The hidden values are converted to
     8-bit rows once, from 32 bits.  No host synchronisation: an expert id out of range (202) is reported through the
     device's status word like the other problems only the device can see."""
     q, scale = x if isinstance(x, Fp8Rows) else (x, None)
