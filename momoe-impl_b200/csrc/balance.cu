@@ -14,8 +14,9 @@
 // launches for small ones.  Forward, two launches: blocks of rows leave partial sums, one slot for each (row block,
 // sequence) that meet; then the slots of a sequence are added in a fixed order, 32 experts a block, and the last block
 // to finish adds the blocks' shares of the loss, also in a fixed order: no result depends on timing.  At 65521 rows of 256
-// logits in 37 sequences the partial sums take 21 us, their sum 7 and the gradient 26, against 16 us for the bytes alone:
-// a row costs an exponential a logit and two reductions across its lanes in each direction.  At 1024 x 32: 3.7, 5.7, 2.9.
+// logits in 37 sequences the partial sums take 21 us, their sum 7 and the gradient 26, against 16 us for the bytes alone.
+// Of a warp's time the partial sums wait 42 % for loads and 9 % for exchanges between lanes, the gradient 25 % and 14 %: a warp
+// has one set of rows in flight.  At 1024 x 32: 3.7, 5.7, 2.9.
 #include <cmath>
 
 #include "internal.h"
@@ -84,7 +85,7 @@ struct BalRow {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            x[i] = __expf(x[i] - base);
+            x[i] = __expf(x[i] - base);      // 2 + 1.2 |x| units of the last place: 2^-17 at e^-100
             s += x[i];
         }
         s = sum(s);
@@ -504,7 +505,8 @@ MOMOE_API int momoe_balance_loss_backward(const void* logits_MN, int32_t type, c
           reinterpret_cast<uintptr_t>(G_logits_MN) | reinterpret_cast<uintptr_t>(grad_BN)) & 15) != 0)
         return MOMOE_ERR_ARG;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // rows of a warp: four blocks an SM, at least the rows that lie side by side in a warp
+    // rows of a warp: four blocks an SM, at least 8 (up to 32 experts a warp has room for 16, so in small calls half of its
+    // lanes have no row; such a call is a launch's latency)
     int RW = (M + sm_count() * 4 * BAL_WARPS - 1) / (sm_count() * 4 * BAL_WARPS);
     RW = RW < 8 ? 8 : RW;
     const int grid = ((M + RW - 1) / RW + BAL_WARPS - 1) / BAL_WARPS;

@@ -143,6 +143,7 @@ __device__ __forceinline__ bool d8_read_out(const Fp8DecArgs& g, D8Epi& c, const
         uint32_t top;
         if constexpr (UP) {
             const float b = __uint_as_float(rb[t]);
+            // off by some 2^-20 relative, before a rounding to e4m3 (2^-4)
             v[t] = b * __fdividef(1.0f, 1.0f + __expf(-b)) * __uint_as_float(r[t]);
             top = __reduce_max_sync(0xffffffffu, abs_bits(v[t]));
         } else {
@@ -442,8 +443,8 @@ static int d8_launch(const CUtensorMap& tmW, const CUtensorMap& tmX, const Fp8De
 }
 
 // Whether two CTAs share an item's k axis: when the items leave half of the SMs idle, and the k axis is long enough to pay
-// for the meeting.  Whole passes of one token, with the up GEMM shared and not: 18.5 / 18.3 us at 8 k slices, 20.5 / 20.4 at
-// 12, 20.6 / 22.4 at 16, 26.2 / 28.7 at 32 (H512, top-4 of 32), 39.0 / 47.0 at 56 (top-8 of 64).
+// for the meeting.  Whole passes of one token, with the up GEMM shared and not: 20.4 / 18.5 us at 8 k slices, 20.5 / 20.2 at
+// 12, 21.4 / 22.4 at 16, 24.6 / 28.7 at 32 (H512, top-4 of 32), 37.0 / 45.2 at 56 (top-8 of 64).
 static bool d8_split(const momoe_plan_t* p, const Fp8DecArgs& g) {
     const long long msum = static_cast<long long>(p->M) * p->K;
     const long long tiles = msum / TILE_M + (msum < p->N ? msum : p->N);      // an upper bound

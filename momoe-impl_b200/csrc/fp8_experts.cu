@@ -12,7 +12,8 @@ __device__ __forceinline__ float f8_value(__nv_bfloat16 v) { return __bfloat162f
 
 // W [N, Kd, G * C] -> q [N, G * C, Kd] (k contiguous, as the MMA reads it) and one scale for each 128 x 128 block
 // [N, G, ceil(C / 128), ceil(Kd / 128)].  A block of columns never crosses a group (the linear and the gate half of the
-// up projection).  Runs once when a model is loaded; bound by HBM, one read and one write of the weights.
+// up projection).  Runs once when a model is loaded; the weights are read twice, once for the maximum of a block and once for
+// its codes, and written once.
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_quantize_weights_kernel(const T* __restrict__ W, int Kd, int G, int C,
                                                                    uint8_t* __restrict__ q, uint8_t* __restrict__ S) {

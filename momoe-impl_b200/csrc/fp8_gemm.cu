@@ -8,7 +8,7 @@
 // no per-block pass over the accumulators, which fp32 scales would need.
 //
 // Bound at large row counts by the tensor pipe at the clock that the power limit leaves and by the tiles' way out of L2, 10
-// TB/s at 16384 tokens (D2048 H1024, top-8 of 128: up 2.3, down 1.9 PFLOP/s).  The structure is that of the 16-bit grouped
+// TB/s at 16384 tokens (D2048 H1024, top-8 of 128: up 2.2, down 1.8 PFLOP/s).  The structure is that of the 16-bit grouped
 // GEMM: a CTA pair computes 256 x 256, each CTA loads its 128 rows of A and half of B, ring of 3 stages of two 128-byte k
 // slices (a slice is 128 values here), warp 0 loads, warp 1 of the leader issues the MMAs, warps 2..9 are the epilogue.
 //
@@ -84,6 +84,7 @@ __device__ __forceinline__ uint32_t f8_pack_f16(float lo, float hi) {
     const __half2 p = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&p);
 }
+// The short exponential and division are off by some 2^-20 relative; the value is rounded to e4m3 (2^-4) next.
 __device__ __forceinline__ float f8_swiglu(float a, float b) { return b * __fdividef(1.0f, 1.0f + __expf(-b)) * a; }
 
 struct Fp8Work {
@@ -585,9 +586,9 @@ static int f8_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUten
 
 // Whether a CTA works on a tile of its own: up to F8_SINGLE_ROWS rows an expert on average.  Whole passes in us, on tiles of
 // their own and in pairs:  rows an expert       48          128          192          256          384
-//   D2176 H1152, top-6 of 64                113 / 130    142 / 156    190 / 199    233 / 219    325 / 277
-//   D2048 H1024, top-8 of 128               178 / 237    221 / 250    289 / 292    376 / 375    507 / 450
-//   D7168 H2048, top-4 of 32                265 / 319    365 / 418    480 / 458    578 / 600    810 / 683
+//   D2176 H1152, top-6 of 64                115 / 132    138 / 163    177 / 194    219 / 220    299 / 291
+//   D2048 H1024, top-8 of 128               173 / 215    227 / 266    298 / 313    353 / 380    497 / 468
+//   D7168 H2048, top-4 of 32                262 / 338    358 / 400    473 / 460    566 / 528    773 / 695
 constexpr long long F8_SINGLE_ROWS = 192;
 static bool f8_single(const momoe_plan_t* p) {
     return static_cast<long long>(p->M) * p->K <= F8_SINGLE_ROWS * static_cast<long long>(p->N);

@@ -1,5 +1,6 @@
 """The experts' forward pass in 8-bit floating point: e4m3 rows and weights with a power of two (e8m0) for each block of
-128, multiplied on the tensor cores with 32-bit accumulation.  Forward only; weights take half the memory of bfloat16.
+128, multiplied on the tensor cores with 32-bit accumulation.  Forward only.  `Fp8Experts` takes half the memory of bfloat16
+weights and needs nothing else; a `MoE` layer keeps its 16-bit weights beside it.
 
     experts = quantize_experts(moe.momoe.Wl1_ND2H, moe.momoe.Wl2_NHD)       # once, when the weights are final
     y_MD, tokens_per_expert_N = experts_forward(x_MD, topk_idx_MK, topk_w_MK, experts)
@@ -14,8 +15,8 @@ from ._lib import as_rows, lib, native, on_device, pitch, ptr, raw_stream
 
 BLOCK = 128                      # values that share a scale
 # Calls with at most this many rows per expert on average stream the weights past the rows; more take the row-tile kernels.
-# Whole passes, streaming against tiles: one token 24.7 / 26.7 us, 1 row an expert 86 / 90, 4 rows 125 / 127, 8 rows 131.5 /
-# 131.9, 12 rows 151 / 145, 24 rows 166 / 154 (D2048 H1024, top-8 of 128).
+# Whole passes, streaming against tiles: one token 26.0 / 30.0 us, 1 row an expert 87 / 91.5, 4 rows 130 / 133.5, 8 rows 142.5 /
+# 145, 12 rows 147.6 / 148.5, 24 rows 167 / 155 (D2048 H1024, top-8 of 128).
 STREAM_MAX_AVG_ROWS = 8
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
@@ -98,8 +99,8 @@ def experts_forward(x, topk_idx_MK, topk_w_MK, experts):
 
     x: bfloat16 [M, D] (converted on the way; other float types are cast to bfloat16 first), or Fp8Rows;
     topk_idx_MK int32 [M, K]: expert ids (one named twice counts with both weights); topk_w_MK float32 [M, K]; experts:
-    Fp8Experts.  D, H multiples of 16 up to 2^22, N <= 1024, K <= 32, M K up to 8.2 million.  Returns (y bfloat16 [M, D], tokens_per_expert_N int64 [N]).  The hidden values are converted to
-    8-bit rows once, from 32 bits.  No host synchronisation: an expert id out of range (202) is reported through the
+    Fp8Experts.  D, H multiples of 16 up to 2^22, N <= 1024, K <= 32, M K up to 8.2 million.  Returns (y bfloat16 [M, D],
+    tokens_per_expert_N int64 [N]).  The hidden values are converted to 8-bit rows once, from 32 bits.  No host synchronisation: an expert id out of range (202) is reported through the
     device's status word like the other problems only the device can see."""
     q, scale = x if isinstance(x, Fp8Rows) else (x, None)
     _lib.require_cuda(q)

@@ -151,7 +151,8 @@ class MoE(nn.Module):
 
     def quantize_experts(self):
         """From now on forward passes use an 8-bit copy of the expert weights as they are now.  Such passes have no
-        backward: they run under torch.no_grad() (or with nothing that requires a gradient).  When the weights have
+        backward: they run under torch.no_grad() (or with nothing that requires a gradient).  The copy is held beside the
+        16-bit weights, is no part of state_dict() and does not follow `.to()`.  When the weights have
         changed since (in place or by other ones; changes through `.data`, and in-place changes of tensors made in inference
         mode, are not seen), forward raises; call this again, or set `experts_fp8 = None` to go back to 16 bits."""
         self.experts_fp8 = fp8.quantize_experts(self.momoe.Wl1_ND2H, self.momoe.Wl2_NHD)
