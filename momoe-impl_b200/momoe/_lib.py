@@ -1,7 +1,8 @@
 """ctypes binding of libmomoe_b200.so (the C ABI declared in include/momoe_b200.h), and the compiled binding `native` of
 the operators around the expert layer (csrc/binding.cpp), whose calls are too short for Python on the way.
 
-There is no fallback: if the library is missing, importing this module raises with the build command.
+There is no fallback: if the library is missing, importing this module raises with the build command, and so does the first
+use of the binding if that is missing.
 """
 import contextlib
 import ctypes as C
@@ -20,25 +21,38 @@ if not os.path.exists(LIB_PATH):
 
 lib = C.CDLL(LIB_PATH)
 
-if not os.path.exists(os.path.join(_HERE, "_native.so")):
-    raise ImportError("_native.so is not built; run `python momoe-impl_b200/build.py` (needs g++ and torch's headers)")
 _BUILT_FOR = "torch %s, Python %d.%d" % (torch.__version__, *sys.version_info[:2])
-_REBUILD = "_native.so does not fit %s: run `python momoe-impl_b200/build.py`" % _BUILT_FOR
-try:
-    from . import _native as native      # torch tensors in, the same library underneath
-except ImportError as e:
-    raise ImportError(_REBUILD) from e
 
 
 def require_fitting(binding):
     """A binding of another torch or Python may load and misread its tensors."""
     built_for = getattr(binding, "built_for", "unknown versions")
     if built_for != _BUILT_FOR:
-        raise ImportError("%s (it was built for %s)" % (_REBUILD, built_for))
+        raise ImportError("_native.so was built for %s, not for %s: run `python momoe-impl_b200/build.py`"
+                          % (built_for, _BUILT_FOR))
 
 
-require_fitting(native)
-native.bind(LIB_PATH)
+class _Native:
+    """The compiled binding: torch tensors in, the same library underneath.  Loaded when first used, since the layer in 16
+    bits does without it."""
+
+    def __getattr__(self, name):
+        try:
+            from . import _native
+        except ImportError as e:
+            raise ImportError("_native.so is not built or does not fit %s: run `python momoe-impl_b200/build.py` (needs g++ "
+                              "and torch's headers)" % _BUILT_FOR) from e
+        require_fitting(_native)
+        _native.bind(LIB_PATH)
+        self.__dict__.update({k: v for k, v in vars(_native).items() if k not in ("__class__", "__dict__")})
+        return getattr(_native, name)
+
+    def launches(self):
+        """Kernels queued through it; replaced by its own count once it is loaded."""
+        return 0
+
+
+native = _Native()
 
 c_i32, c_i64, c_vp, c_sz, c_u32 = C.c_int32, C.c_int64, C.c_void_p, C.c_size_t, C.c_uint32
 

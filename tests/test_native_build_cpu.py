@@ -35,3 +35,40 @@ def test_binding_of_other_versions_is_not_loaded(build):
     for other in (types.SimpleNamespace(built_for="torch 1.0, Python 3.8"), types.SimpleNamespace()):
         with pytest.raises(ImportError, match="build.py"):
             _lib.require_fitting(other)
+
+
+def test_package_without_the_binding(build, tmp_path):
+    """The layer in 16 bits does not need it; the operators that do name the build command."""
+    import subprocess
+    import sys
+    home = tmp_path / "momoe"
+    shutil.copytree(os.path.dirname(build.LIB_PATH), home, ignore=shutil.ignore_patterns("*.so", "__pycache__"))
+    os.symlink(build.LIB_PATH, home / "libmomoe_b200.so")
+    code = """
+import torch, momoe, momoe.norm, momoe.balance, momoe.fp8
+from momoe import _lib, ops
+assert ops.launch_count() == 0
+for use in (lambda: momoe.norm.rms_norm(torch.zeros(2, 8), torch.ones(8)), lambda: _lib.native.bind):
+    for _ in range(2):
+        try:
+            use()
+        except ImportError as e:
+            assert "build.py" in str(e), e
+        else:
+            raise AssertionError
+"""
+    got = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=str(tmp_path)), capture_output=True, text=True)
+    assert got.returncode == 0, got.stderr
+    shutil.copy(build.BINDING_PATH, home / "_native.so")
+    code = """
+import torch, momoe.norm
+from momoe import _lib, ops
+assert ops.launch_count() == 0
+try:
+    momoe.norm.rms_norm(torch.zeros(2, 8), torch.ones(8))
+except RuntimeError as e:
+    assert "no CPU path" in str(e), e
+assert ops.launch_count() == 0 and "launches" in vars(_lib.native) and _lib.native.__file__.endswith("_native.so")
+"""
+    got = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=str(tmp_path)), capture_output=True, text=True)
+    assert got.returncode == 0, got.stderr
