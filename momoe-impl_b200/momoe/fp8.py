@@ -47,7 +47,7 @@ def _blocks(n):
 def quantize_rows(x):
     """x [..., D] (bfloat16, float16 or float32; D a multiple of 8) -> Fp8Rows of the [M, D] view.  The scale of a block
     is the smallest power of two that brings its largest magnitude to 448 at most (1 for a block of zeros, NaN for a block
-    that holds an infinity or a NaN), so only the conversion to e4m3 rounds."""
+    that holds an infinity or a NaN), so only the conversion to e4m3 rounds.  x is taken as a constant: no gradient passes."""
     _lib.require_cuda(x)
     if x.dtype not in _lib.TYPES:
         raise RuntimeError("quantize_rows works on bfloat16, float16 or float32, but got: %s" % x.dtype)
@@ -77,7 +77,7 @@ def _quantize_weights(W, groups):
 
 
 def quantize_experts(Wl1_ND2H, Wl2_NHD):
-    """Up/gate weights [N, D, 2H] and down weights [N, H, D], as `MoMoE` holds them -> Fp8Experts."""
+    """Up/gate weights [N, D, 2H] and down weights [N, H, D], as `MoMoE` holds them -> Fp8Experts.  No gradient passes."""
     dev = _lib.require_one_device(Wl1_ND2H, Wl2_NHD)
     if Wl1_ND2H.dim() != 3 or Wl2_NHD.dim() != 3:
         raise RuntimeError("expert weights must be [N, D, 2H] and [N, H, D], but got: %s and %s"
