@@ -98,12 +98,22 @@ def _version(w):
     return None if w.is_inference() else w._version
 
 
+def _refs(tensors):
+    return tuple(weakref.ref(t) for t in tensors)
+
+
+def _same(refs, tensors):
+    return all(ref() is t for ref, t in zip(refs, tensors))
+
+
 class MoE(nn.Module):
     balance_coef = 0.0     # weight of the balance loss (each of a batch's sequences on its own)
     z_coef = 0.0           # weight of the z-loss
     aux_loss = None        # their sum of the latest forward pass, float32 [], differentiable; None if both are 0
     experts_fp8 = None     # 8-bit weights of forward-only calls, from quantize_experts()
-    _fp8_weights = None    # (experts_fp8, the weights that it stands for with their versions); no weights: none of this layer's
+    # (tensors of experts_fp8, the weights that they stand for with their versions), by weak references; no weights: none of
+    # this layer's.  In a saved state (): those, else None.
+    _fp8_weights = None
 
     def __init__(self, embedding_dim, intermediate_dim, num_experts, num_chosen_experts, num_shared_experts,
                  save_percent=0, bias_update_rate=1e-4, Wg_DN: torch.Tensor | None = None,
@@ -132,20 +142,22 @@ class MoE(nn.Module):
         state = dict(self.__dict__)
         state.pop("aux_loss", None)         # belongs to the graph of a forward pass, not to a copy of the layer
         # a copy has weights of its own, for which its 8-bit ones stand if they stand for this layer's
-        state["_fp8_weights"] = None if self.experts_fp8 is None or self._fp8_fresh() else (self.experts_fp8, ())
+        state["_fp8_weights"] = None if self.experts_fp8 is None or self._fp8_fresh() else ()
         return state
 
     def __setstate__(self, state):
         super().__setstate__(state)
         if self.experts_fp8 is not None:
+            if self._fp8_weights == ():
+                self._fp8_weights = _refs(self.experts_fp8), ()
             self._fp8_fresh()
 
     def _fp8_fresh(self):
         """Whether the 8-bit weights stand for the layer's weights as they are; ones that were set by hand do from the first
         look on."""
         weights = self.momoe.Wl1_ND2H, self.momoe.Wl2_NHD
-        if self._fp8_weights is None or self._fp8_weights[0] is not self.experts_fp8:
-            self._fp8_weights = self.experts_fp8, tuple((weakref.ref(w), _version(w)) for w in weights)
+        if self._fp8_weights is None or not _same(self._fp8_weights[0], self.experts_fp8):
+            self._fp8_weights = _refs(self.experts_fp8), tuple(zip(_refs(weights), map(_version, weights)))
         seen = self._fp8_weights[1]
         return len(seen) == 2 and all(ref() is w and version == _version(w) for (ref, version), w in zip(seen, weights))
 

@@ -183,3 +183,33 @@ def test_eight_bit_weights_set_by_hand_after_others(momoe):
         moe.momoe.Wl1_ND2H.mul_(2)
         with pytest.raises(RuntimeError, match="changed"):
             moe(x)
+
+
+def test_stale_eight_bit_weights_in_a_saved_state(momoe):
+    x = torch.randn(1, 5, 64, device="cuda").bfloat16()
+    with torch.no_grad():
+        moe = momoe.MoE(64, 32, 4, 2, 0)
+        moe.quantize_experts()
+        state = dict(moe.__getstate__(), _fp8_weights=())
+        moe.__setstate__(state)
+        with pytest.raises(RuntimeError, match="changed"):
+            moe(x)
+        moe.quantize_experts()
+        moe(x)
+
+
+def test_eight_bit_weights_are_freed_when_they_are_given_up(momoe):
+    with torch.no_grad():
+        moe = momoe.MoE(256, 128, 16, 2, 0)
+        x = torch.randn(1, 5, 256, device="cuda").bfloat16()
+        moe(x)
+        before = torch.cuda.memory_allocated()
+        moe.quantize_experts()
+        moe(x)
+        size = sum(t.numel() for t in moe.experts_fp8)
+        assert torch.cuda.memory_allocated() >= before + size
+        moe.quantize_experts()
+        moe(x)
+        assert torch.cuda.memory_allocated() < before + 2 * size
+        moe.experts_fp8 = None
+        assert torch.cuda.memory_allocated() < before + size
